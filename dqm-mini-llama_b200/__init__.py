@@ -15,8 +15,8 @@ from typing import Optional, Sequence
 import numpy as np
 
 from . import synth
-from ._lib import (F32, Q40, Q41, Q80, CudaError, ModelConfig, ModelStats, OutOfRange, TpPlan,
-                   build, check, lib)
+from ._lib import (F32, Q40, Q41, Q80, CudaError, KvQ40, ModelConfig, ModelStats, OutOfRange,
+                   TpPlan, build, check, lib)
 
 __all__ = [
     "F32", "Q80", "Q40", "Q41", "OutOfRange", "CudaError", "build", "lib", "synth",
@@ -27,6 +27,7 @@ __all__ = [
     "embedding_lookup_blocks", "argmax", "CudaKvCache", "CudaAttentionDecodeDeviceInput",
     "Model", "Context", "Batch", "BLOCK_BYTES", "linear_batch_packed", "linear_cols_packed",
     "CudaQ41Linear", "CudaQ41LinearDeviceInput", "CudaLinear", "CudaLinearDeviceInput",
+    "qk_norm_rope", "attention_prompt", "KvCacheQ40",
 ]
 
 BLOCK_BYTES = {Q80: 34, Q40: 18, Q41: 20}
@@ -329,6 +330,208 @@ def CudaAttentionDecodeDeviceInput(q, kv: CudaKvCache, layer: int, pos: int, n_h
                                       kv.max_seq_len, n_kv_heads, head_dim, layer, pos, n_heads,
                                       _ptr(out), _stream()))
     return out
+
+
+# ------------------------------------------------------------ attention block
+class _on:
+    """The device of `tensor` and the stream of a call (None: torch's current
+    stream of that device) made current, so that outputs and workspaces are
+    allocated for the stream that uses them."""
+
+    def __init__(self, tensor, stream):
+        torch = _torch()
+        if stream is not None and not isinstance(stream, torch.cuda.Stream):
+            stream = torch.cuda.ExternalStream(stream, device=tensor.device)
+        if stream is not None and stream.device != tensor.device:
+            raise RuntimeError("stream and tensors are on different devices")
+        self.guards = (torch.cuda.device(tensor.device), torch.cuda.stream(stream))
+
+    def __enter__(self):
+        for g in self.guards:
+            g.__enter__()
+        return _torch().cuda.current_stream().cuda_stream
+
+    def __exit__(self, *exc):
+        for g in reversed(self.guards):
+            g.__exit__(*exc)
+
+
+def _check_tensor(api: str, name: str, t, shape, device, dtype=None):
+    """A CUDA tensor of this shape and type on this device, with contiguous
+    rows: everything but the first dimension's stride is fixed."""
+    torch = _torch()
+    dtype = dtype or torch.float32
+    if not isinstance(t, torch.Tensor) or not t.is_cuda or t.device != device:
+        raise RuntimeError(f"{api}: {name} must be a tensor on {device}")
+    if t.dtype != dtype:
+        raise RuntimeError(f"{api}: {name} must be {dtype}, is {t.dtype}")
+    if tuple(t.shape) != tuple(shape):
+        raise RuntimeError(f"{api}: {name} must have shape {tuple(shape)}, has {tuple(t.shape)}")
+    step = 1
+    for dim in range(t.dim() - 1, 0, -1):
+        if t.shape[dim] != 1 and t.stride(dim) != step:
+            raise RuntimeError(f"{api}: the rows of {name} must be contiguous")
+        step *= t.shape[dim]
+    if t.dim() == 1 and t.shape[0] > 1 and t.stride(0) != 1:
+        raise RuntimeError(f"{api}: {name} must be contiguous")
+
+
+def _check_device(api: str, t, dims: int, name: str):
+    torch = _torch()
+    if not isinstance(t, torch.Tensor) or not t.is_cuda or t.dim() != dims:
+        raise RuntimeError(f"{api}: {name} must be a {dims}-dimensional CUDA tensor")
+
+
+def _ld(t) -> int:
+    """Elements from one row to the next."""
+    row = int(np.prod(t.shape[1:]))
+    return t.stride(0) if t.shape[0] > 1 else row
+
+
+def qk_norm_rope(q, k, q_norm, k_norm, positions, theta: float, eps: float, neox: bool = True,
+                 q_out=None, k_out=None, stream=None):
+    """RMSNorm of every head of q [tokens, n_heads, head_dim] and k [tokens,
+    n_kv_heads, head_dim] and the rotary rotation at the tokens' positions
+    (int32, on the device), in one pass.  Heads may be views into wider rows.
+    q_out / k_out may be q / k (in place); by default new tensors.  Returns
+    (q_out, k_out)."""
+    torch = _torch()
+    api = "QkNormRope"
+    _check_device(api, q, 3, "q")
+    n, heads, dim = q.shape
+    _check_device(api, k, 3, "k")
+    kv = k.shape[1]
+    dev = q.device
+    _check_tensor(api, "q", q, (n, heads, dim), dev)
+    _check_tensor(api, "k", k, (n, kv, dim), dev)
+    _check_tensor(api, "q_norm", q_norm, (dim,), dev)
+    _check_tensor(api, "k_norm", k_norm, (dim,), dev)
+    _check_tensor(api, "positions", positions, (n,), dev, torch.int32)
+    with _on(q, stream) as s:
+        q_out = torch.empty((n, heads, dim), device=dev) if q_out is None else q_out
+        k_out = torch.empty((n, kv, dim), device=dev) if k_out is None else k_out
+        _check_tensor(api, "q_out", q_out, q.shape, dev)
+        _check_tensor(api, "k_out", k_out, k.shape, dev)
+        check(lib().dqmk_qk_norm_rope(
+            _ptr(q), _ld(q), _ptr(k), _ld(k), n, heads, kv, dim, _ptr(q_norm), _ptr(k_norm),
+            float(eps), _ptr(positions), float(theta), 1 if neox else 0, _ptr(q_out), _ld(q_out),
+            _ptr(k_out), _ld(k_out), s))
+    return q_out, k_out
+
+
+def attention_prompt(q, k, v, starts, out=None, stream=None):
+    """Causal attention over packed prompts: q [tokens, n_heads, head_dim], k
+    and v [tokens, n_kv_heads, head_dim], starts int32 [sequences + 1] on the
+    device, sequence s = tokens starts[s] .. starts[s+1]-1.  Rows of `out`
+    outside every sequence are left as they were (a new `out` is zero there)."""
+    torch = _torch()
+    api = "AttentionPrompt"
+    _check_device(api, q, 3, "q")
+    n, heads, dim = q.shape
+    _check_device(api, k, 3, "k")
+    kv = k.shape[1]
+    dev = q.device
+    _check_device(api, starts, 1, "starts")
+    seqs = starts.shape[0] - 1
+    if seqs < 0:
+        raise RuntimeError(f"{api}: starts must hold at least one offset")
+    _check_tensor(api, "q", q, (n, heads, dim), dev)
+    _check_tensor(api, "k", k, (n, kv, dim), dev)
+    _check_tensor(api, "v", v, (n, kv, dim), dev)
+    _check_tensor(api, "starts", starts, (seqs + 1,), dev, torch.int32)
+    with _on(q, stream) as s:
+        out = torch.zeros((n, heads, dim), device=dev) if out is None else out
+        _check_tensor(api, "out", out, q.shape, dev)
+        nbytes = lib().dqmk_attention_prompt_workspace(n, seqs, heads, kv, dim)
+        work = torch.empty(nbytes, dtype=torch.uint8, device=dev)
+        check(lib().dqmk_attention_prompt(
+            _ptr(q), _ld(q), _ptr(k), _ld(k), _ptr(v), _ld(v), _ptr(starts), seqs, n, heads, kv,
+            dim, _ptr(out), _ld(out), _ptr(work), nbytes, s))
+    return out
+
+
+class KvCacheQ40:
+    """A KV cache held in 4 bits (dqmk_kv_q40): n_slots sequences of up to
+    max_seq positions for each layer, rows quantized to Q4_0 blocks as they
+    are written."""
+
+    def __init__(self, n_layers: int, n_slots: int, max_seq: int, n_kv_heads: int, head_dim: int,
+                 device="cuda"):
+        torch = _torch()
+        self.n_layers, self.n_slots, self.max_seq = int(n_layers), int(n_slots), int(max_seq)
+        self.n_kv_heads, self.head_dim = int(n_kv_heads), int(head_dim)
+        nbytes = lib().dqmk_kv_q40_bytes(self.n_layers, self.n_slots, self.max_seq,
+                                         self.n_kv_heads, self.head_dim)
+        if nbytes == 0:
+            raise RuntimeError("KvCacheQ40: unsupported shape (head_dim must be a multiple of 32 "
+                               "of at most 128, every count positive)")
+        self.keys = torch.zeros(nbytes, dtype=torch.uint8, device=device)
+        self.values = torch.zeros(nbytes, dtype=torch.uint8, device=device)
+        self._c = KvQ40(_ptr(self.keys), _ptr(self.values), self.n_layers, self.n_slots,
+                        self.max_seq, self.n_kv_heads, self.head_dim)
+
+    def _index(self, api, positions, slots, n):
+        torch = _torch()
+        _check_tensor(api, "positions", positions, (n,), self.keys.device, torch.int32)
+        if slots is not None:
+            _check_tensor(api, "slots", slots, (n,), self.keys.device, torch.int32)
+
+    def write(self, layer: int, k, v, positions, slots=None, stream=None) -> None:
+        """Rows k, v [tokens, n_kv_heads, head_dim] to positions [tokens] of
+        slots [tokens] (None: slot t for token t); position -1 stores nothing."""
+        api = "KvQ40Write"
+        _check_device(api, k, 3, "k")
+        n = k.shape[0]
+        for name, t in (("k", k), ("v", v)):
+            _check_tensor(api, name, t, (n, self.n_kv_heads, self.head_dim), self.keys.device)
+        self._index(api, positions, slots, n)
+        with _on(self.keys, stream) as s:
+            check(lib().dqmk_kv_q40_write(C.byref(self._c), layer, _ptr(k), _ld(k), _ptr(v), _ld(v),
+                                          _ptr(slots), _ptr(positions), n, s))
+
+    def read(self, layer: int, positions, slots=None, k_out=None, v_out=None, stream=None):
+        """The values held at those rows, as (k, v) [tokens, n_kv_heads,
+        head_dim]; rows of position -1 are left as they were (zero in new
+        tensors)."""
+        torch = _torch()
+        api = "KvQ40Read"
+        _check_device(api, positions, 1, "positions")
+        n = positions.shape[0]
+        self._index(api, positions, slots, n)
+        shape = (n, self.n_kv_heads, self.head_dim)
+        dev = self.keys.device
+        with _on(self.keys, stream) as s:
+            k_out = torch.zeros(shape, device=dev) if k_out is None else k_out
+            v_out = torch.zeros(shape, device=dev) if v_out is None else v_out
+            _check_tensor(api, "k_out", k_out, shape, dev)
+            _check_tensor(api, "v_out", v_out, shape, dev)
+            check(lib().dqmk_kv_q40_read(C.byref(self._c), layer, _ptr(slots), _ptr(positions), n,
+                                         _ptr(k_out), _ld(k_out), _ptr(v_out), _ld(v_out), s))
+        return k_out, v_out
+
+    def attention(self, q, layer: int, lengths, slots=None, out=None, stream=None):
+        """Decode attention: q [columns, n_heads, head_dim], column c over the
+        first lengths[c] positions of slots[c] (None: slot c); int32 tensors on
+        the device.  Length 0 gives zeros.  Returns out [columns, n_heads,
+        head_dim]."""
+        torch = _torch()
+        api = "KvQ40Attention"
+        _check_device(api, q, 3, "q")
+        n, heads, _ = q.shape
+        dev = self.keys.device
+        _check_tensor(api, "q", q, (n, heads, self.head_dim), dev)
+        _check_tensor(api, "lengths", lengths, (n,), dev, torch.int32)
+        if slots is not None:
+            _check_tensor(api, "slots", slots, (n,), dev, torch.int32)
+        with _on(self.keys, stream) as s:
+            out = torch.empty(q.shape, device=dev) if out is None else out
+            _check_tensor(api, "out", out, q.shape, dev)
+            nbytes = lib().dqmk_kv_q40_attention_workspace(C.byref(self._c), n, heads)
+            work = torch.empty(nbytes, dtype=torch.uint8, device=dev)
+            check(lib().dqmk_kv_q40_attention(
+                C.byref(self._c), layer, _ptr(q), _ld(q), _ptr(slots), _ptr(lengths), n, heads,
+                _ptr(out), _ld(out), _ptr(work), nbytes, s))
+        return out
 
 
 # ------------------------------------------------------------ engine

@@ -49,6 +49,14 @@ class TpPlan(C.Structure):
                                          "vocab_stride")]
 
 
+class KvQ40(C.Structure):
+    """dqmk_kv_q40: the buffers and shape of a 4-bit KV cache."""
+    _fields_ = [("keys_dev", _vp), ("values_dev", _vp), ("n_layers", _i), ("n_slots", _i),
+                ("max_seq", _i), ("n_kv_heads", _i), ("head_dim", _i)]
+
+
+_kvp = C.POINTER(KvQ40)
+
 SIGNATURES = {
     "dqmk_last_error": ([], C.c_char_p),
     "dqmk_built": ([], _i),
@@ -86,6 +94,17 @@ SIGNATURES = {
     "dqmk_kv_write": ([_vp, _vp, _i, _i, _i, _i, _i, _i, _vp, _vp, _vp], _i),
     "dqmk_attention_decode": ([_vp, _vp, _vp, _i, _i, _i, _i, _i, _i, _i, _vp, _vp], _i),
     "dqmk_attention_decode_noalloc": ([_vp, _vp, _vp, _i, _i, _i, _i, _i, _i, _i, _vp, _vp], _i),
+    "dqmk_qk_norm_rope": ([_vp, _i64, _vp, _i64, _i, _i, _i, _i, _vp, _vp, _f, _vp, _f, _i, _vp,
+                           _i64, _vp, _i64, _vp], _i),
+    "dqmk_attention_prompt_workspace": ([_i, _i, _i, _i, _i], _sz),
+    "dqmk_attention_prompt": ([_vp, _i64, _vp, _i64, _vp, _i64, _vp, _i, _i, _i, _i, _i, _vp, _i64,
+                               _vp, _sz, _vp], _i),
+    "dqmk_kv_q40_bytes": ([_i, _i, _i, _i, _i], _sz),
+    "dqmk_kv_q40_write": ([_kvp, _i, _vp, _i64, _vp, _i64, _vp, _vp, _i, _vp], _i),
+    "dqmk_kv_q40_read": ([_kvp, _i, _vp, _vp, _i, _vp, _i64, _vp, _i64, _vp], _i),
+    "dqmk_kv_q40_attention_workspace": ([_kvp, _i, _i], _sz),
+    "dqmk_kv_q40_attention": ([_kvp, _i, _vp, _i64, _vp, _vp, _i, _i, _vp, _i64, _vp, _sz, _vp],
+                              _i),
     "dqmk_model_create": ([C.POINTER(ModelConfig), _i, C.POINTER(_vp)], _i),
     "dqmk_model_destroy": ([_vp], _i),
     "dqmk_model_upload": ([_vp, C.c_char_p, _i, _vp, _sz, _i, _i], _i),

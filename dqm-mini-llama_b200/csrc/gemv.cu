@@ -1965,12 +1965,15 @@ extern "C" int dqmk_gemv_packed_chained(int qtype, const float* x, int in_featur
 
 extern "C" int dqmk_device_error(int clear) {
   unsigned int flags = 0, prefill_flags = 0, tp_flags = 0, ops_flags = 0, batch_flags = 0;
+  unsigned int kv_flags = 0, prompt_flags = 0;
   cudaError_t e = read_device_error(&flags, clear != 0);
   if (e == cudaSuccess) e = read_prefill_error(&prefill_flags, clear != 0);
   if (e == cudaSuccess) e = read_tp_error(&tp_flags, clear != 0);
   if (e == cudaSuccess) e = read_ops_error(&ops_flags, clear != 0);
   if (e == cudaSuccess) e = read_batch_error(&batch_flags, clear != 0);
-  flags |= prefill_flags | tp_flags | ops_flags | batch_flags;
+  if (e == cudaSuccess) e = read_kv_error(&kv_flags, clear != 0);
+  if (e == cudaSuccess) e = read_prompt_error(&prompt_flags, clear != 0);
+  flags |= prefill_flags | tp_flags | ops_flags | batch_flags | kv_flags | prompt_flags;
   if (e != cudaSuccess) {
     cuda_fail("dqmk_device_error", e);
     return -1;

@@ -57,6 +57,7 @@ class DeviceOnce {
 constexpr unsigned int kErrTimeout = 1u;   // a bounded wait ran out
 constexpr unsigned int kErrNoToken = 2u;   // greedy step without a valid argmax (state kept)
 constexpr unsigned int kErrBadToken = 4u;  // embedding of a token id outside [0, vocab)
+constexpr unsigned int kErrBadIndex = 8u;  // a slot, position, length or offset out of range
 // DQMK_OK when no flag is set, else DQMK_ERR_TIMEOUT with a message prefixed
 // by `api` that names what the flags record.
 int device_flags_status(const char* api, unsigned int flags);
@@ -209,6 +210,10 @@ cudaError_t launch_tp_argmax_advance(const PeerSet& ps, const unsigned long long
 cudaError_t read_tp_error(unsigned int* flags, bool clear);
 // Multi-sequence decode GEMM (batch.cu): bounded-wait flag.
 cudaError_t read_batch_error(unsigned int* flags, bool clear);
+// 4-bit KV cache (kv_q40.cu) and packed prompt attention (attention_prompt.cu):
+// bounded waits and device-side indices out of range.
+cudaError_t read_kv_error(unsigned int* flags, bool clear);
+cudaError_t read_prompt_error(unsigned int* flags, bool clear);
 cudaError_t launch_greedy_advance(const unsigned long long* slot, int* token, int* pos,
                                   int* history, int cap, int vocab, cudaStream_t s);
 cudaError_t launch_kv_write(float* keys, float* values, int max_seq, int n_kv_heads,

@@ -170,7 +170,8 @@ int dqmk_linear_cols_packed(int qtype, const float* x_dev, int cols, int in_feat
 /* Failure detection.  Kernels that wait on asynchronous copies bound every
  * wait (about one second); a wait that runs out records a flag in device
  * memory and the kernel exits instead of hanging.  dqmk_device_error returns
- * the flags (bit 0: a bounded wait timed out; -1 if the read itself failed)
+ * the flags (bit 0: a bounded wait timed out; bit 3: a slot, position, length
+ * or offset outside its range was skipped; -1 if the read itself failed)
  * and clears them when `clear` != 0.  The engine's synchronous calls check
  * the flag and return DQMK_ERR_TIMEOUT.  No reference counterpart: the
  * reference has no device-side waits. */
@@ -286,6 +287,100 @@ int dqmk_attention_decode_noalloc(const float* q_dev, const float* keys_dev,
                                   const float* values_dev, int n_layers, int max_seq,
                                   int n_kv_heads, int head_dim, int layer, int pos, int n_heads,
                                   float* out_dev, void* stream);
+
+/* ------------------------------------------------------------------ */
+/* Attention block of many tokens (no reference counterpart)            */
+/* ------------------------------------------------------------------ */
+
+/* RMSNorm of every query and key head and the rotary rotation, in one pass,
+ * for n_tokens tokens at the device positions positions_dev[n_tokens]: head
+ * row x -> x * (1/sqrt(mean(x^2) + eps)) * norm, then pairs (i, i+head_dim/2)
+ * (neox != 0) or (2i, 2i+1) turn by positions[t] * theta^(-2i/head_dim).
+ * q_dev holds n_heads and k_dev n_kv_heads rows of head_dim values a token;
+ * token t starts at element t * ldq (ldk), so the heads may be views into the
+ * rows of one fused projection.  q_norm_dev / k_norm_dev [head_dim] are shared
+ * by all heads.  Outputs have strides of their own and may be the inputs (same
+ * pointer and stride); other overlap is not allowed.  A count of heads may be
+ * 0 (its pointers are then not read).  The angles are formed in 64 bits (any
+ * int32 position is right to a float's rounding); dqmk_rope's are the
+ * reference's float expressions, up to 2^-24 of the angle away.
+ * head_dim: even, at most 256. */
+int dqmk_qk_norm_rope(const float* q_dev, int64_t ldq, const float* k_dev, int64_t ldk,
+                      int n_tokens, int n_heads, int n_kv_heads, int head_dim,
+                      const float* q_norm_dev, const float* k_norm_dev, float eps,
+                      const int* positions_dev, float theta, int neox, float* q_out_dev,
+                      int64_t ldq_out, float* k_out_dev, int64_t ldk_out, void* stream);
+
+/* Causal attention over packed prompts: sequence s is the tokens
+ * starts_dev[s] .. starts_dev[s+1]-1 (starts_dev: n_seqs + 1 non-decreasing
+ * offsets into the n_tokens rows; a sequence may be empty); each of its tokens
+ * attends to itself and the sequence's earlier tokens: softmax(q.k /
+ * sqrt(head_dim)) v, query head h with KV head h / (n_heads / n_kv_heads).
+ * q_dev / out_dev hold n_heads, k_dev / v_dev n_kv_heads rows of head_dim
+ * values a token, token t at element t * ld; out_dev must not overlap the
+ * inputs.  Rows outside every sequence (behind the last one) are left as they
+ * were.  A sequence whose offsets are out of order or outside 0..n_tokens is
+ * skipped and recorded (dqmk_device_error bit 3).  Results are within f32
+ * summation order of f32 arithmetic, and the same for the same arguments every
+ * time.  head_dim: a multiple of 4, at most 128; pointers 16-byte aligned,
+ * strides multiples of 4.  workspace_dev: dqmk_attention_prompt_workspace
+ * bytes, contents ignored; calls that may overlap on the GPU need one each. */
+size_t dqmk_attention_prompt_workspace(int n_tokens, int n_seqs, int n_heads, int n_kv_heads,
+                                       int head_dim);
+int dqmk_attention_prompt(const float* q_dev, int64_t ldq, const float* k_dev, int64_t ldk,
+                          const float* v_dev, int64_t ldv, const int* starts_dev, int n_seqs,
+                          int n_tokens, int n_heads, int n_kv_heads, int head_dim, float* out_dev,
+                          int64_t ldo, void* workspace_dev, size_t workspace_bytes, void* stream);
+
+/* A KV cache held as Q4_0 blocks: n_slots independent sequences of up to
+ * max_seq positions for each of n_layers layers.  keys_dev and values_dev are
+ * device buffers of dqmk_kv_q40_bytes each (16-byte aligned, contents opaque;
+ * they need no initialisation: only written positions are read).  head_dim: a
+ * multiple of 32, at most 128. */
+typedef struct dqmk_kv_q40 {
+  void* keys_dev;
+  void* values_dev;
+  int n_layers, n_slots, max_seq, n_kv_heads, head_dim;
+} dqmk_kv_q40;
+
+/* Bytes of each of the two buffers (0: a shape that is not supported). */
+size_t dqmk_kv_q40_bytes(int n_layers, int n_slots, int max_seq, int n_kv_heads, int head_dim);
+
+/* Quantizes the key and value rows of n_tokens tokens (n_kv_heads rows of
+ * head_dim values; token t at element t * ldk / t * ldv), block by block as
+ * dqmk_quantize_q40 does, and stores token t at position positions_dev[t] of
+ * slot slots_dev[t] (slots_dev NULL: slot t) of layer `layer`.  A token with
+ * position -1 is padding and stores nothing.  A slot or position outside the
+ * cache stores nothing and is recorded (dqmk_device_error bit 3).  A (slot,
+ * position) pair at most once in a call: of two rows it is not said which
+ * blocks stay. */
+int dqmk_kv_q40_write(const dqmk_kv_q40* kv, int layer, const float* k_dev, int64_t ldk,
+                      const float* v_dev, int64_t ldv, const int* slots_dev,
+                      const int* positions_dev, int n_tokens, void* stream);
+
+/* The values that the cache holds for those rows, as f32; rows of padding and
+ * of indices outside the cache are left as they were. */
+int dqmk_kv_q40_read(const dqmk_kv_q40* kv, int layer, const int* slots_dev,
+                     const int* positions_dev, int n_tokens, float* k_dev, int64_t ldk,
+                     float* v_dev, int64_t ldv, void* stream);
+
+/* Decode attention over the 4-bit cache: column c is one query token, q_dev
+ * [n_heads][head_dim] at element c * ldq, over positions 0 .. lengths_dev[c]-1
+ * of slot slots_dev[c] (NULL: slot c); softmax(q.k / sqrt(head_dim)) v to
+ * out_dev at element c * ldo.  Query heads h use KV head h / (n_heads /
+ * n_kv_heads).  Several columns may name one slot (a prompt's tokens with
+ * growing lengths, once their rows are written).  Length 0 gives a row of
+ * zeros; so do a length outside 0..max_seq and a slot outside the cache, which
+ * are recorded (dqmk_device_error bit 3).  Results are those of f32 arithmetic
+ * on the cache's values (within f32 summation order), and the same for the
+ * same arguments every time.  workspace_dev: dqmk_kv_q40_attention_workspace
+ * bytes, 16-byte aligned, contents ignored; calls that may overlap on the GPU
+ * need one each. */
+size_t dqmk_kv_q40_attention_workspace(const dqmk_kv_q40* kv, int n_cols, int n_heads);
+int dqmk_kv_q40_attention(const dqmk_kv_q40* kv, int layer, const float* q_dev, int64_t ldq,
+                          const int* slots_dev, const int* lengths_dev, int n_cols, int n_heads,
+                          float* out_dev, int64_t ldo, void* workspace_dev,
+                          size_t workspace_bytes, void* stream);
 
 /* ------------------------------------------------------------------ */
 /* Engine: device-resident model + context (ForwardToken / ForwardBatch)*/

@@ -333,18 +333,27 @@ def CudaAttentionDecodeDeviceInput(q, kv: CudaKvCache, layer: int, pos: int, n_h
 
 
 # ------------------------------------------------------------ attention block
-class _on:
-    """The device of `tensor` and the stream of a call (None: torch's current
-    stream of that device) made current, so that outputs and workspaces are
-    allocated for the stream that uses them."""
+class _Here:
+    """A call on the current device and stream."""
 
-    def __init__(self, tensor, stream):
+    def __enter__(self):
+        return _torch().cuda.current_stream().cuda_stream
+
+    def __exit__(self, *exc):
+        pass
+
+
+class _There:
+    """A call on another device or a given stream: both are made current, so
+    that outputs and workspaces are allocated for the stream that uses them."""
+
+    def __init__(self, device, stream):
         torch = _torch()
         if stream is not None and not isinstance(stream, torch.cuda.Stream):
-            stream = torch.cuda.ExternalStream(stream, device=tensor.device)
-        if stream is not None and stream.device != tensor.device:
+            stream = torch.cuda.ExternalStream(stream, device=device)
+        if stream is not None and stream.device != device:
             raise RuntimeError("stream and tensors are on different devices")
-        self.guards = (torch.cuda.device(tensor.device), torch.cuda.stream(stream))
+        self.guards = (torch.cuda.device(device), torch.cuda.stream(stream))
 
     def __enter__(self):
         for g in self.guards:
@@ -356,36 +365,48 @@ class _on:
             g.__exit__(*exc)
 
 
-def _check_tensor(api: str, name: str, t, shape, device, dtype=None):
-    """A CUDA tensor of this shape and type on this device, with contiguous
-    rows: everything but the first dimension's stride is fixed."""
+_here = _Here()
+
+
+def _on(device, stream):
+    if stream is None and device.index == _torch().cuda.current_device():
+        return _here
+    return _There(device, stream)
+
+
+def _refuse(api: str, name: str, t, shape, dtype, device):
     torch = _torch()
-    dtype = dtype or torch.float32
-    if not isinstance(t, torch.Tensor) or not t.is_cuda or t.device != device:
+    if not isinstance(t, torch.Tensor) or t.device != device:
         raise RuntimeError(f"{api}: {name} must be a tensor on {device}")
     if t.dtype != dtype:
         raise RuntimeError(f"{api}: {name} must be {dtype}, is {t.dtype}")
     if tuple(t.shape) != tuple(shape):
         raise RuntimeError(f"{api}: {name} must have shape {tuple(shape)}, has {tuple(t.shape)}")
-    step = 1
-    for dim in range(t.dim() - 1, 0, -1):
-        if t.shape[dim] != 1 and t.stride(dim) != step:
-            raise RuntimeError(f"{api}: the rows of {name} must be contiguous")
-        step *= t.shape[dim]
-    if t.dim() == 1 and t.shape[0] > 1 and t.stride(0) != 1:
-        raise RuntimeError(f"{api}: {name} must be contiguous")
+    raise RuntimeError(f"{api}: the rows of {name} must be contiguous")
 
 
-def _check_device(api: str, t, dims: int, name: str):
-    torch = _torch()
-    if not isinstance(t, torch.Tensor) or not t.is_cuda or t.dim() != dims:
+def _first(api: str, name: str, t, dims: int):
+    """The device of the tensor that a call's other tensors are checked against."""
+    if not isinstance(t, _torch().Tensor) or not t.is_cuda or t.dim() != dims:
         raise RuntimeError(f"{api}: {name} must be a {dims}-dimensional CUDA tensor")
+    return t.device
 
 
-def _ld(t) -> int:
-    """Elements from one row to the next."""
-    row = int(np.prod(t.shape[1:]))
-    return t.stride(0) if t.shape[0] > 1 else row
+def _rows(api: str, name: str, t, shape, device) -> int:
+    """Elements from one row to the next of a float32 [rows, heads, head_dim]
+    tensor of this shape and device whose rows are contiguous."""
+    f32 = _torch().float32
+    if isinstance(t, _torch().Tensor) and t.dtype is f32 and t.shape == shape and t.device == device:
+        row, head, value = t.stride()
+        if (value == 1 or shape[2] == 1) and (head == shape[2] or shape[1] < 2):
+            return row if shape[0] > 1 else shape[1] * shape[2]
+    _refuse(api, name, t, shape, f32, device)
+
+
+def _vector(api: str, name: str, t, n: int, device, dtype):
+    if not (isinstance(t, _torch().Tensor) and t.dtype is dtype and t.shape == (n,) and
+            t.device == device and (n < 2 or t.stride(0) == 1)):
+        _refuse(api, name, t, (n,), dtype, device)
 
 
 def qk_norm_rope(q, k, q_norm, k_norm, positions, theta: float, eps: float, neox: bool = True,
@@ -397,25 +418,28 @@ def qk_norm_rope(q, k, q_norm, k_norm, positions, theta: float, eps: float, neox
     (q_out, k_out)."""
     torch = _torch()
     api = "QkNormRope"
-    _check_device(api, q, 3, "q")
-    n, heads, dim = q.shape
-    _check_device(api, k, 3, "k")
+    dev = _first(api, "q", q, 3)
+    _first(api, "k", k, 3)
+    n, heads, dim = shape = q.shape
     kv = k.shape[1]
-    dev = q.device
-    _check_tensor(api, "q", q, (n, heads, dim), dev)
-    _check_tensor(api, "k", k, (n, kv, dim), dev)
-    _check_tensor(api, "q_norm", q_norm, (dim,), dev)
-    _check_tensor(api, "k_norm", k_norm, (dim,), dev)
-    _check_tensor(api, "positions", positions, (n,), dev, torch.int32)
-    with _on(q, stream) as s:
-        q_out = torch.empty((n, heads, dim), device=dev) if q_out is None else q_out
-        k_out = torch.empty((n, kv, dim), device=dev) if k_out is None else k_out
-        _check_tensor(api, "q_out", q_out, q.shape, dev)
-        _check_tensor(api, "k_out", k_out, k.shape, dev)
+    ldq = _rows(api, "q", q, shape, dev)
+    ldk = _rows(api, "k", k, (n, kv, dim), dev)
+    _vector(api, "q_norm", q_norm, dim, dev, torch.float32)
+    _vector(api, "k_norm", k_norm, dim, dev, torch.float32)
+    _vector(api, "positions", positions, n, dev, torch.int32)
+    with _on(dev, stream) as s:
+        if q_out is None:
+            q_out, ldqo = q.new_empty(shape), heads * dim
+        else:
+            ldqo = _rows(api, "q_out", q_out, shape, dev)
+        if k_out is None:
+            k_out, ldko = k.new_empty((n, kv, dim)), kv * dim
+        else:
+            ldko = _rows(api, "k_out", k_out, (n, kv, dim), dev)
         check(lib().dqmk_qk_norm_rope(
-            _ptr(q), _ld(q), _ptr(k), _ld(k), n, heads, kv, dim, _ptr(q_norm), _ptr(k_norm),
-            float(eps), _ptr(positions), float(theta), 1 if neox else 0, _ptr(q_out), _ld(q_out),
-            _ptr(k_out), _ld(k_out), s))
+            q.data_ptr(), ldq, k.data_ptr(), ldk, n, heads, kv, dim, q_norm.data_ptr(),
+            k_norm.data_ptr(), eps, positions.data_ptr(), theta, 1 if neox else 0,
+            q_out.data_ptr(), ldqo, k_out.data_ptr(), ldko, s))
     return q_out, k_out
 
 
@@ -426,27 +450,27 @@ def attention_prompt(q, k, v, starts, out=None, stream=None):
     outside every sequence are left as they were (a new `out` is zero there)."""
     torch = _torch()
     api = "AttentionPrompt"
-    _check_device(api, q, 3, "q")
-    n, heads, dim = q.shape
-    _check_device(api, k, 3, "k")
-    kv = k.shape[1]
-    dev = q.device
-    _check_device(api, starts, 1, "starts")
-    seqs = starts.shape[0] - 1
+    dev = _first(api, "q", q, 3)
+    _first(api, "k", k, 3)
+    _first(api, "starts", starts, 1)
+    n, heads, dim = shape = q.shape
+    kv, seqs = k.shape[1], starts.shape[0] - 1
     if seqs < 0:
         raise RuntimeError(f"{api}: starts must hold at least one offset")
-    _check_tensor(api, "q", q, (n, heads, dim), dev)
-    _check_tensor(api, "k", k, (n, kv, dim), dev)
-    _check_tensor(api, "v", v, (n, kv, dim), dev)
-    _check_tensor(api, "starts", starts, (seqs + 1,), dev, torch.int32)
-    with _on(q, stream) as s:
-        out = torch.zeros((n, heads, dim), device=dev) if out is None else out
-        _check_tensor(api, "out", out, q.shape, dev)
-        nbytes = lib().dqmk_attention_prompt_workspace(n, seqs, heads, kv, dim)
+    ldq = _rows(api, "q", q, shape, dev)
+    ldk = _rows(api, "k", k, (n, kv, dim), dev)
+    ldv = _rows(api, "v", v, (n, kv, dim), dev)
+    _vector(api, "starts", starts, seqs + 1, dev, torch.int32)
+    with _on(dev, stream) as s:
+        if out is None:
+            out = torch.zeros(shape, dtype=torch.float32, device=dev)
+        ldo = _rows(api, "out", out, shape, dev)
+        L = lib()
+        nbytes = L.dqmk_attention_prompt_workspace(n, seqs, heads, kv, dim)
         work = torch.empty(nbytes, dtype=torch.uint8, device=dev)
-        check(lib().dqmk_attention_prompt(
-            _ptr(q), _ld(q), _ptr(k), _ld(k), _ptr(v), _ld(v), _ptr(starts), seqs, n, heads, kv,
-            dim, _ptr(out), _ld(out), _ptr(work), nbytes, s))
+        check(L.dqmk_attention_prompt(
+            q.data_ptr(), ldq, k.data_ptr(), ldk, v.data_ptr(), ldv, starts.data_ptr(), seqs, n,
+            heads, kv, dim, out.data_ptr(), ldo, work.data_ptr(), nbytes, s))
     return out
 
 
@@ -467,46 +491,50 @@ class KvCacheQ40:
                                "of at most 128, every count positive)")
         self.keys = torch.zeros(nbytes, dtype=torch.uint8, device=device)
         self.values = torch.zeros(nbytes, dtype=torch.uint8, device=device)
+        self.device = self.keys.device
         self._c = KvQ40(_ptr(self.keys), _ptr(self.values), self.n_layers, self.n_slots,
                         self.max_seq, self.n_kv_heads, self.head_dim)
-
-    def _index(self, api, positions, slots, n):
-        torch = _torch()
-        _check_tensor(api, "positions", positions, (n,), self.keys.device, torch.int32)
-        if slots is not None:
-            _check_tensor(api, "slots", slots, (n,), self.keys.device, torch.int32)
+        self._ref = C.byref(self._c)
 
     def write(self, layer: int, k, v, positions, slots=None, stream=None) -> None:
         """Rows k, v [tokens, n_kv_heads, head_dim] to positions [tokens] of
         slots [tokens] (None: slot t for token t); position -1 stores nothing."""
-        api = "KvQ40Write"
-        _check_device(api, k, 3, "k")
+        api, dev, i32 = "KvQ40Write", self.device, _torch().int32
+        _first(api, "k", k, 3)
         n = k.shape[0]
-        for name, t in (("k", k), ("v", v)):
-            _check_tensor(api, name, t, (n, self.n_kv_heads, self.head_dim), self.keys.device)
-        self._index(api, positions, slots, n)
-        with _on(self.keys, stream) as s:
-            check(lib().dqmk_kv_q40_write(C.byref(self._c), layer, _ptr(k), _ld(k), _ptr(v), _ld(v),
-                                          _ptr(slots), _ptr(positions), n, s))
+        shape = (n, self.n_kv_heads, self.head_dim)
+        ldk = _rows(api, "k", k, shape, dev)
+        ldv = _rows(api, "v", v, shape, dev)
+        _vector(api, "positions", positions, n, dev, i32)
+        if slots is not None:
+            _vector(api, "slots", slots, n, dev, i32)
+        with _on(dev, stream) as s:
+            check(lib().dqmk_kv_q40_write(
+                self._ref, layer, k.data_ptr(), ldk, v.data_ptr(), ldv,
+                None if slots is None else slots.data_ptr(), positions.data_ptr(), n, s))
 
     def read(self, layer: int, positions, slots=None, k_out=None, v_out=None, stream=None):
         """The values held at those rows, as (k, v) [tokens, n_kv_heads,
         head_dim]; rows of position -1 are left as they were (zero in new
         tensors)."""
         torch = _torch()
-        api = "KvQ40Read"
-        _check_device(api, positions, 1, "positions")
+        api, dev = "KvQ40Read", self.device
+        _first(api, "positions", positions, 1)
         n = positions.shape[0]
-        self._index(api, positions, slots, n)
         shape = (n, self.n_kv_heads, self.head_dim)
-        dev = self.keys.device
-        with _on(self.keys, stream) as s:
-            k_out = torch.zeros(shape, device=dev) if k_out is None else k_out
-            v_out = torch.zeros(shape, device=dev) if v_out is None else v_out
-            _check_tensor(api, "k_out", k_out, shape, dev)
-            _check_tensor(api, "v_out", v_out, shape, dev)
-            check(lib().dqmk_kv_q40_read(C.byref(self._c), layer, _ptr(slots), _ptr(positions), n,
-                                         _ptr(k_out), _ld(k_out), _ptr(v_out), _ld(v_out), s))
+        _vector(api, "positions", positions, n, dev, torch.int32)
+        if slots is not None:
+            _vector(api, "slots", slots, n, dev, torch.int32)
+        with _on(dev, stream) as s:
+            if k_out is None:
+                k_out = torch.zeros(shape, dtype=torch.float32, device=dev)
+            if v_out is None:
+                v_out = torch.zeros(shape, dtype=torch.float32, device=dev)
+            ldk = _rows(api, "k_out", k_out, shape, dev)
+            ldv = _rows(api, "v_out", v_out, shape, dev)
+            check(lib().dqmk_kv_q40_read(
+                self._ref, layer, None if slots is None else slots.data_ptr(),
+                positions.data_ptr(), n, k_out.data_ptr(), ldk, v_out.data_ptr(), ldv, s))
         return k_out, v_out
 
     def attention(self, q, layer: int, lengths, slots=None, out=None, stream=None):
@@ -515,22 +543,25 @@ class KvCacheQ40:
         the device.  Length 0 gives zeros.  Returns out [columns, n_heads,
         head_dim]."""
         torch = _torch()
-        api = "KvQ40Attention"
-        _check_device(api, q, 3, "q")
+        api, dev = "KvQ40Attention", self.device
+        _first(api, "q", q, 3)
         n, heads, _ = q.shape
-        dev = self.keys.device
-        _check_tensor(api, "q", q, (n, heads, self.head_dim), dev)
-        _check_tensor(api, "lengths", lengths, (n,), dev, torch.int32)
+        shape = (n, heads, self.head_dim)
+        ldq = _rows(api, "q", q, shape, dev)
+        _vector(api, "lengths", lengths, n, dev, torch.int32)
         if slots is not None:
-            _check_tensor(api, "slots", slots, (n,), dev, torch.int32)
-        with _on(self.keys, stream) as s:
-            out = torch.empty(q.shape, device=dev) if out is None else out
-            _check_tensor(api, "out", out, q.shape, dev)
-            nbytes = lib().dqmk_kv_q40_attention_workspace(C.byref(self._c), n, heads)
+            _vector(api, "slots", slots, n, dev, torch.int32)
+        with _on(dev, stream) as s:
+            if out is None:
+                out, ldo = q.new_empty(shape), heads * self.head_dim
+            else:
+                ldo = _rows(api, "out", out, shape, dev)
+            L = lib()
+            nbytes = L.dqmk_kv_q40_attention_workspace(self._ref, n, heads)
             work = torch.empty(nbytes, dtype=torch.uint8, device=dev)
-            check(lib().dqmk_kv_q40_attention(
-                C.byref(self._c), layer, _ptr(q), _ld(q), _ptr(slots), _ptr(lengths), n, heads,
-                _ptr(out), _ld(out), _ptr(work), nbytes, s))
+            check(L.dqmk_kv_q40_attention(
+                self._ref, layer, q.data_ptr(), ldq, None if slots is None else slots.data_ptr(),
+                lengths.data_ptr(), n, heads, out.data_ptr(), ldo, work.data_ptr(), nbytes, s))
         return out
 
 

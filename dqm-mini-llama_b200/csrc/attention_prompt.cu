@@ -1,12 +1,41 @@
-// attention_prompt.cu -- causal attention over packed prompts.
+// attention_prompt.cu -- causal attention over packed prompts, on tcgen05.
 //
 // Sequence s holds tokens starts[s] .. starts[s+1]-1 of the packed rows; token
 // i of it, query head h, key/value head h / group:
 //   s_ij = q_i . k_j / sqrt(D) for j <= i, softmax over j, out_i = sum p_ij v_j
+//
+// Both products run on the tensor cores with f32 results: an operand is scaled
+// by a power of two and split into two fp16 terms (x = hi + lo + r, |r| <=
+// 2^-22 |x|), and A_hi B_hi + A_hi B_lo + A_lo B_hi accumulate in fp32 tensor
+// memory.  That is three products for one, 562 TFLOP/s of the measured 1686;
+// f32 FMAs have an eighth of it.
+//
+// First kernel (prompt_split): K and V of every sequence, in tiles of 64 keys
+// that start at the sequence's first token, become the shared-memory images of
+// the second kernel's operands (K rows, V columns, both terms, 128-byte
+// swizzle), so that a tile is one contiguous bulk copy and needs neither a
+// tensor map nor any alignment of the sequence's first token.  K and V take one
+// power of two a tile.  A tile whose rows differ by more than 2^16 in size, or
+// that holds an infinity or a NaN, would lose the smaller rows' bits or reach
+// queries that must not see it; it is marked, and the second kernel takes it
+// in f32 straight from the inputs.
+//
+// Second kernel: a CTA takes 128 rows (token, head of the group) of one
+// sequence and KV head, row f = token * group + head: the heads that share
+// keys fill a tile also where the sequence is short, and a tile of rows spans
+// few tokens, so little of the masked triangle is computed.  Row r is TMEM lane
+// r.  One warp streams the tiles, one issues the products, eight run the
+// softmax, warps w and w + 4 on the same 32 rows and half of the columns each:
+//   S(j) = Q K_j^T      A = Q (TMEM), B = K_j
+//   P(j) = exp2(S f - m) 2^14, two terms, over S(j)'s own columns
+//   O'(j) = P(j) V_j    A = P(j) (TMEM), B = V_j; o = o corr + O' 2^e in registers
+// S(j+1) is issued before P(j) is waited for, so the tensor cores work on the
+// next scores while the softmax runs.
 #include <climits>
 
 #include "common.cuh"
 #include "internal.h"
+#include "tc_dev.cuh"
 
 namespace dqmk {
 namespace {
@@ -14,6 +43,7 @@ namespace {
 __device__ unsigned int g_prompt_error;  // kErrTimeout / kErrBadIndex
 
 constexpr int kMaxDim = 128;
+constexpr int kRows = 128, kKeys = 64;
 constexpr float kLog2e = 1.44269504088896341f;
 
 struct PromptArgs {
@@ -23,88 +53,552 @@ struct PromptArgs {
   int n_seqs, n_tokens, n_heads, n_kv_heads, group, head_dim;
   float* out;
   int64_t ldo;
-  float scale;  // log2(e) / sqrt(D)
+  float scale;            // log2(e) / sqrt(D)
+  unsigned char* images;  // [tile][kv_head] operand images
+  float4* meta;           // [tile][kv_head]: 2^ek, 2^ev, marked, -
+  int max_tiles;
 };
 
-constexpr int kThreads = 128, kRows = 16, kKeys = 32, kRowsPerWarp = kRows / 4;
+// DP: head_dim rounded up to 64 or 128.
+template <int DP>
+struct Cfg {
+  static constexpr int kPlane = kKeys * DP * 2;     // one term of K or V
+  static constexpr int kOperand = 2 * kPlane;       // both terms
+  static constexpr int kImage = 2 * kOperand;       // K, then V
+  static constexpr int kStages = 3;
+  static constexpr int kBufs = DP == 128 ? 3 : 2;   // score buffers
+  static constexpr int kCtas = DP == 128 ? 1 : 2;   // for each SM
+  static constexpr int kSmem = kStages * kImage + 1024;
+  static constexpr uint32_t kTmem = DP == 128 ? 512 : 256;
+  static constexpr uint32_t kColQ = 0, kColO = DP, kColS = 2 * DP;
+  static_assert(2 * DP + 64 * kBufs <= kTmem, "tensor memory plan");
+};
 
-// One CTA: 16 rows (token, head of the group) of one sequence and KV head.
-__global__ void __launch_bounds__(kThreads) attention_prompt_kernel(const PromptArgs a) {
-  __shared__ float ks[kKeys][kMaxDim + 1], vs[kKeys][kMaxDim];
-  __shared__ float qs[kRows][kMaxDim];
-  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, D = a.head_dim;
-  const int kvh = blockIdx.y;
-  // block x -> (sequence, first row)
-  int seq = 0, t0 = 0, n = 0;
-  int64_t blk = blockIdx.x;
-  for (; seq < a.n_seqs; ++seq) {
-    t0 = a.starts[seq];
-    const int t1 = a.starts[seq + 1];
-    if (t0 < 0 || t1 < t0 || t1 > a.n_tokens) {
-      if (tid == 0) atomicOr(&g_prompt_error, kErrBadIndex);
-      continue;
+// One sequence's place in the packed work: row tiles and key tiles of the
+// sequences before it.
+struct Place {
+  int seq, first, n;
+  int64_t row_tiles, key_tiles;  // before this sequence
+};
+
+__device__ __forceinline__ int seq_len(const PromptArgs& a, int s) {
+  const int t0 = a.starts[s], t1 = a.starts[s + 1];
+  return t0 >= 0 && t1 >= t0 && t1 <= a.n_tokens ? t1 - t0 : 0;
+}
+__device__ __forceinline__ int64_t row_tiles_of(const PromptArgs& a, int n) {
+  return ((int64_t)n * a.group + kRows - 1) / kRows;
+}
+
+// The sequence that holds row tile (by_rows) or key tile `index` of the whole
+// pack; false past the end.  All threads call; `shared` is one Place.
+__device__ __forceinline__ bool find_place(const PromptArgs& a, int64_t index, bool by_rows,
+                                           int64_t* warp_sums, Place* shared) {
+  int64_t rows = 0, keys = 0;
+  if (threadIdx.x == 0) shared->seq = -1;
+  for (int s0 = 0; s0 < a.n_seqs; s0 += blockDim.x) {
+    const int s = s0 + threadIdx.x;
+    const int n = s < a.n_seqs ? seq_len(a, s) : 0;
+    const int64_t mine_r = row_tiles_of(a, n), mine_k = (n + kKeys - 1) / kKeys;
+    int64_t before;
+    const int64_t sum = block_scan(mine_r << 32 | mine_k, &before, warp_sums);
+    const int64_t br = rows + (before >> 32), bk = keys + (before & 0xffffffff);
+    const int64_t b = by_rows ? br : bk, mine = by_rows ? mine_r : mine_k;
+    if (index >= b && index < b + mine) *shared = Place{s, a.starts[s], n, br, bk};
+    rows += sum >> 32;
+    keys += sum & 0xffffffff;
+    if (index < (by_rows ? rows : keys)) break;
+  }
+  __syncthreads();
+  return shared->seq >= 0;
+}
+
+// Byte offset of 16-byte chunk c (8 fp16) of row r in a 128-byte-swizzled
+// K-major operand tile (8-row atoms of 1024 bytes).
+__device__ __forceinline__ uint32_t sw128(int r, int c) {
+  return (uint32_t)((r >> 3) * 1024 + (r & 7) * 128 + ((c ^ (r & 7)) << 4));
+}
+__device__ __forceinline__ float pow2f(int e) { return __int_as_float((127 + e) << 23); }
+// e such that top 2^-e lies in [2^14, 2^15); 0 for 0.
+__device__ __forceinline__ int pow2_ex(float top) {
+  const int fe = ((__float_as_int(top) >> 23) & 0xff) - 126;
+  return top > 0.0f ? min(max(fe - 15, -120), 120) : 0;
+}
+// Two values to packed fp16 pairs with x = hi + lo + r, |r| <= 2^-22 |x|.
+__device__ __forceinline__ void split2(float x0, float x1, uint32_t& hi, uint32_t& lo) {
+  const __half2 h = __floats2half2_rn(x0, x1);
+  const float2 back = __half22float2(h);
+  const __half2 l = __floats2half2_rn(__fsub_rn(x0, back.x), __fsub_rn(x1, back.y));
+  hi = *reinterpret_cast<const uint32_t*>(&h);
+  lo = *reinterpret_cast<const uint32_t*>(&l);
+}
+
+// ------------------------------------------------------------ first kernel
+constexpr int kSplitThreads = 256;
+constexpr int kMostSpread = 16;  // exponents between a tile's largest and smallest row
+
+template <int DP>
+__global__ void __launch_bounds__(kSplitThreads) prompt_split_kernel(const PromptArgs a) {
+  using C = Cfg<DP>;
+  constexpr int kF4 = DP / 4, kPer = kKeys * kF4 / kSplitThreads;  // float4s a row, a thread
+  __shared__ int64_t warp_sums[kSplitThreads / 32];
+  __shared__ Place place;
+  __shared__ float vt[kKeys][DP + 1];
+  __shared__ int top_bits, low_bits;
+  const int tid = threadIdx.x, kvh = blockIdx.y, D = a.head_dim;
+  if (blockIdx.x == 0 && kvh == 0)
+    for (int s = tid; s < a.n_seqs; s += kSplitThreads) {
+      const int t0 = a.starts[s], t1 = a.starts[s + 1];
+      if (t0 < 0 || t1 < t0 || t1 > a.n_tokens) atomicOr(&g_prompt_error, kErrBadIndex);
     }
-    n = t1 - t0;
-    const int64_t blocks = ((int64_t)n * a.group + kRows - 1) / kRows;
-    if (blk < blocks) break;
-    blk -= blocks;
-  }
-  if (seq == a.n_seqs) return;
-  const int64_t f0 = blk * kRows, rows = (int64_t)n * a.group;
-  for (int i = tid; i < kRows * D; i += kThreads) {
-    const int r = i / D, d = i % D;
-    const int64_t f = f0 + r;
-    qs[r][d] = f < rows ? a.q[(t0 + f / a.group) * a.ldq + (kvh * a.group + f % a.group) * D + d] * a.scale : 0.0f;
-  }
-  float m[kRowsPerWarp], l[kRowsPerWarp], o[kRowsPerWarp][4];
-  int token[kRowsPerWarp];
+  const bool found = find_place(a, blockIdx.x, false, warp_sums, &place);
+  pdl_trigger();
+  if (!found) return;
+  const int64_t tile = blockIdx.x;  // < max_tiles: the grid's size
+  const int k0 = (int)(tile - place.key_tiles) * kKeys, live = min(kKeys, place.n - k0);
+  unsigned char* image = a.images + (tile * a.n_kv_heads + kvh) * C::kImage;
+  float scales[2];
+  bool marked = false;
+
+  // a thread's float4s of one row sit kSplitThreads / kF4 rows apart
+  const int c4 = tid % kF4, r0 = tid / kF4;
+  float4 x[2][kPer];
 #pragma unroll
-  for (int r = 0; r < kRowsPerWarp; ++r) {
-    const int64_t f = f0 + warp * kRowsPerWarp + r;
-    token[r] = f < rows ? (int)(f / a.group) : -1;
-    m[r] = -INFINITY, l[r] = 0.0f;
+  for (int which = 0; which < 2; ++which) {
+    const float* base = (which ? a.v : a.k) + (int64_t)(place.first + k0) * (which ? a.ldv : a.ldk) +
+                        (int64_t)kvh * D;
+    const int64_t ld = which ? a.ldv : a.ldk;
 #pragma unroll
-    for (int e = 0; e < 4; ++e) o[r][e] = 0.0f;
+    for (int i = 0; i < kPer; ++i) {
+      const int r = r0 + i * (kSplitThreads / kF4);
+      x[which][i] = r < live && 4 * c4 < D ? *reinterpret_cast<const float4*>(base + r * ld + 4 * c4)
+                                           : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+    }
   }
-  const int last = (int)(min(f0 + kRows, rows) - 1) / a.group;
-  for (int k0 = 0; k0 <= last; k0 += kKeys) {
-    __syncthreads();
-    for (int i = tid; i < kKeys * D; i += kThreads) {
-      const int j = i / D, d = i % D;
-      const bool in = k0 + j < n;
-      ks[j][d] = in ? a.k[(t0 + k0 + j) * a.ldk + kvh * D + d] : 0.0f;
-      vs[j][d] = in ? a.v[(t0 + k0 + j) * a.ldv + kvh * D + d] : 0.0f;
+#pragma unroll
+  for (int which = 0; which < 2; ++which) {
+    if (tid == 0) {
+      top_bits = 0;
+      low_bits = INT_MAX;
     }
     __syncthreads();
+    // sizes compare as integers; an infinity or a NaN is larger than any number
 #pragma unroll
-    for (int r = 0; r < kRowsPerWarp; ++r) {
-      const float* q = qs[warp * kRowsPerWarp + r];
-      float s = 0.0f;
-      for (int d = 0; d < D; ++d) s = fmaf(q[d], ks[lane][d], s);
-      if (k0 + lane > token[r]) s = -INFINITY;
-      const float mx = fmaxf(m[r], warp_max(s)), ref = mx == -INFINITY ? 0.0f : mx;
-      const float corr = exp2f(m[r] - ref), p = exp2f(s - ref);
-      l[r] = fmaf(l[r], corr, warp_sum(p));
-      m[r] = mx;
+    for (int i = 0; i < kPer; ++i) {
+      const float4 f = x[which][i];
+      int top = max(max(__float_as_int(fabsf(f.x)), __float_as_int(fabsf(f.y))),
+                    max(__float_as_int(fabsf(f.z)), __float_as_int(fabsf(f.w))));
 #pragma unroll
-      for (int e = 0; e < 4; ++e) o[r][e] *= corr;
-      for (int j = 0; j < kKeys && k0 + j <= token[r]; ++j) {
-        const float pj = __shfl_sync(0xffffffffu, p, j);
-#pragma unroll
-        for (int e = 0; e < 4; ++e)
-          if (lane + 32 * e < D) o[r][e] = fmaf(pj, vs[j][lane + 32 * e], o[r][e]);
+      for (int o = 1; o < (kF4 < 32 ? kF4 : 32); o <<= 1)
+        top = max(top, __shfl_xor_sync(0xffffffffu, top, o));
+      if (c4 == 0 && top > 0) {
+        atomicMax(&top_bits, top);
+        atomicMin(&low_bits, top);
       }
     }
+    __syncthreads();
+    const int top = top_bits, low = low_bits;
+    if (top >= 0x7f800000 || (top > 0 && (top >> 23) - (low >> 23) > kMostSpread)) marked = true;
+    const int e = pow2_ex(__int_as_float(top));
+    scales[which] = pow2f(e);
+    const float down = pow2f(-e);
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < kPer; ++i) {
+      float4& f = x[which][i];
+      f.x *= down, f.y *= down, f.z *= down, f.w *= down;
+    }
+  }
+  if (marked) {  // the products must add nothing
+#pragma unroll
+    for (int i = 0; i < kPer; ++i)
+      x[0][i] = x[1][i] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
   }
 #pragma unroll
-  for (int r = 0; r < kRowsPerWarp; ++r) {
-    const int64_t f = f0 + warp * kRowsPerWarp + r;
-    if (f >= rows) continue;
-    float* y = a.out + (t0 + f / a.group) * a.ldo + (kvh * a.group + f % a.group) * D;
-#pragma unroll
-    for (int e = 0; e < 4; ++e)
-      if (lane + 32 * e < D) y[lane + 32 * e] = __fdiv_rn(o[r][e], l[r]);
+  for (int i = 0; i < kPer; ++i) {
+    const int r = r0 + i * (kSplitThreads / kF4);
+    const float4 f = x[0][i];
+    uint2 hi, lo;
+    split2(f.x, f.y, hi.x, lo.x);
+    split2(f.z, f.w, hi.y, lo.y);
+    // columns 64 h ..: plane half h, 8-byte half (c4 & 1) of chunk (c4 % 16) / 2
+    unsigned char* dst = image + (c4 / 16) * (kKeys * 128) + sw128(r, (c4 % 16) >> 1) + (c4 & 1) * 8;
+    *reinterpret_cast<uint2*>(dst) = hi;
+    *reinterpret_cast<uint2*>(dst + C::kPlane) = lo;
+    const float4 g = x[1][i];
+    vt[r][4 * c4] = g.x, vt[r][4 * c4 + 1] = g.y, vt[r][4 * c4 + 2] = g.z, vt[r][4 * c4 + 3] = g.w;
   }
+  __syncthreads();
+  // V: operand row d holds the 64 keys; a thread writes 16-byte chunks of 8 keys
+  for (int i = tid; i < DP * 8; i += kSplitThreads) {
+    const int d = i / 8, c = i % 8;
+    uint4 hi, lo;
+    split2(vt[8 * c][d], vt[8 * c + 1][d], hi.x, lo.x);
+    split2(vt[8 * c + 2][d], vt[8 * c + 3][d], hi.y, lo.y);
+    split2(vt[8 * c + 4][d], vt[8 * c + 5][d], hi.z, lo.z);
+    split2(vt[8 * c + 6][d], vt[8 * c + 7][d], hi.w, lo.w);
+    unsigned char* dst = image + C::kOperand + sw128(d, c);
+    *reinterpret_cast<uint4*>(dst) = hi;
+    *reinterpret_cast<uint4*>(dst + C::kPlane) = lo;
+  }
+  if (tid == 0)
+    a.meta[tile * a.n_kv_heads + kvh] = make_float4(scales[0], scales[1], marked ? 1.0f : 0.0f, 0.0f);
+}
+
+// ------------------------------------------------------------ second kernel
+constexpr int kSoftWarps = 8, kThreads = 32 * (kSoftWarps + 2);
+
+__device__ __forceinline__ void bulk_load(void* dst, const void* src, uint32_t bytes, uint64_t* bar) {
+  asm volatile(
+      "cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(
+          tc::su32(dst)),
+      "l"(src), "r"(bytes), "r"(tc::su32(bar))
+      : "memory");
+}
+// The 64 threads of warps w and w + 4.
+__device__ __forceinline__ void pair_sync(int quarter) {
+  asm volatile("bar.sync %0, 64;" ::"r"(quarter + 1) : "memory");
+}
+__device__ __forceinline__ void tmem_st_n(uint32_t addr, const uint32_t (&r)[32]) { tc::tmem_st32(addr, r); }
+__device__ __forceinline__ void tmem_st_n(uint32_t addr, const uint32_t (&r)[16]) { tc::tmem_st16(addr, r); }
+
+template <int DP>
+__global__ void __launch_bounds__(kThreads, Cfg<DP>::kCtas) attention_prompt_kernel(const PromptArgs a) {
+  using C = Cfg<DP>;
+  constexpr int ST = C::kStages, NB = C::kBufs, W = DP / 2;  // W: output columns of a thread
+  extern __shared__ unsigned char raw[];
+  __shared__ __align__(8) uint64_t kfull[ST], kempty[ST], vfull[ST], vempty[ST];
+  __shared__ __align__(8) uint64_t s_done[NB], p_ready[NB], o_done, o_free, q_ready, fin;
+  __shared__ uint32_t tmem_slot;
+  __shared__ volatile int abort_flag;
+  __shared__ float red[2][2][kRows];
+  __shared__ int64_t warp_sums[kThreads / 32];
+  __shared__ Place place;
+  unsigned char* smem = reinterpret_cast<unsigned char*>(
+      (reinterpret_cast<uintptr_t>(raw) + 1023) & ~(uintptr_t)1023);
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  const int kvh = blockIdx.x % a.n_kv_heads;
+  // no such tile of rows; or its sequence has more key tiles than the workspace
+  // holds (offsets that overlap, which are recorded)
+  if (!find_place(a, blockIdx.x / a.n_kv_heads, true, warp_sums, &place) ||
+      place.key_tiles + (place.n + kKeys - 1) / kKeys > a.max_tiles) {
+    pdl_wait();  // so that this grid's end is also the first kernel's
+    return;
+  }
+  const int n = place.n, t0 = place.first;
+  const int64_t tiles_here = row_tiles_of(a, n);
+  // the last tokens see the most keys: their tiles first
+  const int64_t f0 = (tiles_here - 1 - (blockIdx.x / a.n_kv_heads - place.row_tiles)) * kRows;
+  const int64_t rows = (int64_t)n * a.group;
+  const int first_tok = (int)(f0 / a.group);
+  const int last_tok = (int)((min(f0 + kRows, rows) - 1) / a.group);
+  const int nt = last_tok / kKeys + 1;
+  const unsigned char* images = a.images + (place.key_tiles * a.n_kv_heads + kvh) * C::kImage;
+  const float4* meta = a.meta + place.key_tiles * a.n_kv_heads + kvh;
+  const size_t image_step = (size_t)a.n_kv_heads * C::kImage;
+
+  if (tid == 0) {
+    for (int i = 0; i < ST; ++i) {
+      tc::bar_init(&kfull[i], 1);
+      tc::bar_init(&kempty[i], 1);
+      tc::bar_init(&vfull[i], 1);
+      tc::bar_init(&vempty[i], 1);
+    }
+    for (int i = 0; i < NB; ++i) {
+      tc::bar_init(&s_done[i], 1);
+      tc::bar_init(&p_ready[i], 32 * kSoftWarps);
+    }
+    tc::bar_init(&o_done, 1);
+    tc::bar_init(&o_free, 32 * kSoftWarps);
+    tc::bar_init(&q_ready, 32 * kSoftWarps);
+    tc::bar_init(&fin, 1);
+    abort_flag = 0;
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+  }
+  if (warp == kSoftWarps + 1) tc::tmem_alloc(&tmem_slot, C::kTmem);
+  tc::tc_fence_before();
+  __syncthreads();
+  tc::tc_fence_after();
+  const uint32_t tmem = tmem_slot;
+  auto wait = [&](uint64_t* b, int phase) {
+    return tc::bar_wait(b, (uint32_t)(phase & 1), &abort_flag, &g_prompt_error);
+  };
+
+  if (warp == kSoftWarps) {
+    // ---- the tiles, by one thread
+    if (lane == 0) {
+      pdl_wait();
+      asm volatile("fence.proxy.async.global;" ::: "memory");
+      int nk = 0, nv = 0;  // copies issued
+      for (int j = 0; j < nt; ++j) {
+        const int st = j % ST;
+        unsigned char* dst = smem + st * C::kImage;
+        const unsigned char* src = images + j * image_step;
+        if (j >= ST && !wait(&kempty[st], j / ST - 1)) break;
+        tc::bar_expect_tx(&kfull[st], C::kOperand);
+        bulk_load(dst, src, C::kOperand, &kfull[st]);
+        ++nk;
+        if (j >= ST && !wait(&vempty[st], j / ST - 1)) break;
+        tc::bar_expect_tx(&vfull[st], C::kOperand);
+        bulk_load(dst + C::kOperand, src + C::kOperand, C::kOperand, &vfull[st]);
+        ++nv;
+      }
+      if (abort_flag) {  // copies in flight land before the CTA ends
+        const unsigned long long begin = tc::now_ns();
+        for (int j = max(0, nk - ST); j < nk; ++j)
+          while (!tc::bar_try(&kfull[j % ST], (uint32_t)(j / ST) & 1) &&
+                 tc::now_ns() - begin < tc::kWaitNs) {
+          }
+        for (int j = max(0, nv - ST); j < nv; ++j)
+          while (!tc::bar_try(&vfull[j % ST], (uint32_t)(j / ST) & 1) &&
+                 tc::now_ns() - begin < tc::kWaitNs) {
+          }
+      }
+    }
+    __syncwarp();
+  } else if (warp == kSoftWarps + 1) {
+    // ---- the products, by one thread
+    if (tc::elect_one()) {
+      constexpr uint32_t kIdescS = tc::idesc_f16(kRows, kKeys), kIdescO = tc::idesc_f16(kRows, DP);
+      auto scores = [&](int j) {
+        const uint32_t d = tmem + C::kColS + 64u * (j % NB), q = tmem + C::kColQ;
+        const uint32_t base = tc::su32(smem + (j % ST) * C::kImage);
+#pragma unroll
+        for (int k = 0; k < DP / 16; ++k) {
+          // a K = 16 slice: 8 TMEM columns of A, 32 bytes (+2) of the descriptor
+          const uint32_t off = (k / 4) * (kKeys * 128);
+          const uint64_t hi = tc::smem_desc(base + off) + 2u * (k % 4);
+          const uint64_t lo = tc::smem_desc(base + off + C::kPlane) + 2u * (k % 4);
+          tc::mma_f16_ts(d, q + 8u * k, hi, kIdescS, k > 0 ? 1u : 0u);
+          tc::mma_f16_ts(d, q + 8u * k, lo, kIdescS, 1u);
+          tc::mma_f16_ts(d, q + DP / 2 + 8u * k, hi, kIdescS, 1u);
+        }
+        tc::mma_commit(&s_done[j % NB]);
+        tc::mma_commit(&kempty[j % ST]);
+      };
+      bool ok = wait(&q_ready, 0) && wait(&kfull[0], 0);
+      tc::tc_fence_after();
+      if (ok) scores(0);
+      for (int j = 0; ok && j < nt; ++j) {
+        if (j + 1 < nt) {
+          ok = wait(&kfull[(j + 1) % ST], (j + 1) / ST);
+          // S(j+1) goes over P(j+1-NB), which O'(j+1-NB) has to have read: with
+          // three buffers o_free of that product was waited for before O'(j-1)
+          if (ok && NB == 2 && j > 0) ok = wait(&o_done, j - 1);
+          if (!ok) break;
+          tc::tc_fence_after();
+          scores(j + 1);
+        }
+        ok = wait(&vfull[j % ST], j / ST) && wait(&p_ready[j % NB], j / NB) &&
+             (j == 0 || wait(&o_free, j - 1));
+        if (!ok) break;
+        tc::tc_fence_after();
+        const uint32_t p = tmem + C::kColS + 64u * (j % NB), d = tmem + C::kColO;
+        const uint32_t base = tc::su32(smem + (j % ST) * C::kImage + C::kOperand);
+        const uint64_t hi = tc::smem_desc(base), lo = tc::smem_desc(base + C::kPlane);
+#pragma unroll
+        for (int k = 0; k < kKeys / 16; ++k) {
+          tc::mma_f16_ts(d, p + 8u * k, hi + 2u * k, kIdescO, k > 0 ? 1u : 0u);
+          tc::mma_f16_ts(d, p + 8u * k, lo + 2u * k, kIdescO, 1u);
+          tc::mma_f16_ts(d, p + 32 + 8u * k, hi + 2u * k, kIdescO, 1u);
+        }
+        tc::mma_commit(&o_done);
+        tc::mma_commit(&vempty[j % ST]);
+      }
+      tc::mma_commit(&fin);
+    }
+    __syncwarp();
+  } else {
+    // ---- the softmax.  After a wait that ran out the warps go on to the end
+    // without waiting (their pairs meet at barriers) and store nothing.
+    const int quarter = warp & 3, half = warp >> 2;
+    const int row = 32 * quarter + lane;
+    const uint32_t lanes = (uint32_t)(32 * quarter) << 16;
+    const int64_t f = f0 + row;
+    const bool valid = f < rows;
+    const int tok = valid ? (int)(f / a.group) : -1;
+    const int head = kvh * a.group + (int)(f % a.group);
+    const float* qrow = a.q + (int64_t)(t0 + max(tok, 0)) * a.ldq + (int64_t)head * a.head_dim;
+
+    float fq;  // scores in base 2: S' fq 2^ek
+    {
+      float4 x[W / 4];
+      float top = 0.0f;
+#pragma unroll
+      for (int i = 0; i < W / 4; ++i) {
+        const int d = half * W + 4 * i;
+        x[i] = valid && d < a.head_dim ? *reinterpret_cast<const float4*>(qrow + d)
+                                       : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+        top = fmaxf(top, fmaxf(fmaxf(fabsf(x[i].x), fabsf(x[i].y)), fmaxf(fabsf(x[i].z), fabsf(x[i].w))));
+      }
+      red[0][half][row] = top;
+      pair_sync(quarter);
+      top = fmaxf(red[0][0][row], red[0][1][row]);
+      const int e = pow2_ex(top);
+      const float down = pow2f(-e);
+      fq = pow2f(e) * a.scale;
+      uint32_t hi[W / 2], lo[W / 2];
+#pragma unroll
+      for (int i = 0; i < W / 4; ++i) {
+        split2(x[i].x * down, x[i].y * down, hi[2 * i], lo[2 * i]);
+        split2(x[i].z * down, x[i].w * down, hi[2 * i + 1], lo[2 * i + 1]);
+      }
+      tmem_st_n(tmem + lanes + C::kColQ + half * (W / 2), hi);
+      tmem_st_n(tmem + lanes + C::kColQ + DP / 2 + half * (W / 2), lo);
+      tc::tmem_wait_st();
+      tc::tc_fence_before();
+      tc::bar_arrive(&q_ready);
+      pair_sync(quarter);  // red is written again below
+    }
+
+    pdl_wait();  // meta
+    float o[W];
+#pragma unroll
+    for (int d = 0; d < W; ++d) o[d] = 0.0f;
+    float m = -INFINITY, l = 0.0f, corr = 1.0f, vscale = 0.0f;
+    // O'(j): o = o corr(j) + O'(j) 2^ev(j)
+    auto take_output = [&](int j) {
+      wait(&o_done, j);
+      tc::tc_fence_after();
+#pragma unroll
+      for (int c = 0; c < W; c += 32) {
+        uint32_t r[32];
+        tc::tmem_ld32(tmem + lanes + C::kColO + half * W + c, r);
+        tc::tmem_wait_ld();
+#pragma unroll
+        for (int d = 0; d < 32; ++d)
+          o[c + d] = fmaf(__uint_as_float(r[d]), vscale, o[c + d] * corr);
+      }
+      tc::tc_fence_before();
+      tc::bar_arrive(&o_free);
+    };
+    float4 next = __ldcg(meta);
+    for (int j = 0; j < nt; ++j) {
+      const float4 mt = next;
+      if (j + 1 < nt) next = __ldcg(meta + (int64_t)(j + 1) * a.n_kv_heads);
+      const int kt = j * kKeys;
+      const uint32_t buf = tmem + lanes + C::kColS + 64u * (j % NB);
+      wait(&s_done[j % NB], j / NB);
+      tc::tc_fence_after();
+      uint32_t r[32];
+      tc::tmem_ld32(buf + 32 * half, r);
+      tc::tmem_wait_ld();
+      const bool slow = mt.z != 0.0f;  // the whole CTA's
+      float tmax = -INFINITY;
+      if (kt + kKeys - 1 <= first_tok) {  // every key is visible to every row
+#pragma unroll
+        for (int i = 0; i < 32; ++i) tmax = fmaxf(tmax, __uint_as_float(r[i]));
+      } else {
+#pragma unroll
+        for (int i = 0; i < 32; ++i) {
+          if (kt + 32 * half + i > tok) r[i] = 0xff800000u;  // -inf
+          tmax = fmaxf(tmax, __uint_as_float(r[i]));
+        }
+      }
+      red[j & 1][half][row] = tmax;
+      pair_sync(quarter);
+      tmax = fmaxf(red[j & 1][0][row], red[j & 1][1][row]);
+      const float fs = fq * mt.x;
+      const float mnew = slow ? m : fmaxf(m, tmax * fs);
+      const float ref = mnew == -INFINITY ? 0.0f : mnew;
+      const float c = exp2f(m - ref);
+      m = mnew;
+      uint32_t ph[16], pl[16];
+      float sum = 0.0f;
+#pragma unroll
+      for (int i = 0; i < 16; ++i) {
+        float p0 = exp2f(fmaf(__uint_as_float(r[2 * i]), fs, 14.0f - ref));
+        float p1 = exp2f(fmaf(__uint_as_float(r[2 * i + 1]), fs, 14.0f - ref));
+        if (slow) p0 = p1 = 0.0f;
+        sum += p0;
+        sum += p1;
+        split2(p0, p1, ph[i], pl[i]);
+      }
+      if (!slow) l = fmaf(l, c, sum);
+      tc::tmem_st16(buf + 16 * half, ph);
+      tc::tmem_st16(buf + 32 + 16 * half, pl);
+      tc::tmem_wait_st();
+      tc::tc_fence_before();
+      tc::bar_arrive(&p_ready[j % NB]);
+      if (j > 0) take_output(j - 1);
+      corr = slow ? 1.0f : c;
+      vscale = mt.y;
+      if (slow && valid) {
+        // the marked tile in f32, key by key, from the inputs; o is at m's scale
+        for (int key = kt; key <= min(tok, kt + kKeys - 1); ++key) {
+          const float* kr = a.k + (int64_t)(t0 + key) * a.ldk + (int64_t)kvh * a.head_dim;
+          const float* vr = a.v + (int64_t)(t0 + key) * a.ldv + (int64_t)kvh * a.head_dim;
+          float s = 0.0f;
+          for (int d = 0; d < a.head_dim; ++d) s = fmaf(qrow[d], kr[d], s);
+          s *= a.scale;
+          const float top = fmaxf(m, s), at = top == -INFINITY ? 0.0f : top;
+          const float down = exp2f(m - at), p = exp2f(s - at + 14.0f);
+          l *= down;
+          if (half == 0) l += p;
+          m = top;
+#pragma unroll
+          for (int d = 0; d < W; ++d) {
+            const int dd = half * W + d;
+            o[d] = fmaf(p, dd < a.head_dim ? vr[dd] : 0.0f, o[d] * down);
+          }
+        }
+      }
+    }
+    take_output(nt - 1);
+    red[0][half][row] = l;
+    pair_sync(quarter);
+    l = red[0][0][row] + red[0][1][row];
+    if (valid && !abort_flag) {
+      float* y = a.out + (int64_t)(t0 + tok) * a.ldo + (int64_t)head * a.head_dim + half * W;
+#pragma unroll
+      for (int i = 0; i < W / 4; ++i)
+        if (half * W + 4 * i < a.head_dim)
+          *reinterpret_cast<float4*>(y + 4 * i) =
+              make_float4(__fdiv_rn(o[4 * i], l), __fdiv_rn(o[4 * i + 1], l),
+                          __fdiv_rn(o[4 * i + 2], l), __fdiv_rn(o[4 * i + 3], l));
+    }
+  }
+  tc::tc_fence_before();
+  __syncthreads();
+  if (warp == kSoftWarps + 1) {
+    // every product has completed before its tensor memory is freed
+    const unsigned long long begin = tc::now_ns();
+    while (!tc::bar_try(&fin, 0u)) {
+      if (tc::now_ns() - begin > tc::kWaitNs) {
+        atomicOr(&g_prompt_error, kErrTimeout);
+        break;
+      }
+    }
+    __syncwarp();
+    tc::tmem_free(tmem, C::kTmem);
+  }
+}
+
+// Key tiles that n_tokens tokens in n_seqs sequences can have.
+int64_t most_tiles(int n_tokens, int n_seqs) {
+  const int64_t t = (int64_t)n_tokens / kKeys + n_seqs;
+  return t < n_tokens ? t : n_tokens;
+}
+
+template <int DP>
+cudaError_t launch_prompt(const PromptArgs& a, int64_t row_tiles, cudaStream_t st) {
+  static DeviceOnce once;
+  cudaError_t e = once.run([] {
+    return cudaFuncSetAttribute(attention_prompt_kernel<DP>,
+                                cudaFuncAttributeMaxDynamicSharedMemorySize, Cfg<DP>::kSmem);
+  });
+  if (e != cudaSuccess) return e;
+  e = launch(prompt_split_kernel<DP>, dim3(a.max_tiles, a.n_kv_heads), dim3(kSplitThreads), 0, st,
+             false, a);
+  if (e != cudaSuccess) return e;
+  return launch(attention_prompt_kernel<DP>, dim3((unsigned)(row_tiles * a.n_kv_heads)),
+                dim3(kThreads), Cfg<DP>::kSmem, st, use_pdl(), a);
+}
+
+bool prompt_shape_ok(int n_heads, int n_kv_heads, int head_dim) {
+  return n_heads > 0 && n_kv_heads > 0 && n_heads % n_kv_heads == 0 && head_dim > 0;
+}
+size_t meta_bytes(int64_t tiles, int n_kv_heads) {
+  return ((size_t)tiles * n_kv_heads * sizeof(float4) + 255) / 256 * 256;
 }
 
 }  // namespace
@@ -123,16 +617,14 @@ cudaError_t read_prompt_error(unsigned int* flags, bool clear) {
 // ------------------------------------------------------------------ C ABI
 using namespace dqmk;
 
-namespace {
-bool prompt_shape_ok(int n_heads, int n_kv_heads, int head_dim) {
-  return n_heads > 0 && n_kv_heads > 0 && n_heads % n_kv_heads == 0 && head_dim > 0;
-}
-}  // namespace
-
 extern "C" size_t dqmk_attention_prompt_workspace(int n_tokens, int n_seqs, int n_heads,
                                                   int n_kv_heads, int head_dim) {
-  if (n_tokens <= 0 || n_seqs <= 0 || !prompt_shape_ok(n_heads, n_kv_heads, head_dim)) return 0;
-  return 16;
+  if (n_tokens <= 0 || n_seqs <= 0 || !prompt_shape_ok(n_heads, n_kv_heads, head_dim) ||
+      head_dim > kMaxDim)
+    return 0;
+  const int64_t tiles = most_tiles(n_tokens, n_seqs);
+  const size_t image = head_dim > 64 ? Cfg<128>::kImage : Cfg<64>::kImage;
+  return meta_bytes(tiles, n_kv_heads) + (size_t)tiles * n_kv_heads * image;
 }
 
 extern "C" int dqmk_attention_prompt(const float* q, int64_t ldq, const float* k, int64_t ldk,
@@ -166,10 +658,15 @@ extern "C" int dqmk_attention_prompt(const float* q, int64_t ldq, const float* k
   a.n_heads = n_heads, a.n_kv_heads = n_kv_heads, a.group = n_heads / n_kv_heads;
   a.head_dim = head_dim, a.out = out, a.ldo = ldo;
   a.scale = kLog2e / sqrtf((float)head_dim);
-  // blocks of a sequence round up, so at most one more than their share each
-  const int64_t blocks = ((int64_t)n_tokens * a.group) / kRows + n_seqs;
-  if (blocks > INT_MAX || n_kv_heads > 65535) return fail(DQMK_ERR_UNSUPPORTED, api + ": too many rows");
-  DQMK_CUDA_RET(api.c_str(), launch(attention_prompt_kernel, dim3((unsigned)blocks, n_kv_heads),
-                                    dim3(kThreads), 0, static_cast<cudaStream_t>(stream), false, a));
+  a.max_tiles = (int)most_tiles(n_tokens, n_seqs);
+  a.meta = static_cast<float4*>(workspace);
+  a.images = static_cast<unsigned char*>(workspace) + meta_bytes(a.max_tiles, n_kv_heads);
+  // a sequence's last tile of rows may be short: at most one more for each
+  const int64_t row_tiles = (int64_t)n_tokens * a.group / kRows + n_seqs;
+  if (row_tiles * n_kv_heads > INT_MAX || n_kv_heads > 65535)
+    return fail(DQMK_ERR_UNSUPPORTED, api + ": too many rows");
+  cudaStream_t st = static_cast<cudaStream_t>(stream);
+  DQMK_CUDA_RET(api.c_str(), head_dim > 64 ? launch_prompt<128>(a, row_tiles, st)
+                                           : launch_prompt<64>(a, row_tiles, st));
   return DQMK_OK;
 }

@@ -130,6 +130,28 @@ __device__ __forceinline__ float warp_max(float v) {
   return v;
 }
 
+// Sum of `x` over the CTA's threads, and in *before the sum over the threads
+// before this one; warp_sums: shared memory, one entry a warp.  All threads call.
+__device__ __forceinline__ int64_t block_scan(int64_t x, int64_t* before, int64_t* warp_sums) {
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, warps = blockDim.x >> 5;
+  int64_t incl = x;
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const int64_t y = __shfl_up_sync(0xffffffffu, incl, o);
+    if (lane >= o) incl += y;
+  }
+  __syncthreads();  // warp_sums may still be read from the last call
+  if (lane == 31) warp_sums[warp] = incl;
+  __syncthreads();
+  int64_t base = 0, total = 0;
+  for (int w = 0; w < warps; ++w) {
+    if (w < warp) base += warp_sums[w];
+    total += warp_sums[w];
+  }
+  *before = base + incl - x;
+  return total;
+}
+
 // Total-order key for a float so that unsigned max == float max; among equal
 // values the smaller index wins (the reference's ArgMax keeps the first max,
 // src/ops.cc:182-195).

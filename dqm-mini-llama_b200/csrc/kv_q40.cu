@@ -296,27 +296,6 @@ __device__ __forceinline__ float half_at(uint32_t w, int i) {
   return h2f((uint16_t)(i ? w >> 16 : w));
 }
 
-// Sum over the CTA of `x`, and the sum over the threads before this one.
-__device__ __forceinline__ int64_t block_scan(int64_t x, int64_t* before, int64_t* warp_sums) {
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, warps = blockDim.x >> 5;
-  int64_t incl = x;
-#pragma unroll
-  for (int o = 1; o < 32; o <<= 1) {
-    const int64_t y = __shfl_up_sync(0xffffffffu, incl, o);
-    if (lane >= o) incl += y;
-  }
-  __syncthreads();  // warp_sums may still be read from the last call
-  if (lane == 31) warp_sums[warp] = incl;
-  __syncthreads();
-  int64_t base = 0, total = 0;
-  for (int w = 0; w < warps; ++w) {
-    if (w < warp) base += warp_sums[w];
-    total += warp_sums[w];
-  }
-  *before = base + incl - x;
-  return total;
-}
-
 template <int NB>
 __global__ void __launch_bounds__(kThreads, 3) kv_q40_attention_kernel(const AttnQ40Args a) {
   using S = Shape<NB>;

@@ -333,16 +333,6 @@ def CudaAttentionDecodeDeviceInput(q, kv: CudaKvCache, layer: int, pos: int, n_h
 
 
 # ------------------------------------------------------------ attention block
-class _Here:
-    """A call on the current device and stream."""
-
-    def __enter__(self):
-        return _torch().cuda.current_stream().cuda_stream
-
-    def __exit__(self, *exc):
-        pass
-
-
 class _There:
     """A call on another device or a given stream: both are made current, so
     that outputs and workspaces are allocated for the stream that uses them."""
@@ -365,12 +355,23 @@ class _There:
             g.__exit__(*exc)
 
 
-_here = _Here()
+class _Here:
+    """A call on the current device and stream.  The raw handle comes from
+    torch's binding: current_stream() costs more than the launch."""
+
+    def __init__(self, index):
+        self.index = index
+
+    def __enter__(self):
+        return _torch()._C._cuda_getCurrentRawStream(self.index)
+
+    def __exit__(self, *exc):
+        pass
 
 
 def _on(device, stream):
-    if stream is None and device.index == _torch().cuda.current_device():
-        return _here
+    if stream is None and device.index == _torch()._C._cuda_getDevice():
+        return _Here(device.index)
     return _There(device, stream)
 
 

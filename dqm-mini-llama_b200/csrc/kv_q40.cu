@@ -3,17 +3,19 @@
 // Rows are quantized to Q4_0 blocks exactly as dqmk_quantize_q40 does (a
 // block of 32 values: fp16 scale d = absmax / 7, codes n = round(v / d + 8) in
 // 0..15, value d (n - 8)).  Each of the two buffers (keys, values) holds, for
-// every layer, slot and KV head, the rows of its positions one after the
-// other, first all quants, then all scales:
+// every layer, slot and KV head, its positions in tiles of 32, one after the
+// other; a tile is the quants of its 32 rows, then their scales:
 //
-//   quants [layer][slot][kv_head][rows][D/2 bytes]
-//   scales [layer][slot][kv_head][rows][D/32 fp16]     rows = max_seq up to 32
+//   [layer][slot][kv_head][tile]  quants [32][D/2 bytes], scales [16][D/32][2 fp16]
 //
-// so the positions that a query reads are one contiguous run a head.  Inside a
-// row the bytes of the blocks (byte j: value j low, value j + 16 high) are
+// so the positions that a query reads are one contiguous run a head and a tile
+// is one copy.  A block's scales of two neighbouring rows make one pair of
+// halves.  The bytes of the blocks (byte j: value j low, value j + 16 high) are
 // interleaved so that one thread's share of a matrix operand is contiguous:
-//   keys    4-byte words [t][block], word t = bytes 4t .. 4t+3 of the block
-//   values  2-byte units [g][block], unit g = bytes 2g, 2g+1 of the block
+//   keys    a row: 4-byte words [t][block], word t = bytes 4t .. 4t+3 of the block
+//   values  two neighbouring rows: [g][block][row] units of 2 bytes, unit g =
+//           bytes 2g, 2g+1 of the block; the 8 parts g of row pair r are turned
+//           by 2r, so that 4 pairs lie in different shared-memory banks
 #include <climits>
 
 #include "common.cuh"
@@ -26,23 +28,23 @@ namespace {
 __device__ unsigned int g_kv_error;  // kErrTimeout / kErrBadIndex
 
 constexpr int kMaxBlocks = 4;  // 32-value blocks of a row: head_dim at most 128
+constexpr int kTile = 32;      // positions of a tile
 
-__host__ __device__ __forceinline__ int64_t padded_rows(int max_seq) {
-  return ((int64_t)max_seq + 31) / 32 * 32;
+__host__ __device__ __forceinline__ int64_t tiles_of(int max_seq) {
+  return ((int64_t)max_seq + kTile - 1) / kTile;
 }
+// Bytes of a tile: 18 for a block.
+__host__ __device__ constexpr int tile_bytes(int nb) { return kTile * 18 * nb; }
 
 // One layer of the cache.
 struct Plane {
-  uint8_t* kq;
-  uint16_t* kd;
-  uint8_t* vq;
-  uint16_t* vd;
+  unsigned char *k, *v;
   int n_slots, max_seq, n_kv_heads, nb;
-  int64_t rows;  // padded rows of one head
+  int64_t tiles;  // of one head
 };
 
-__device__ __forceinline__ int64_t plane_row(const Plane& c, int slot, int head, int pos) {
-  return ((int64_t)slot * c.n_kv_heads + head) * c.rows + pos;
+__device__ __forceinline__ int64_t first_tile(const Plane& c, int slot, int head) {
+  return ((int64_t)slot * c.n_kv_heads + head) * c.tiles;
 }
 
 // --------------------------------------------------------- write and read
@@ -55,6 +57,20 @@ struct RowsArgs {
   int n_tokens;
 };
 
+// Offset in its buffer of word t (0..3) of block b of a key row, of unit g
+// (0..7) of block b of a value row, and of a block's scale.
+__device__ __forceinline__ int64_t key_at(int64_t row, int t, int b, int nb) {
+  return (row / kTile) * tile_bytes(nb) + (row % kTile) * (16 * nb) + (t * nb + b) * 4;
+}
+__host__ __device__ __forceinline__ int value_part(int pair, int g) { return (g + 2 * pair) & 7; }
+__device__ __forceinline__ int64_t value_at(int64_t row, int g, int b, int nb) {
+  const int r = (int)(row % kTile), pair = r >> 1;
+  return (row / kTile) * tile_bytes(nb) + pair * (32 * nb) + (value_part(pair, g) * nb + b) * 4 + (r & 1) * 2;
+}
+__device__ __forceinline__ int64_t scale_at(int64_t row, int b, int nb) {
+  return (row / kTile) * tile_bytes(nb) + kTile * 16 * nb + ((row % kTile / 2) * nb + b) * 4 + (row & 1) * 2;
+}
+
 // The cache row a token names, or -1: a padding token (position -1), or a slot
 // or position outside the cache, which is recorded.
 __device__ __forceinline__ int64_t token_row(const RowsArgs& a, int token, int head) {
@@ -64,7 +80,7 @@ __device__ __forceinline__ int64_t token_row(const RowsArgs& a, int token, int h
     atomicOr(&g_kv_error, kErrBadIndex);
     return -1;
   }
-  return plane_row(a.c, slot, head, pos);
+  return first_tile(a.c, slot, head) * kTile + pos;
 }
 
 // 8 lanes take one block, 4 values each.  VEC: 16-byte accesses to the f32
@@ -117,16 +133,16 @@ __global__ void __launch_bounds__(256) kv_q40_write_kernel(RowsArgs a) {
     const int64_t row = live ? token_row(a, token, head) : -1;
     if (row < 0) continue;
     const uint32_t word = codes | high << 4;
+    unsigned char* base = is_v ? a.c.v : a.c.k;
     if (i8 < 4) {
       if (is_v) {
-        uint16_t* u = reinterpret_cast<uint16_t*>(a.c.vq + row * (16 * nb));
-        u[2 * i8 * nb + b] = (uint16_t)word;
-        u[(2 * i8 + 1) * nb + b] = (uint16_t)(word >> 16);
+        *reinterpret_cast<uint16_t*>(base + value_at(row, 2 * i8, b, nb)) = (uint16_t)word;
+        *reinterpret_cast<uint16_t*>(base + value_at(row, 2 * i8 + 1, b, nb)) = (uint16_t)(word >> 16);
       } else {
-        reinterpret_cast<uint32_t*>(a.c.kq + row * (16 * nb))[i8 * nb + b] = word;
+        *reinterpret_cast<uint32_t*>(base + key_at(row, i8, b, nb)) = word;
       }
     }
-    if (i8 == 0) (is_v ? a.c.vd : a.c.kd)[row * nb + b] = d;
+    if (i8 == 0) *reinterpret_cast<uint16_t*>(base + scale_at(row, b, nb)) = d;
   }
 }
 
@@ -147,14 +163,15 @@ __global__ void __launch_bounds__(256) kv_q40_read_kernel(RowsArgs a) {
     const int64_t row = token_row(a, token, head);
     if (row < 0) continue;
     uint32_t word;
+    const unsigned char* base = is_v ? a.c.v : a.c.k;
     if (is_v) {
-      const uint16_t* u = reinterpret_cast<const uint16_t*>(a.c.vq + row * (16 * nb));
-      word = u[2 * t * nb + b] | (uint32_t)u[(2 * t + 1) * nb + b] << 16;
+      word = *reinterpret_cast<const uint16_t*>(base + value_at(row, 2 * t, b, nb)) |
+             (uint32_t)*reinterpret_cast<const uint16_t*>(base + value_at(row, 2 * t + 1, b, nb)) << 16;
     } else {
-      word = reinterpret_cast<const uint32_t*>(a.c.kq + row * (16 * nb))[t * nb + b];
+      word = *reinterpret_cast<const uint32_t*>(base + key_at(row, t, b, nb));
     }
     if (i8 >= 4) word >>= 4;
-    const float d = h2f((is_v ? a.c.vd : a.c.kd)[row * nb + b]);
+    const float d = h2f(*reinterpret_cast<const uint16_t*>(base + scale_at(row, b, nb)));
     float y[4];
 #pragma unroll
     for (int e = 0; e < 4; ++e) y[e] = __fmul_rn(d, (float)(int)((word >> (8 * e)) & 15u) - 8.0f);
@@ -185,14 +202,17 @@ __global__ void __launch_bounds__(256) kv_q40_read_kernel(RowsArgs a) {
 //   output   A = w = p d_b 2^(15-E), B = codes n - 8 (columns of V):
 //            O[c] = 2^(E-15) sum_j w_j (n_jc - 8), a block's channels at a time
 // E is a running bound of the exponents of V's scales, kept like the running
-// maximum of the scores: when it grows, the sums are scaled down.
+// maximum of the scores: when it grows, the sums are scaled down.  The terms of
+// w come from p = ph + pl and d in fp16 arithmetic: hi = ph d, lo = (ph d - hi)
+// + pl d, whose first part a fused multiply-add leaves exact.
 //
 // A code becomes a half by one AND/OR, (w & 0x000f) | 0x6400 = 1024 + n, and
 // one addition that centres it: n - 8 (16 (n - 8) from a high nibble; its
 // channel of q takes 1/16).  The code's own bits are n 2^-24 as a subnormal
 // half and would need neither, but the products align their sums by the
-// operands' exponent fields, and 10 bits of every sum are lost (measured: 2e-6
-// of the output against 3e-7).
+// operands' exponent fields, and 10 bits of every sum are lost.  For the same
+// reason (the accumulators round towards zero) a tile's products start from
+// zero and are added to the running sums in f32.
 //
 // Bound: 18 bytes for 32 values, each used by every head of the group; at the
 // memory rate an SM has about 1.4 instruction slots a value, and the unpacking,
@@ -203,8 +223,8 @@ __global__ void __launch_bounds__(256) kv_q40_read_kernel(RowsArgs a) {
 // CTA that holds only part of a (column, group)'s chunks leaves its partial
 // sums in the workspace for a second kernel.  Each warp streams its own tiles
 // of 32 positions through a ring of bulk copies.
-constexpr int kWarps = 4, kThreads = 32 * kWarps, kTile = 32, kChunk = kTile * kWarps;
-constexpr int kStages = 3, kGroup = 8;
+constexpr int kWarps = 4, kThreads = 32 * kWarps, kChunk = kTile * kWarps;
+constexpr int kStages = 3, kGroup = 8, kCtasPerSm = 3;
 constexpr float kLog2e = 1.44269504088896341f;
 
 struct AttnQ40Args {
@@ -217,26 +237,25 @@ struct AttnQ40Args {
   int n_cols, n_heads, group, subs;  // subs: (KV head, 8-head group) pairs of a column
   float scale;                       // log2(e) / sqrt(D)
   float* part;                       // [CTA][2][part_floats]
-  int n_ctas;                        // CTAs of the first kernel
+  int2* spans;                       // [column][sub]: first and last CTA
 };
 
 template <int NB>
 struct Shape {
   static constexpr int kD = 32 * NB;
-  static constexpr int kQuantBytes = kTile * 16 * NB, kScaleBytes = kTile * 2 * NB;
-  static constexpr int kStageBytes = 2 * (kQuantBytes + kScaleBytes);
+  static constexpr int kTileBytes = tile_bytes(NB), kQuantBytes = kTile * 16 * NB;
+  static constexpr int kStageBytes = 2 * kTileBytes;
   static constexpr int kPartFloats = kGroup * (kD + 2);
 };
 
 // Visible positions of a column: 0 for a length or slot outside the cache.
-__device__ __forceinline__ int visible(const AttnQ40Args& a, int col) {
-  const int n = a.lengths[col];
-  const int s = a.slots ? a.slots[col] : col;
-  return n > 0 && n <= a.c.max_seq && s >= 0 && s < a.c.n_slots ? n : 0;
+__device__ __forceinline__ int visible(const AttnQ40Args& a, int n, int slot) {
+  return n > 0 && n <= a.c.max_seq && slot >= 0 && slot < a.c.n_slots ? n : 0;
 }
-__device__ __forceinline__ int64_t units_of(const AttnQ40Args& a, int len) {
-  return (int64_t)((len + kChunk - 1) / kChunk) * a.subs;
+__device__ __forceinline__ int slot_of(const AttnQ40Args& a, int col) {
+  return a.slots ? a.slots[col] : col;
 }
+__device__ __forceinline__ int chunks_of(int len) { return (len + kChunk - 1) / kChunk; }
 // The CTA whose run of the `total` units holds unit u: run i is
 // [i total / n, (i + 1) total / n).
 __device__ __forceinline__ int cta_of(int64_t u, int64_t total, int n) {
@@ -244,11 +263,23 @@ __device__ __forceinline__ int cta_of(int64_t u, int64_t total, int n) {
 }
 
 __device__ __forceinline__ void mma16816(float (&d)[4], const uint4& a, uint32_t b0, uint32_t b1) {
-  asm volatile(
+  asm(
       "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, "
       "{%0,%1,%2,%3};"
       : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
       : "r"(a.x), "r"(a.y), "r"(a.z), "r"(a.w), "r"(b0), "r"(b1));
+}
+// The same without an addend.
+__device__ __forceinline__ void mma16816_first(float (&d)[4], const uint4& a, uint32_t b0, uint32_t b1) {
+  asm(
+      "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, "
+      "{%10,%10,%10,%10};"
+      : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3])
+      : "r"(a.x), "r"(a.y), "r"(a.z), "r"(a.w), "r"(b0), "r"(b1), "f"(0.0f));
+}
+// High and low term rows of a product, added: columns 2t and 2t + 1.
+__device__ __forceinline__ unsigned long long both_terms(const float (&c)[4]) {
+  return fadd2(f2_pack(c[0], c[1]), f2_pack(c[2], c[3]));
 }
 __device__ __forceinline__ void bulk_load(void* dst, const void* src, uint32_t bytes, uint64_t* bar) {
   asm volatile(
@@ -257,27 +288,34 @@ __device__ __forceinline__ void bulk_load(void* dst, const void* src, uint32_t b
       "l"(src), "r"(bytes), "r"(tc::su32(bar))
       : "memory");
 }
+__device__ __forceinline__ __half2 as_h2(uint32_t x) { return *reinterpret_cast<const __half2*>(&x); }
+__device__ __forceinline__ uint32_t bits(__half2 x) { return *reinterpret_cast<const uint32_t*>(&x); }
 // Two values to packed fp16 pairs with x = hi + lo + r, |r| <= 2^-22 |x|.
-__device__ __forceinline__ void split2(float x0, float x1, uint32_t& hi, uint32_t& lo) {
-  const __half2 h = __floats2half2_rn(x0, x1);
-  const float2 back = __half22float2(h);
-  const __half2 l = __floats2half2_rn(__fsub_rn(x0, back.x), __fsub_rn(x1, back.y));
-  hi = *reinterpret_cast<const uint32_t*>(&h);
-  lo = *reinterpret_cast<const uint32_t*>(&l);
+__device__ __forceinline__ void split2(float x0, float x1, __half2& hi, __half2& lo) {
+  hi = __floats2half2_rn(x0, x1);
+  const float2 back = __half22float2(hi);
+  lo = __floats2half2_rn(__fsub_rn(x0, back.x), __fsub_rn(x1, back.y));
 }
 // The codes in bits 0-3 and 16-19 of a word as the halves n - 8, and those in
 // bits 4-7 and 20-23 as 16 (n - 8).
-__device__ __forceinline__ uint32_t add_h2(uint32_t x, uint32_t y) {
-  const __half2 z = __hadd2(*reinterpret_cast<const __half2*>(&x), *reinterpret_cast<const __half2*>(&y));
-  return *reinterpret_cast<const uint32_t*>(&z);
+__device__ __forceinline__ uint32_t and_or(uint32_t w, uint32_t mask, uint32_t with) {
+  uint32_t r;
+  asm("lop3.b32 %0, %1, %2, %3, 0xea;" : "=r"(r) : "r"(w), "r"(mask), "r"(with));
+  return r;
 }
 __device__ __forceinline__ uint32_t codes_low(uint32_t w) {
-  return add_h2((w & 0x000f000fu) | 0x64006400u, 0xe408e408u);  // -1032
+  return bits(__hadd2(as_h2(and_or(w, 0x000f000fu, 0x64006400u)), as_h2(0xe408e408u)));  // -1032
 }
 __device__ __forceinline__ uint32_t codes_high(uint32_t w) {
-  return add_h2((w & 0x00f000f0u) | 0x64006400u, 0xe480e480u);  // -1152
+  return bits(__hadd2(as_h2(and_or(w, 0x00f000f0u, 0x64006400u)), as_h2(0xe480e480u)));  // -1152
 }
 __device__ __forceinline__ float pow2f(int e) { return __int_as_float((127 + e) << 23); }
+// 2^x; results below 2^-126 are 0.
+__device__ __forceinline__ float ex2(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
 
 template <int N>
 __device__ __forceinline__ void lds_words(uint32_t (&r)[N], const void* p) {
@@ -292,12 +330,9 @@ __device__ __forceinline__ void lds_words(uint32_t (&r)[N], const void* p) {
     for (int i = 0; i < N; ++i) r[i] = static_cast<const uint32_t*>(p)[i];
   }
 }
-__device__ __forceinline__ float half_at(uint32_t w, int i) {
-  return h2f((uint16_t)(i ? w >> 16 : w));
-}
 
 template <int NB>
-__global__ void __launch_bounds__(kThreads, 3) kv_q40_attention_kernel(const AttnQ40Args a) {
+__global__ void __launch_bounds__(kThreads, kCtasPerSm) kv_q40_attention_kernel(const AttnQ40Args a) {
   using S = Shape<NB>;
   constexpr int D = S::kD;
   extern __shared__ __align__(128) unsigned char smem[];
@@ -308,7 +343,7 @@ __global__ void __launch_bounds__(kThreads, 3) kv_q40_attention_kernel(const Att
   __shared__ int red_e[kWarps];
   __shared__ int64_t warp_sums[kWarps];
   __shared__ int64_t s_first;
-  __shared__ int s_col;
+  __shared__ int s_col, s_len, s_slot;
   __shared__ volatile int abort_flag;
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const int g = lane >> 2, t = lane & 3;
@@ -319,46 +354,53 @@ __global__ void __launch_bounds__(kThreads, 3) kv_q40_attention_kernel(const Att
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
 
-  // ---- this CTA's run of the chunk list
-  int64_t total = 0;
-  for (int c0 = 0; c0 < a.n_cols; c0 += kThreads) {
+  // ---- this CTA's run of the chunk list: the list's length, then the column
+  // that holds the run's first unit
+  int64_t total = 0, before = 0, mine_units = 0;
+  int my_len = 0, my_slot = 0;
+  auto count = [&](int c0) {  // columns c0 + tid: units of those before, sum
     const int col = c0 + tid;
-    int64_t before;
-    const int len = col < a.n_cols ? visible(a, col) : 0;
-    total += block_scan(units_of(a, len), &before, warp_sums);
-    // columns that see nothing: their rows are zero, shared out over the CTAs
-    if (col < a.n_cols && blockIdx.x == 0) {
-      const int n = a.lengths[col], s = a.slots ? a.slots[col] : col;
-      if (n < 0 || n > a.c.max_seq || s < 0 || s >= a.c.n_slots) atomicOr(&g_kv_error, kErrBadIndex);
+    int n = 0;
+    my_slot = 0, my_len = 0;
+    if (col < a.n_cols) {
+      n = a.lengths[col];
+      my_slot = slot_of(a, col);
+      my_len = visible(a, n, my_slot);
+      if (my_len != n && blockIdx.x == 0) atomicOr(&g_kv_error, kErrBadIndex);
     }
-  }
-  for (int col = blockIdx.x; col < a.n_cols; col += gridDim.x)
-    if (visible(a, col) == 0)
-      for (int i = tid; i < a.n_heads * D; i += kThreads) a.out[col * a.ldo + i] = 0.0f;
+    mine_units = (int64_t)chunks_of(my_len) * a.subs;
+    return block_scan(mine_units, &before, warp_sums);
+  };
+  for (int c0 = 0; c0 < a.n_cols; c0 += kThreads) total += count(c0);
+  // columns that see nothing have no units; their rows are zero
+  auto zero_rows = [&] {
+    for (int c = blockIdx.x; c < a.n_cols; c += gridDim.x)
+      if (visible(a, a.lengths[c], slot_of(a, c)) == 0)
+        for (int i = tid; i < a.n_heads * D; i += kThreads) a.out[c * a.ldo + i] = 0.0f;
+  };
   const int n_ctas = (int)min((int64_t)gridDim.x, total);
   if ((int)blockIdx.x >= n_ctas) {
     pdl_trigger();
+    zero_rows();
     return;
   }
   const int64_t u0 = blockIdx.x * total / n_ctas, u1 = (blockIdx.x + 1) * total / n_ctas;
   {
     int64_t run = 0;
-    for (int c0 = 0; c0 < a.n_cols; c0 += kThreads) {
-      const int col = c0 + tid;
-      int64_t before;
-      const int64_t x = col < a.n_cols ? units_of(a, visible(a, col)) : 0;
-      const int64_t sum = block_scan(x, &before, warp_sums);
-      before += run;
-      if (before <= u0 && u0 < before + x) {
-        s_col = col;
-        s_first = before;
+    for (int c0 = 0; run <= u0; c0 += kThreads) {
+      // up to kThreads columns the counts are still there
+      const int64_t sum = a.n_cols > kThreads ? count(c0) : total;
+      if (run + before <= u0 && u0 < run + before + mine_units) {
+        s_col = c0 + tid;
+        s_len = my_len;
+        s_slot = my_slot;
+        s_first = run + before;
       }
       run += sum;
-      if (run > u0) break;
     }
   }
   __syncthreads();
-  int col = s_col;
+  int col = s_col, len = s_len, slot = s_slot;
   int64_t first = s_first;  // unit 0 of the column
 
   unsigned char* ring = smem + (size_t)warp * kStages * S::kStageBytes;
@@ -367,20 +409,20 @@ __global__ void __launch_bounds__(kThreads, 3) kv_q40_attention_kernel(const Att
   bool ok = true;
 
   for (int64_t u = u0; u < u1 && ok;) {
-    const int len = visible(a, col);
-    const int chunks = (len + kChunk - 1) / kChunk;
+    const int chunks = chunks_of(len);
     const int64_t rel = u - first;
     if (rel >= (int64_t)chunks * a.subs) {  // past this column (or it is empty)
       first += (int64_t)chunks * a.subs;
       ++col;
+      slot = slot_of(a, col);
+      len = visible(a, a.lengths[col], slot);
       continue;
     }
     const int sub = (int)(rel / chunks), ch0 = (int)(rel % chunks);
     const int take = (int)min((int64_t)(chunks - ch0), u1 - u);
     const int kvh = sub % a.c.n_kv_heads, h0 = (sub / a.c.n_kv_heads) * kGroup;
     const int n_here = min(kGroup, a.group - h0);  // heads of this group
-    const int slot = a.slots ? a.slots[col] : col;
-    const int64_t row0 = plane_row(a.c, slot, kvh, 0);
+    const int64_t head_tile = first_tile(a.c, slot, kvh);
     const int tile_end = min((ch0 + take) * kWarps, (len + kTile - 1) / kTile);
     const int tile0 = ch0 * kWarps + warp;
     const int mine = tile0 < tile_end ? (tile_end - tile0 + kWarps - 1) / kWarps : 0;
@@ -388,88 +430,100 @@ __global__ void __launch_bounds__(kThreads, 3) kv_q40_attention_kernel(const Att
     auto issue = [&](int i) {  // lane 0: this warp's tile i of the piece
       unsigned char* st = ring + (issued % kStages) * S::kStageBytes;
       uint64_t* bar = &bars[warp][issued % kStages];
-      const int64_t row = row0 + (int64_t)(tile0 + i * kWarps) * kTile;
+      const int64_t at = (head_tile + tile0 + i * kWarps) * S::kTileBytes;
       tc::bar_expect_tx(bar, S::kStageBytes);
-      bulk_load(st, a.c.kq + row * (16 * NB), S::kQuantBytes, bar);
-      bulk_load(st + S::kQuantBytes, a.c.vq + row * (16 * NB), S::kQuantBytes, bar);
-      bulk_load(st + 2 * S::kQuantBytes, a.c.kd + row * NB, S::kScaleBytes, bar);
-      bulk_load(st + 2 * S::kQuantBytes + S::kScaleBytes, a.c.vd + row * NB, S::kScaleBytes, bar);
+      bulk_load(st, a.c.k + at, S::kTileBytes, bar);
+      bulk_load(st + S::kTileBytes, a.c.v + at, S::kTileBytes, bar);
     };
     for (int i = 0; i < min(mine, kStages); ++i) {
       if (lane == 0) issue(i);
       ++issued;
     }
 
-    // ---- the group's queries as A operands (high and low terms)
-    for (int hh = warp * 2; hh < warp * 2 + 2; ++hh) {
-      float x[NB], top = 0.0f;
+    // ---- the group's queries as A operands (high and low terms), two heads a warp
+    {
+      float x[2][NB];
 #pragma unroll
-      for (int b = 0; b < NB; ++b) {
-        const int64_t head = (int64_t)kvh * a.group + h0 + hh;
-        x[b] = hh < n_here ? a.q[col * a.ldq + head * D + 32 * b + lane] : 0.0f;
-        top = fmaxf(top, fabsf(x[b]));
-      }
-      top = warp_max(top);
-      // 2^-e brings the row's largest value into [2^14, 2^15)
-      const int e = top > 0.0f ? min(max(((__float_as_int(top) >> 23) & 0xff) - 141, -120), 120) : 0;
-      const bool high = lane >= 16;
-      const int jj = lane & 15, tq = jj >> 2, el = jj & 3;
+      for (int i = 0; i < 2; ++i)
 #pragma unroll
-      for (int b = 0; b < NB; ++b) {
-        // a high nibble stands for 16 (n - 8): its channel takes 1/16
-        const float v = x[b] * pow2f(-e) * (high ? 0.0625f : 1.0f);
-        const __half hi = __float2half_rn(v);
-        const __half lo = __float2half_rn(v - __half2float(hi));
-        __half* dst = reinterpret_cast<__half*>(&qfrag[b][el & 1][hh * 4 + tq]) + (high ? 4 : 0) + (el >> 1);
-        dst[0] = hi;
-        dst[2] = lo;
+        for (int b = 0; b < NB; ++b) {
+          const int hh = warp * 2 + i;
+          const int64_t head = (int64_t)kvh * a.group + h0 + hh;
+          x[i][b] = hh < n_here ? a.q[col * a.ldq + head * D + 32 * b + lane] : 0.0f;
+        }
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        const int hh = warp * 2 + i;
+        float top = 0.0f;
+#pragma unroll
+        for (int b = 0; b < NB; ++b) top = fmaxf(top, fabsf(x[i][b]));
+        top = warp_max(top);
+        // 2^-e brings the row's largest value into [2^14, 2^15)
+        const int e = top > 0.0f ? min(max(((__float_as_int(top) >> 23) & 0xff) - 141, -120), 120) : 0;
+        const bool high = lane >= 16;
+        const int jj = lane & 15, tq = jj >> 2, el = jj & 3;
+#pragma unroll
+        for (int b = 0; b < NB; ++b) {
+          // a high nibble stands for 16 (n - 8): its channel takes 1/16
+          const float v = x[i][b] * pow2f(-e) * (high ? 0.0625f : 1.0f);
+          const __half hi = __float2half_rn(v);
+          const __half lo = __float2half_rn(v - __half2float(hi));
+          __half* dst = reinterpret_cast<__half*>(&qfrag[b][el & 1][hh * 4 + tq]) + (high ? 4 : 0) + (el >> 1);
+          dst[0] = hi;
+          dst[2] = lo;
+        }
+        if (lane == 0) qscale[hh] = pow2f(e) * a.scale;
       }
-      if (lane == 0) qscale[hh] = pow2f(e) * a.scale;
     }
     __syncthreads();
 
-    float o[NB][4][4];
+    // running sums of head g: channels 4t + {0, 2}, {1, 3} of a block's halves
+    unsigned long long o[NB][4];
 #pragma unroll
     for (int b = 0; b < NB; ++b)
 #pragma unroll
-      for (int s = 0; s < 4; ++s)
-#pragma unroll
-        for (int r = 0; r < 4; ++r) o[b][s][r] = 0.0f;
+      for (int s = 0; s < 4; ++s) o[b][s] = 0ull;
     float m = -INFINITY, l = 0.0f;
     int ev = -20;  // V's scales so far are below 2^ev
     const float qs = qscale[g];
 
     for (int i = 0; i < mine; ++i) {
       const uint32_t stage = used % kStages;
-      const bool landed = tc::bar_wait(&bars[warp][stage], (used / kStages) & 1, &abort_flag, &g_kv_error);
-      ok = __all_sync(0xffffffffu, landed);
-      if (!ok) break;
+      uint64_t* bar = &bars[warp][stage];
+      const uint32_t phase = (used / kStages) & 1;
+      if (__any_sync(0xffffffffu, !tc::bar_try(bar, phase))) {
+        ok = __all_sync(0xffffffffu, tc::bar_wait(bar, phase, &abort_flag, &g_kv_error));
+        if (!ok) break;
+      }
       ++used;
       unsigned char* st = ring + stage * S::kStageBytes;
       const unsigned char* kq = st;
-      const unsigned char* vq = st + S::kQuantBytes;
-      uint16_t* kd = reinterpret_cast<uint16_t*>(st + 2 * S::kQuantBytes);
-      uint16_t* vd = kd + kTile * NB;
+      const unsigned char* vq = st + S::kTileBytes;
+      uint32_t* kd = reinterpret_cast<uint32_t*>(st + S::kQuantBytes);
+      uint32_t* vd = reinterpret_cast<uint32_t*>(st + S::kTileBytes + S::kQuantBytes);
       const int left = len - (tile0 + i * kWarps) * kTile;  // live positions of the tile
       if (left < kTile) {
         // rows past the end may hold anything: zero scales take them out
         if (lane >= left) {
 #pragma unroll
-          for (int b = 0; b < NB; ++b) kd[lane * NB + b] = vd[lane * NB + b] = 0;
+          for (int b = 0; b < NB; ++b) {
+            const int at = ((lane >> 1) * NB + b) * 2 + (lane & 1);
+            reinterpret_cast<uint16_t*>(kd)[at] = reinterpret_cast<uint16_t*>(vd)[at] = 0;
+          }
         }
         tc::fence_proxy_async_smem();
         __syncwarp();
       }
 
       // ---- scores of keys 8 j + 2 t + {0, 1} for head g
-      float s[4][2];
+      unsigned long long s2[4];
       {
         uint32_t kw[4][NB], dk[4][NB];
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
           lds_words<NB>(kw[j], kq + (8 * j + g) * (16 * NB) + t * (4 * NB));
-          lds_words<NB>(dk[j], kd + (8 * j + 2 * t) * NB);
-          s[j][0] = s[j][1] = 0.0f;
+          lds_words<NB>(dk[j], kd + (4 * j + t) * NB);
+          s2[j] = 0ull;
         }
 #pragma unroll
         for (int b = 0; b < NB; ++b) {
@@ -477,100 +531,94 @@ __global__ void __launch_bounds__(kThreads, 3) kv_q40_attention_kernel(const Att
 #pragma unroll
           for (int j = 0; j < 4; ++j) {
             const uint32_t w = kw[j][b], w8 = w >> 8;
-            float c[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-            mma16816(c, a0, codes_low(w), codes_high(w));
+            float c[4];
+            mma16816_first(c, a0, codes_low(w), codes_high(w));
             mma16816(c, a1, codes_low(w8), codes_high(w8));
-            // scales of keys 2t (halves 0 .. NB-1) and 2t + 1 (NB .. 2 NB - 1)
-            s[j][0] = fmaf(half_at(dk[j][b >> 1], b & 1), c[0] + c[2], s[j][0]);
-            s[j][1] = fmaf(half_at(dk[j][(NB + b) >> 1], (NB + b) & 1), c[1] + c[3], s[j][1]);
+            const float2 d = __half22float2(as_h2(dk[j][b]));
+            s2[j] = ffma2(f2_pack(d.x, d.y), both_terms(c), s2[j]);
           }
         }
       }
-      float mx = m;
-#pragma unroll
-      for (int j = 0; j < 4; ++j)
-#pragma unroll
-        for (int e = 0; e < 2; ++e) {
-          s[j][e] *= qs;
-          if (left < kTile && 8 * j + 2 * t + e >= left) s[j][e] = -INFINITY;
-          mx = fmaxf(mx, s[j][e]);
-        }
-      mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
-      mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 2));
-      const float mref = mx == -INFINITY ? 0.0f : mx;
-      uint32_t dv[4][NB], dtop = 0;
+      float s[4][2];
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
-        lds_words<NB>(dv[j], vd + (8 * j + 2 * t) * NB);
-#pragma unroll
-        for (int b = 0; b < NB; ++b) dtop = __vmaxu2(dtop, dv[j][b]);
+        s[j][0] = f2_lo(s2[j]);
+        s[j][1] = f2_hi(s2[j]);
       }
-      dtop = max(dtop >> 16, dtop & 0xffffu);
-      dtop = max(dtop, __shfl_xor_sync(0xffffffffu, dtop, 1));
-      dtop = max(dtop, __shfl_xor_sync(0xffffffffu, dtop, 2));
+      if (left < kTile) {
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+#pragma unroll
+          for (int e = 0; e < 2; ++e)
+            if (8 * j + 2 * t + e >= left) s[j][e] = -INFINITY;
+      }
+      float mx = fmaxf(fmaxf(fmaxf(s[0][0], s[0][1]), fmaxf(s[1][0], s[1][1])),
+                       fmaxf(fmaxf(s[2][0], s[2][1]), fmaxf(s[3][0], s[3][1])));
+      mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
+      mx = fmaxf(m, fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 2)) * qs);
+      const float mref = mx == -INFINITY ? 0.0f : mx;
+      uint32_t dtop = 0;
+#pragma unroll
+      for (int w = 0; w < (NB + 1) / 2; ++w)
+        if (lane + 32 * w < kTile / 2 * NB) dtop = __vmaxu2(dtop, vd[lane + 32 * w]);
+      dtop = __reduce_max_sync(0xffffffffu, max(dtop >> 16, dtop & 0xffffu));
       const int enew = max(ev, (int)(dtop >> 10) - 14);
-      const float corr = exp2f(m - mref);
-      float psum = 0.0f;
-      const float up = pow2f(15 - enew);
-#pragma unroll
-      for (int j = 0; j < 4; ++j)
-#pragma unroll
-        for (int e = 0; e < 2; ++e) {
-          s[j][e] = exp2f(s[j][e] - mref);
-          psum += s[j][e];
-          s[j][e] *= up;
-        }
-      l = fmaf(l, corr, psum);
-      m = mx;
+      const float corr = ex2(m - mref);
       const float down = corr * pow2f(ev - enew);
+      const unsigned long long down2 = f2_pack(down, down);
+      const __half2 unit = __float2half2_rn(pow2f(-enew));
+      m = mx;
       ev = enew;
-      if (__any_sync(0xffffffffu, down != 1.0f)) {
+      // weights 2^15 p, so that the small ones keep their bits
+      __half2 ph[4], pl[4];
+      float psum = 0.0f;
 #pragma unroll
-        for (int b = 0; b < NB; ++b)
-#pragma unroll
-          for (int c = 0; c < 4; ++c)
-#pragma unroll
-            for (int r = 0; r < 4; ++r) o[b][c][r] *= down;
+      for (int j = 0; j < 4; ++j) {
+        const float p0 = ex2(fmaf(s[j][0], qs, 15.0f - mref));
+        const float p1 = ex2(fmaf(s[j][1], qs, 15.0f - mref));
+        psum += p0;
+        psum += p1;
+        split2(p0, p1, ph[j], pl[j]);
       }
+      l = fmaf(l, corr, psum);
 
-      // ---- output: 16 keys at a time
+      // ---- output, a block's 32 channels at a time: keys 16 h + {2t, 2t+1, 2t+8,
+      // 2t+9} of unit g
+      uint32_t vw[4][NB], dv[4][NB];
 #pragma unroll
-      for (int h = 0; h < 2; ++h) {
-        constexpr int W = (NB + 1) / 2;
-        uint32_t vw[4][W];  // keys 16 h + {2t, 2t+1, 2t+8, 2t+9}, unit g of every block
+      for (int j = 0; j < 4; ++j) {
+        lds_words<NB>(vw[j], vq + (4 * j + t) * (32 * NB) + value_part(t, g) * (4 * NB));
+        lds_words<NB>(dv[j], vd + (4 * j + t) * NB);
+      }
 #pragma unroll
-        for (int k = 0; k < 4; ++k) {
-          const unsigned char* p = vq + (16 * h + 2 * t + (k & 1) + (k >> 1) * 8) * (16 * NB) + g * (2 * NB);
-          if constexpr (NB % 2 == 0) {
-            lds_words<W>(vw[k], p);
-          } else {
-            const uint16_t* u = reinterpret_cast<const uint16_t*>(p);
+      for (int b = 0; b < NB; ++b) {
+        uint32_t hi[4], lo[4];
 #pragma unroll
-            for (int w = 0; w < W; ++w)
-              vw[k][w] = u[2 * w] | (2 * w + 1 < NB ? (uint32_t)u[2 * w + 1] << 16 : 0u);
-          }
+        for (int j = 0; j < 4; ++j) {
+          const __half2 d = __hmul2(as_h2(dv[j][b]), unit);
+          const __half2 x = __hmul2(ph[j], d);
+          hi[j] = bits(x);
+          lo[j] = bits(__hfma2(pl[j], d, __hfma2(ph[j], d, __hneg2(x))));
         }
+        float c[4][4];
 #pragma unroll
-        for (int b = 0; b < NB; ++b) {
-          uint4 w4;
-          {
-            const int j0 = 2 * h, j1 = 2 * h + 1;
-            split2(s[j0][0] * half_at(dv[j0][b >> 1], b & 1),
-                   s[j0][1] * half_at(dv[j0][(NB + b) >> 1], (NB + b) & 1), w4.x, w4.y);
-            split2(s[j1][0] * half_at(dv[j1][b >> 1], b & 1),
-                   s[j1][1] * half_at(dv[j1][(NB + b) >> 1], (NB + b) & 1), w4.z, w4.w);
-          }
+        for (int h = 0; h < 2; ++h) {
+          const uint4 w4 = make_uint4(hi[2 * h], lo[2 * h], hi[2 * h + 1], lo[2 * h + 1]);
 #pragma unroll
           for (int byte = 0; byte < 2; ++byte) {
-            const uint32_t i0 = (b & 1) * 2 + byte;
-            const uint32_t sel = i0 | i0 << 4 | (i0 + 4) << 8 | (i0 + 4) << 12;
-            const uint32_t x0 = __byte_perm(vw[0][b >> 1], vw[1][b >> 1], sel);
-            const uint32_t x1 = __byte_perm(vw[2][b >> 1], vw[3][b >> 1], sel);
+            const uint32_t x0 = vw[2 * h][b] >> (8 * byte), x1 = vw[2 * h + 1][b] >> (8 * byte);
             // channels 2g + byte (low nibbles) and 2g + byte + 16 (high)
-            mma16816(o[b][byte], w4, codes_low(x0), codes_low(x1));
-            mma16816(o[b][2 + byte], w4, codes_high(x0), codes_high(x1));
+            if (h == 0) {
+              mma16816_first(c[byte], w4, codes_low(x0), codes_low(x1));
+              mma16816_first(c[2 + byte], w4, codes_high(x0), codes_high(x1));
+            } else {
+              mma16816(c[byte], w4, codes_low(x0), codes_low(x1));
+              mma16816(c[2 + byte], w4, codes_high(x0), codes_high(x1));
+            }
           }
         }
+#pragma unroll
+        for (int n = 0; n < 4; ++n) o[b][n] = ffma2(o[b][n], down2, both_terms(c[n]));
       }
       __syncwarp();
       if (i + kStages < mine) {
@@ -597,10 +645,10 @@ __global__ void __launch_bounds__(kThreads, 3) kv_q40_attention_kernel(const Att
 #pragma unroll
         for (int e = 0; e < 2; ++e) {
           // column 2t + e of the products: channels 2 (2t + e) + byte, + 16
-          float2* lo = reinterpret_cast<float2*>(ro + g * D + 32 * b + 4 * t + 2 * e);
-          lo[0] = make_float2(o[b][0][e] + o[b][0][e + 2], o[b][1][e] + o[b][1][e + 2]);
-          lo[8] = make_float2((o[b][2][e] + o[b][2][e + 2]) * 0.0625f,
-                              (o[b][3][e] + o[b][3][e + 2]) * 0.0625f);
+          float2* to = reinterpret_cast<float2*>(ro + g * D + 32 * b + 4 * t + 2 * e);
+          auto pick = [&](unsigned long long v) { return e ? f2_hi(v) : f2_lo(v); };
+          to[0] = make_float2(pick(o[b][0]), pick(o[b][1]));
+          to[8] = make_float2(pick(o[b][2]) * 0.0625f, pick(o[b][3]) * 0.0625f);
         }
     }
     __syncthreads();
@@ -612,10 +660,10 @@ __global__ void __launch_bounds__(kThreads, 3) kv_q40_attention_kernel(const Att
       for (int w = 0; w < warps_used; ++w) mm = fmaxf(mm, red_m[w][h]);
       const float ref = mm == -INFINITY ? 0.0f : mm;
       for (int w = 0; w < warps_used; ++w) {
-        const float f = exp2f(red_m[w][h] - ref);
+        const float f = ex2(red_m[w][h] - ref);
         ll = fmaf(red_l[w][h], f, ll);
         const float x = reinterpret_cast<const float*>(smem + (size_t)w * kStages * S::kStageBytes)[i];
-        acc = fmaf(x * pow2f(red_e[w] - 15), f, acc);
+        acc = fmaf(x * pow2f(red_e[w]), f, acc);
       }
       if (whole) {
         a.out[col * a.ldo + ((int64_t)kvh * a.group + h0) * D + i] = __fdiv_rn(acc, ll);
@@ -627,6 +675,9 @@ __global__ void __launch_bounds__(kThreads, 3) kv_q40_attention_kernel(const Att
         }
       }
     }
+    if (ch0 == 0 && tid == 0)
+      a.spans[(int64_t)col * a.subs + sub] =
+          make_int2(blockIdx.x, cta_of(u + chunks - 1, total, n_ctas));
     tc::fence_proxy_async_smem();  // the next piece's copies overwrite the sums
     __syncthreads();
     u += take;
@@ -639,71 +690,67 @@ __global__ void __launch_bounds__(kThreads, 3) kv_q40_attention_kernel(const Att
     }
   }
   pdl_trigger();
+  zero_rows();
 }
 
 // Joins the partial sums of a (column, group) whose chunks lie in more than
-// one CTA's run, in CTA order: one CTA for one head, D / 4 lanes for a
-// partial sum.
-constexpr int kJoinThreads = 256;
-template <int NB>
+// one CTA's run.  A warp sums every kSlots-th partial of one head, then the
+// warps' sums are joined in order.  HEADS heads a CTA: 1 where there are few
+// groups and many partials of each, 8 where there are many groups.
+constexpr int kJoinThreads = 512, kJoinWarps = kJoinThreads / 32;
+template <int NB, int HEADS>
 __global__ void __launch_bounds__(kJoinThreads) kv_q40_join_kernel(const AttnQ40Args a) {
   using S = Shape<NB>;
-  constexpr int D = S::kD, kLanes = D / 4, kSlots = kJoinThreads / kLanes;
-  __shared__ int64_t warp_sums[kJoinThreads / 32];
-  __shared__ float4 acc_s[kSlots][kLanes];
-  __shared__ float l_s[kSlots], m_s[kJoinThreads / 32];
-  const int tid = threadIdx.x, col = blockIdx.x / a.subs, sub = blockIdx.x % a.subs, h = blockIdx.y;
+  constexpr int D = S::kD, kSlots = kJoinWarps / HEADS;
+  __shared__ float acc_s[kJoinWarps][D], m_s[kJoinWarps], l_s[kJoinWarps];
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  const int col = blockIdx.x / a.subs, sub = blockIdx.x % a.subs;
   const int kvh = sub % a.c.n_kv_heads, h0 = (sub / a.c.n_kv_heads) * kGroup;
-  int64_t total = 0, first = 0, before;
-  for (int c0 = 0; c0 < a.n_cols; c0 += kJoinThreads) {
-    const int c = c0 + tid;
-    const int64_t x = c < a.n_cols ? units_of(a, visible(a, c)) : 0;
-    total += block_scan(x, &before, warp_sums);
-    if (c0 < col) first += block_scan(c < col ? x : 0, &before, warp_sums);
-  }
-  const int len = visible(a, col), chunks = (len + kChunk - 1) / kChunk;
-  // every CTA waits, so that this grid's end is also the first kernel's
-  pdl_wait();
-  if (chunks == 0 || h0 + h >= a.group) return;
-  const int n_ctas = (int)min((int64_t)a.n_ctas, total);
-  first += (int64_t)sub * chunks;
-  const int i0 = cta_of(first, total, n_ctas), i1 = cta_of(first + chunks - 1, total, n_ctas);
-  if (i0 == i1) return;
-  // the first run ends with this group's start, the others begin inside it
-  auto part = [&](int i) { return a.part + ((int64_t)i * 2 + (i == i0 ? 1 : 0)) * S::kPartFloats; };
-  float mm = -INFINITY;
-  for (int i = i0 + tid; i <= i1; i += kJoinThreads) mm = fmaxf(mm, __ldcg(part(i) + kGroup * D + h));
-  mm = warp_max(mm);
-  if ((tid & 31) == 0) m_s[tid >> 5] = mm;
-  __syncthreads();
-  for (int w = 0; w < kJoinThreads / 32; ++w) mm = fmaxf(mm, m_s[w]);
-  const float ref = mm == -INFINITY ? 0.0f : mm;
-  const int lane = tid % kLanes, row = tid / kLanes;
-  if (row < kSlots) {
-    float4 acc = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-    float l = 0.0f;
+  const int len = visible(a, a.lengths[col], slot_of(a, col));
+  pdl_wait();  // every CTA waits, so that this grid's end is also the first kernel's
+  if (chunks_of(len) == 0) return;
+  const int2 span = __ldcg(a.spans + blockIdx.x);
+  if (span.x == span.y) return;
+  const int h = blockIdx.y * HEADS + warp % HEADS, slot = warp / HEADS;
+  float m = -INFINITY, l = 0.0f, acc[NB];
+#pragma unroll
+  for (int b = 0; b < NB; ++b) acc[b] = 0.0f;
+  if (h0 + h < a.group) {
 #pragma unroll 4
-    for (int i = i0 + row; i <= i1; i += kSlots) {
-      const float* p = part(i);
-      const float f = exp2f(__ldcg(p + kGroup * D + h) - ref);
-      const float4 x = __ldcg(reinterpret_cast<const float4*>(p + h * D) + lane);
-      l = fmaf(__ldcg(p + kGroup * D + kGroup + h), f, l);
-      acc.x = fmaf(x.x, f, acc.x);
-      acc.y = fmaf(x.y, f, acc.y);
-      acc.z = fmaf(x.z, f, acc.z);
-      acc.w = fmaf(x.w, f, acc.w);
+    for (int i = span.x + slot; i <= span.y; i += kSlots) {
+      // the first run ends with this group's start, the others begin inside it
+      const float* p = a.part + ((int64_t)i * 2 + (i == span.x ? 1 : 0)) * S::kPartFloats;
+      const float mi = __ldcg(p + kGroup * D + h), li = __ldcg(p + kGroup * D + kGroup + h);
+      float x[NB];
+#pragma unroll
+      for (int b = 0; b < NB; ++b) x[b] = __ldcg(p + h * D + 32 * b + lane);
+      const float top = fmaxf(m, mi), ref = top == -INFINITY ? 0.0f : top;
+      const float f = ex2(m - ref), fi = ex2(mi - ref);
+      m = top;
+      l = fmaf(li, fi, l * f);
+#pragma unroll
+      for (int b = 0; b < NB; ++b) acc[b] = fmaf(x[b], fi, acc[b] * f);
     }
-    acc_s[row][lane] = acc;
-    if (lane == 0) l_s[row] = l;
+  }
+#pragma unroll
+  for (int b = 0; b < NB; ++b) acc_s[warp][32 * b + lane] = acc[b];
+  if (lane == 0) {
+    m_s[warp] = m;
+    l_s[warp] = l;
   }
   __syncthreads();
-  if (tid < D) {
-    float x = 0.0f, l = 0.0f;
+  for (int i = tid; i < HEADS * D; i += kJoinThreads) {
+    const int hh = i / D, d = i % D, head = h0 + blockIdx.y * HEADS + hh;
+    if (head >= a.group) continue;
+    float mm = -INFINITY, ll = 0.0f, x = 0.0f;
+    for (int s = 0; s < kSlots; ++s) mm = fmaxf(mm, m_s[s * HEADS + hh]);
+    const float ref = mm == -INFINITY ? 0.0f : mm;
     for (int s = 0; s < kSlots; ++s) {
-      x += reinterpret_cast<const float*>(&acc_s[s][0])[tid];
-      l += l_s[s];
+      const float f = ex2(m_s[s * HEADS + hh] - ref);
+      ll = fmaf(l_s[s * HEADS + hh], f, ll);
+      x = fmaf(acc_s[s * HEADS + hh][d], f, x);
     }
-    a.out[col * a.ldo + ((int64_t)kvh * a.group + h0 + h) * D + tid] = __fdiv_rn(x, l);
+    a.out[col * a.ldo + ((int64_t)kvh * a.group + head) * D + d] = __fdiv_rn(x, ll);
   }
 }
 
@@ -716,7 +763,7 @@ static_assert(Shape<1>::kStageBytes * kStages >= kGroup * 32 * 4 &&
               "a warp's ring holds its sums");
 
 template <int NB>
-cudaError_t launch_attention_q40(const AttnQ40Args& args, bool join, cudaStream_t st) {
+cudaError_t launch_attention_q40(const AttnQ40Args& args, int n_ctas, bool join, cudaStream_t st) {
   static DeviceOnce once;
   cudaError_t e = once.run([] {
     return cudaFuncSetAttribute(kv_q40_attention_kernel<NB>,
@@ -724,21 +771,30 @@ cudaError_t launch_attention_q40(const AttnQ40Args& args, bool join, cudaStream_
                                 (int)attention_smem<NB>());
   });
   if (e != cudaSuccess) return e;
-  e = launch(kv_q40_attention_kernel<NB>, dim3(args.n_ctas), dim3(kThreads), attention_smem<NB>(),
-             st, false, args);
+  e = launch(kv_q40_attention_kernel<NB>, dim3(n_ctas), dim3(kThreads), attention_smem<NB>(), st,
+             false, args);
   if (e != cudaSuccess || !join) return e;
-  return launch(kv_q40_join_kernel<NB>, dim3((unsigned)(args.n_cols * args.subs), kGroup),
-                dim3(kJoinThreads), 0, st, use_pdl(), args);
+  const unsigned groups = (unsigned)(args.n_cols * args.subs);
+  if (groups < 64)
+    return launch(kv_q40_join_kernel<NB, 1>, dim3(groups, kGroup), dim3(kJoinThreads), 0, st,
+                  use_pdl(), args);
+  return launch(kv_q40_join_kernel<NB, kGroup>, dim3(groups), dim3(kJoinThreads), 0, st, use_pdl(),
+                args);
 }
 
-// CTAs of the attention kernel: three for each SM, or the most chunks there can be.
+// CTAs of the attention kernel: what the SMs hold at once, or the most chunks
+// there can be.
 int attention_ctas(int n_cols, int subs, int max_seq) {
   const int64_t units = (int64_t)n_cols * subs * ((max_seq + kChunk - 1) / kChunk);
-  const int64_t most = (int64_t)3 * sm_count();
+  const int64_t most = (int64_t)kCtasPerSm * sm_count();
   return (int)(units < most ? units : most);
 }
+// The workspace: partial sums, then the groups' spans.
 size_t part_bytes(int n_cols, int subs, int max_seq, int head_dim) {
   return (size_t)attention_ctas(n_cols, subs, max_seq) * 2 * kGroup * (head_dim + 2) * sizeof(float);
+}
+size_t workspace_need(int n_cols, int subs, int max_seq, int head_dim) {
+  return part_bytes(n_cols, subs, max_seq, head_dim) + (size_t)n_cols * subs * sizeof(int2);
 }
 
 bool shape_ok(int n_layers, int n_slots, int max_seq, int n_kv_heads, int head_dim) {
@@ -756,17 +812,13 @@ int check_cache(const std::string& api, const dqmk_kv_q40* kv, int layer, Plane*
   if ((reinterpret_cast<uintptr_t>(kv->keys_dev) | reinterpret_cast<uintptr_t>(kv->values_dev)) & 15u)
     return fail(DQMK_ERR_INVALID, api + ": KV cache must be 16-byte aligned");
   if (layer < 0 || layer >= kv->n_layers) return fail(DQMK_ERR_RANGE, api + ": layer out of range");
-  const int64_t rows = padded_rows(kv->max_seq);
-  const int64_t per_layer = (int64_t)kv->n_slots * kv->n_kv_heads * rows, all = per_layer * kv->n_layers;
+  const int64_t tiles = tiles_of(kv->max_seq);
   const int nb = kv->head_dim / 32;
-  uint8_t* kb = static_cast<uint8_t*>(kv->keys_dev);
-  uint8_t* vb = static_cast<uint8_t*>(kv->values_dev);
-  out->kq = kb + per_layer * layer * 16 * nb;
-  out->vq = vb + per_layer * layer * 16 * nb;
-  out->kd = reinterpret_cast<uint16_t*>(kb + all * 16 * nb) + per_layer * layer * nb;
-  out->vd = reinterpret_cast<uint16_t*>(vb + all * 16 * nb) + per_layer * layer * nb;
+  const int64_t at = (int64_t)layer * kv->n_slots * kv->n_kv_heads * tiles * tile_bytes(nb);
+  out->k = static_cast<unsigned char*>(kv->keys_dev) + at;
+  out->v = static_cast<unsigned char*>(kv->values_dev) + at;
   out->n_slots = kv->n_slots, out->max_seq = kv->max_seq, out->n_kv_heads = kv->n_kv_heads;
-  out->nb = nb, out->rows = rows;
+  out->nb = nb, out->tiles = tiles;
   return DQMK_OK;
 }
 
@@ -810,7 +862,7 @@ using namespace dqmk;
 extern "C" size_t dqmk_kv_q40_bytes(int n_layers, int n_slots, int max_seq, int n_kv_heads,
                                     int head_dim) {
   if (!shape_ok(n_layers, n_slots, max_seq, n_kv_heads, head_dim)) return 0;
-  return (size_t)n_layers * n_slots * n_kv_heads * padded_rows(max_seq) * (head_dim / 32) * 18;
+  return (size_t)n_layers * n_slots * n_kv_heads * tiles_of(max_seq) * tile_bytes(head_dim / 32);
 }
 
 extern "C" int dqmk_kv_q40_write(const dqmk_kv_q40* kv, int layer, const float* k, int64_t ldk,
@@ -856,7 +908,7 @@ extern "C" size_t dqmk_kv_q40_attention_workspace(const dqmk_kv_q40* kv, int n_c
       n_cols <= 0 || n_heads <= 0 || n_heads % kv->n_kv_heads != 0)
     return 0;
   const int subs = kv->n_kv_heads * ((n_heads / kv->n_kv_heads + kGroup - 1) / kGroup);
-  return part_bytes(n_cols, subs, kv->max_seq, kv->head_dim);
+  return workspace_need(n_cols, subs, kv->max_seq, kv->head_dim);
 }
 
 extern "C" int dqmk_kv_q40_attention(const dqmk_kv_q40* kv, int layer, const float* q, int64_t ldq,
@@ -881,7 +933,7 @@ extern "C" int dqmk_kv_q40_attention(const dqmk_kv_q40* kv, int layer, const flo
   const int64_t subs = (int64_t)kv->n_kv_heads * ((a.group + kGroup - 1) / kGroup);
   if (subs * n_cols > INT_MAX) return fail(DQMK_ERR_UNSUPPORTED, api + ": too many columns");
   a.subs = (int)subs;
-  const size_t need = part_bytes(n_cols, a.subs, kv->max_seq, kv->head_dim);
+  const size_t need = workspace_need(n_cols, a.subs, kv->max_seq, kv->head_dim);
   if (workspace_bytes < need)
     return fail(DQMK_ERR_INVALID, api + ": workspace of " + std::to_string(workspace_bytes) +
                                       " bytes, needs " + std::to_string(need));
@@ -889,15 +941,17 @@ extern "C" int dqmk_kv_q40_attention(const dqmk_kv_q40* kv, int layer, const flo
   a.lengths = lengths, a.slots = slots, a.n_cols = n_cols, a.n_heads = n_heads;
   a.scale = kLog2e / sqrtf((float)kv->head_dim);
   a.part = static_cast<float*>(workspace);
-  a.n_ctas = attention_ctas(n_cols, a.subs, kv->max_seq);
+  a.spans = reinterpret_cast<int2*>(static_cast<char*>(workspace) +
+                                    part_bytes(n_cols, a.subs, kv->max_seq, kv->head_dim));
+  const int n_ctas = attention_ctas(n_cols, a.subs, kv->max_seq);
   const bool join = kv->max_seq > kChunk;  // else every run ends with a whole group
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   cudaError_t e;
   switch (a.c.nb) {
-    case 1: e = launch_attention_q40<1>(a, join, st); break;
-    case 2: e = launch_attention_q40<2>(a, join, st); break;
-    case 3: e = launch_attention_q40<3>(a, join, st); break;
-    default: e = launch_attention_q40<4>(a, join, st); break;
+    case 1: e = launch_attention_q40<1>(a, n_ctas, join, st); break;
+    case 2: e = launch_attention_q40<2>(a, n_ctas, join, st); break;
+    case 3: e = launch_attention_q40<3>(a, n_ctas, join, st); break;
+    default: e = launch_attention_q40<4>(a, n_ctas, join, st); break;
   }
   DQMK_CUDA_RET(api.c_str(), e);
   return DQMK_OK;

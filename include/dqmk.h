@@ -370,7 +370,7 @@ int dqmk_kv_q40_read(const dqmk_kv_q40* kv, int layer, const int* slots_dev,
  * out_dev at element c * ldo.  Query heads h use KV head h / (n_heads /
  * n_kv_heads).  Several columns may name one slot (a prompt's tokens with
  * growing lengths, once their rows are written).  Length 0 gives a row of
- * zeros; so do a length outside 0..max_seq and a slot outside the cache, which
+ * zeros, whatever its slot; so do a length outside 0..max_seq and a slot outside the cache, which
  * are recorded (dqmk_device_error bit 3).  Results are those of f32 arithmetic
  * on the cache's values (within f32 summation order), and the same for the
  * same arguments every time.  workspace_dev: dqmk_kv_q40_attention_workspace

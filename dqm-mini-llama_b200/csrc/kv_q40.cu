@@ -199,16 +199,17 @@ __global__ void __launch_bounds__(256) kv_q40_read_kernel(RowsArgs a) {
 // product does both:
 //   scores   A = q 2^-e, B = codes n - 8 (rows of K), one sum for each block:
 //            S = 2^e / sqrt(D) sum_b d_b sum q (n - 8)
-//   output   A = w = p d_b 2^(15-E), B = codes n - 8 (columns of V):
-//            O[c] = 2^(E-15) sum_j w_j (n_jc - 8), a block's channels at a time
-// E is a running bound of the exponents of V's scales, kept like the running
-// maximum of the scores: when it grows, the sums are scaled down.  The terms of
-// w come from p = ph + pl and d in fp16 arithmetic: hi = ph d, lo = (ph d - hi)
-// + pl d, whose first part a fused multiply-add leaves exact.
+//   output   A = w = p d_b 2^X, B = codes n - 8 (columns of V):
+//            O[c] = 2^-X sum_j w_j (n_jc - 8), a block's channels at a time
+// X keeps w in fp16's range: E is a running bound of the exponents of V's
+// scales, kept like the running maximum of the scores, and p takes 2^15 (less
+// where d is above 1) and d a power of two where it is below 2^-6.  The terms
+// of w come from p = ph + pl and d in fp16 arithmetic: hi = ph d, lo = (ph d -
+// hi) + pl d, whose first part a fused multiply-add leaves exact.
 //
 // A code becomes a half by one AND/OR, (w & 0x000f) | 0x6400 = 1024 + n, and
-// one addition that centres it: n - 8 (16 (n - 8) from a high nibble; its
-// channel of q takes 1/16).  The code's own bits are n 2^-24 as a subnormal
+// one addition that centres it: n - 8 (16 (n - 8) from a high nibble; for a key
+// its channel of q takes 1/16).  The code's own bits are n 2^-24 as a subnormal
 // half and would need neither, but the products align their sums by the
 // operands' exponent fields, and 10 bits of every sum are lost.  For the same
 // reason (the accumulators round towards zero) a tile's products start from
@@ -271,15 +272,10 @@ __device__ __forceinline__ void mma16816(float (&d)[4], const uint4& a, uint32_t
 }
 // The same without an addend.
 __device__ __forceinline__ void mma16816_first(float (&d)[4], const uint4& a, uint32_t b0, uint32_t b1) {
-  asm(
-      "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, "
+  asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, "
       "{%10,%10,%10,%10};"
       : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3])
       : "r"(a.x), "r"(a.y), "r"(a.z), "r"(a.w), "r"(b0), "r"(b1), "f"(0.0f));
-}
-// High and low term rows of a product, added: columns 2t and 2t + 1.
-__device__ __forceinline__ unsigned long long both_terms(const float (&c)[4]) {
-  return fadd2(f2_pack(c[0], c[1]), f2_pack(c[2], c[3]));
 }
 __device__ __forceinline__ void bulk_load(void* dst, const void* src, uint32_t bytes, uint64_t* bar) {
   asm volatile(
@@ -296,13 +292,13 @@ __device__ __forceinline__ void split2(float x0, float x1, __half2& hi, __half2&
   const float2 back = __half22float2(hi);
   lo = __floats2half2_rn(__fsub_rn(x0, back.x), __fsub_rn(x1, back.y));
 }
-// The codes in bits 0-3 and 16-19 of a word as the halves n - 8, and those in
-// bits 4-7 and 20-23 as 16 (n - 8).
 __device__ __forceinline__ uint32_t and_or(uint32_t w, uint32_t mask, uint32_t with) {
   uint32_t r;
   asm("lop3.b32 %0, %1, %2, %3, 0xea;" : "=r"(r) : "r"(w), "r"(mask), "r"(with));
   return r;
 }
+// The codes in bits 0-3 and 16-19 of a word as the halves n - 8, and those in
+// bits 4-7 and 20-23 as 16 (n - 8).
 __device__ __forceinline__ uint32_t codes_low(uint32_t w) {
   return bits(__hadd2(as_h2(and_or(w, 0x000f000fu, 0x64006400u)), as_h2(0xe408e408u)));  // -1032
 }
@@ -310,6 +306,9 @@ __device__ __forceinline__ uint32_t codes_high(uint32_t w) {
   return bits(__hadd2(as_h2(and_or(w, 0x00f000f0u, 0x64006400u)), as_h2(0xe480e480u)));  // -1152
 }
 __device__ __forceinline__ float pow2f(int e) { return __int_as_float((127 + e) << 23); }
+// V's scales that are all below 2^kSmall are raised by this power of two.
+constexpr int kSmall = -6;
+__device__ __forceinline__ int small_scales(int ev) { return max(0, kSmall - ev); }
 // 2^x; results below 2^-126 are 0.
 __device__ __forceinline__ float ex2(float x) {
   float y;
@@ -478,13 +477,14 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) kv_q40_attention_kernel(
     __syncthreads();
 
     // running sums of head g: channels 4t + {0, 2}, {1, 3} of a block's halves
-    unsigned long long o[NB][4];
+    float o[NB][4][2];
 #pragma unroll
     for (int b = 0; b < NB; ++b)
 #pragma unroll
-      for (int s = 0; s < 4; ++s) o[b][s] = 0ull;
+      for (int s = 0; s < 4; ++s) o[b][s][0] = o[b][s][1] = 0.0f;
     float m = -INFINITY, l = 0.0f;
-    int ev = -20;  // V's scales so far are below 2^ev
+    float ref = -INFINITY;  // weights are 2^(score - ref)
+    int ev = -14;           // V's scales so far are below 2^ev
     const float qs = qscale[g];
 
     for (int i = 0; i < mine; ++i) {
@@ -516,14 +516,14 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) kv_q40_attention_kernel(
       }
 
       // ---- scores of keys 8 j + 2 t + {0, 1} for head g
-      unsigned long long s2[4];
+      float s[4][2];
       {
         uint32_t kw[4][NB], dk[4][NB];
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
           lds_words<NB>(kw[j], kq + (8 * j + g) * (16 * NB) + t * (4 * NB));
           lds_words<NB>(dk[j], kd + (4 * j + t) * NB);
-          s2[j] = 0ull;
+          s[j][0] = s[j][1] = 0.0f;
         }
 #pragma unroll
         for (int b = 0; b < NB; ++b) {
@@ -535,15 +535,10 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) kv_q40_attention_kernel(
             mma16816_first(c, a0, codes_low(w), codes_high(w));
             mma16816(c, a1, codes_low(w8), codes_high(w8));
             const float2 d = __half22float2(as_h2(dk[j][b]));
-            s2[j] = ffma2(f2_pack(d.x, d.y), both_terms(c), s2[j]);
+            s[j][0] = fmaf(d.x, c[0] + c[2], s[j][0]);
+            s[j][1] = fmaf(d.y, c[1] + c[3], s[j][1]);
           }
         }
-      }
-      float s[4][2];
-#pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        s[j][0] = f2_lo(s2[j]);
-        s[j][1] = f2_hi(s2[j]);
       }
       if (left < kTile) {
 #pragma unroll
@@ -555,27 +550,23 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) kv_q40_attention_kernel(
       float mx = fmaxf(fmaxf(fmaxf(s[0][0], s[0][1]), fmaxf(s[1][0], s[1][1])),
                        fmaxf(fmaxf(s[2][0], s[2][1]), fmaxf(s[3][0], s[3][1])));
       mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
-      mx = fmaxf(m, fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 2)) * qs);
-      const float mref = mx == -INFINITY ? 0.0f : mx;
+      m = fmaxf(m, fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 2)) * qs);
       uint32_t dtop = 0;
 #pragma unroll
       for (int w = 0; w < (NB + 1) / 2; ++w)
         if (lane + 32 * w < kTile / 2 * NB) dtop = __vmaxu2(dtop, vd[lane + 32 * w]);
       dtop = __reduce_max_sync(0xffffffffu, max(dtop >> 16, dtop & 0xffffu));
-      const int enew = max(ev, (int)(dtop >> 10) - 14);
-      const float corr = ex2(m - mref);
-      const float down = corr * pow2f(ev - enew);
-      const unsigned long long down2 = f2_pack(down, down);
-      const __half2 unit = __float2half2_rn(pow2f(-enew));
-      m = mx;
-      ev = enew;
-      // weights 2^15 p, so that the small ones keep their bits
+      const int eold = ev;
+      ev = max(ev, (int)(dtop >> 10) - 14);
+      const float rnew = (m == -INFINITY ? 0.0f : m) + (float)(max(ev, 0) - 15);
+      const float corr = ex2(ref - rnew);
+      const float down = corr * pow2f(small_scales(ev) - small_scales(eold));
+      ref = rnew;
       __half2 ph[4], pl[4];
       float psum = 0.0f;
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
-        const float p0 = ex2(fmaf(s[j][0], qs, 15.0f - mref));
-        const float p1 = ex2(fmaf(s[j][1], qs, 15.0f - mref));
+        const float p0 = ex2(fmaf(s[j][0], qs, -rnew)), p1 = ex2(fmaf(s[j][1], qs, -rnew));
         psum += p0;
         psum += p1;
         split2(p0, p1, ph[j], pl[j]);
@@ -590,12 +581,19 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) kv_q40_attention_kernel(
         lds_words<NB>(vw[j], vq + (4 * j + t) * (32 * NB) + value_part(t, g) * (4 * NB));
         lds_words<NB>(dv[j], vd + (4 * j + t) * NB);
       }
+      if (ev < kSmall) {
+        const __half2 up = __float2half2_rn(pow2f(small_scales(ev)));
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+#pragma unroll
+          for (int b = 0; b < NB; ++b) dv[j][b] = bits(__hmul2(as_h2(dv[j][b]), up));
+      }
 #pragma unroll
       for (int b = 0; b < NB; ++b) {
         uint32_t hi[4], lo[4];
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
-          const __half2 d = __hmul2(as_h2(dv[j][b]), unit);
+          const __half2 d = as_h2(dv[j][b]);
           const __half2 x = __hmul2(ph[j], d);
           hi[j] = bits(x);
           lo[j] = bits(__hfma2(pl[j], d, __hfma2(ph[j], d, __hneg2(x))));
@@ -618,7 +616,10 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) kv_q40_attention_kernel(
           }
         }
 #pragma unroll
-        for (int n = 0; n < 4; ++n) o[b][n] = ffma2(o[b][n], down2, both_terms(c[n]));
+        for (int n = 0; n < 4; ++n) {
+          o[b][n][0] = fmaf(o[b][n][0], down, c[n][0] + c[n][2]);
+          o[b][n][1] = fmaf(o[b][n][1], down, c[n][1] + c[n][3]);
+        }
       }
       __syncwarp();
       if (i + kStages < mine) {
@@ -633,10 +634,10 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) kv_q40_attention_kernel(
     l += __shfl_xor_sync(0xffffffffu, l, 1);
     l += __shfl_xor_sync(0xffffffffu, l, 2);
     if (t == 0) {
-      red_m[warp][g] = m;
+      red_m[warp][g] = ref;
       red_l[warp][g] = l;
     }
-    if (lane == 0) red_e[warp] = ev;
+    if (lane == 0) red_e[warp] = small_scales(ev);
     const int warps_used = min(kWarps, tile_end - ch0 * kWarps);
     if (mine) {
       float* ro = reinterpret_cast<float*>(ring);  // [head][channel], this warp's ring is empty
@@ -646,9 +647,8 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) kv_q40_attention_kernel(
         for (int e = 0; e < 2; ++e) {
           // column 2t + e of the products: channels 2 (2t + e) + byte, + 16
           float2* to = reinterpret_cast<float2*>(ro + g * D + 32 * b + 4 * t + 2 * e);
-          auto pick = [&](unsigned long long v) { return e ? f2_hi(v) : f2_lo(v); };
-          to[0] = make_float2(pick(o[b][0]), pick(o[b][1]));
-          to[8] = make_float2(pick(o[b][2]) * 0.0625f, pick(o[b][3]) * 0.0625f);
+          to[0] = make_float2(o[b][0][e], o[b][1][e]);
+          to[8] = make_float2(o[b][2][e] * 0.0625f, o[b][3][e] * 0.0625f);
         }
     }
     __syncthreads();
@@ -658,12 +658,11 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) kv_q40_attention_kernel(
       const int h = i / D;
       float mm = -INFINITY, ll = 0.0f, acc = 0.0f;
       for (int w = 0; w < warps_used; ++w) mm = fmaxf(mm, red_m[w][h]);
-      const float ref = mm == -INFINITY ? 0.0f : mm;
       for (int w = 0; w < warps_used; ++w) {
-        const float f = ex2(red_m[w][h] - ref);
+        const float f = ex2(red_m[w][h] - mm);
         ll = fmaf(red_l[w][h], f, ll);
         const float x = reinterpret_cast<const float*>(smem + (size_t)w * kStages * S::kStageBytes)[i];
-        acc = fmaf(x * pow2f(red_e[w]), f, acc);
+        acc = fmaf(x * pow2f(-red_e[w]), f, acc);
       }
       if (whole) {
         a.out[col * a.ldo + ((int64_t)kvh * a.group + h0) * D + i] = __fdiv_rn(acc, ll);

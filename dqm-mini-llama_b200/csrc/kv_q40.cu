@@ -219,13 +219,14 @@ __global__ void __launch_bounds__(256) kv_q40_read_kernel(RowsArgs a) {
 // memory rate an SM has about 1.4 instruction slots a value, and the unpacking,
 // scaling and splitting above take most of them.
 //
-// Work: the positions of all columns and heads form one list of chunks of
-// kChunk positions, cut into equal runs for the CTAs, whatever the lengths; a
-// CTA that holds only part of a (column, group)'s chunks leaves its partial
-// sums in the workspace for a second kernel.  Each warp streams its own tiles
-// of 32 positions through a ring of bulk copies.
+// Work: the positions of all columns and heads form one list of units, kExtra
+// for each (column, group), what its start and end cost, and one for each of
+// its chunks of kChunk positions.  The list is cut into equal runs for the CTAs,
+// whatever the lengths; a CTA that holds only part of a group's chunks leaves
+// its partial sums in the workspace for a second kernel.  Each warp streams its
+// own tiles of 32 positions through a ring of bulk copies.
 constexpr int kWarps = 4, kThreads = 32 * kWarps, kChunk = kTile * kWarps;
-constexpr int kStages = 3, kGroup = 8, kCtasPerSm = 3;
+constexpr int kStages = 2, kGroup = 8, kCtasPerSm = 3, kExtra = 2;
 constexpr float kLog2e = 1.44269504088896341f;
 
 struct AttnQ40Args {
@@ -257,6 +258,7 @@ __device__ __forceinline__ int slot_of(const AttnQ40Args& a, int col) {
   return a.slots ? a.slots[col] : col;
 }
 __device__ __forceinline__ int chunks_of(int len) { return (len + kChunk - 1) / kChunk; }
+__device__ __forceinline__ int64_t units_of(int len) { return len ? chunks_of(len) + kExtra : 0; }
 // The CTA whose run of the `total` units holds unit u: run i is
 // [i total / n, (i + 1) total / n).
 __device__ __forceinline__ int cta_of(int64_t u, int64_t total, int n) {
@@ -330,11 +332,16 @@ __device__ __forceinline__ void lds_words(uint32_t (&r)[N], const void* p) {
   }
 }
 
+// One CTA's share of one (column, group): chunks ch0 .. ch0 + take - 1.
+struct Piece {
+  int col, len, slot, sub, ch0, take;
+};
+
 template <int NB>
 __global__ void __launch_bounds__(kThreads, kCtasPerSm) kv_q40_attention_kernel(const AttnQ40Args a) {
   using S = Shape<NB>;
   constexpr int D = S::kD;
-  extern __shared__ __align__(128) unsigned char smem[];
+  extern __shared__ __align__(128) unsigned char smem[];  // rings, then the warps' sums
   __shared__ __align__(8) uint64_t bars[kWarps][kStages];
   __shared__ uint4 qfrag[NB][2][32];
   __shared__ float qscale[kGroup];
@@ -347,6 +354,7 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) kv_q40_attention_kernel(
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const int g = lane >> 2, t = lane & 3;
 
+  pdl_trigger();  // the join kernel waits for this grid's end
   if (tid < kWarps * kStages) tc::bar_init(&bars[tid / kStages][tid % kStages], 1);
   if (tid == 0) {
     abort_flag = 0;
@@ -359,15 +367,14 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) kv_q40_attention_kernel(
   int my_len = 0, my_slot = 0;
   auto count = [&](int c0) {  // columns c0 + tid: units of those before, sum
     const int col = c0 + tid;
-    int n = 0;
     my_slot = 0, my_len = 0;
     if (col < a.n_cols) {
-      n = a.lengths[col];
+      const int n = a.lengths[col];
       my_slot = slot_of(a, col);
       my_len = visible(a, n, my_slot);
       if (my_len != n && blockIdx.x == 0) atomicOr(&g_kv_error, kErrBadIndex);
     }
-    mine_units = (int64_t)chunks_of(my_len) * a.subs;
+    mine_units = units_of(my_len) * a.subs;
     return block_scan(mine_units, &before, warp_sums);
   };
   for (int c0 = 0; c0 < a.n_cols; c0 += kThreads) total += count(c0);
@@ -379,7 +386,6 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) kv_q40_attention_kernel(
   };
   const int n_ctas = (int)min((int64_t)gridDim.x, total);
   if ((int)blockIdx.x >= n_ctas) {
-    pdl_trigger();
     zero_rows();
     return;
   }
@@ -399,80 +405,114 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) kv_q40_attention_kernel(
     }
   }
   __syncthreads();
-  int col = s_col, len = s_len, slot = s_slot;
-  int64_t first = s_first;  // unit 0 of the column
 
   unsigned char* ring = smem + (size_t)warp * kStages * S::kStageBytes;
+  float* sums = reinterpret_cast<float*>(smem + (size_t)kWarps * kStages * S::kStageBytes);
   uint32_t used = 0;  // tiles this warp has waited for: stage used % kStages
   uint32_t issued = 0;
   bool ok = true;
 
-  for (int64_t u = u0; u < u1 && ok;) {
-    const int chunks = chunks_of(len);
-    const int64_t rel = u - first;
-    if (rel >= (int64_t)chunks * a.subs) {  // past this column (or it is empty)
-      first += (int64_t)chunks * a.subs;
-      ++col;
-      slot = slot_of(a, col);
-      len = visible(a, a.lengths[col], slot);
-      continue;
-    }
-    const int sub = (int)(rel / chunks), ch0 = (int)(rel % chunks);
-    const int take = (int)min((int64_t)(chunks - ch0), u1 - u);
-    const int kvh = sub % a.c.n_kv_heads, h0 = (sub / a.c.n_kv_heads) * kGroup;
-    const int n_here = min(kGroup, a.group - h0);  // heads of this group
-    const int64_t head_tile = first_tile(a.c, slot, kvh);
-    const int tile_end = min((ch0 + take) * kWarps, (len + kTile - 1) / kTile);
-    const int tile0 = ch0 * kWarps + warp;
-    const int mine = tile0 < tile_end ? (tile_end - tile0 + kWarps - 1) / kWarps : 0;
-
-    auto issue = [&](int i) {  // lane 0: this warp's tile i of the piece
-      unsigned char* st = ring + (issued % kStages) * S::kStageBytes;
-      uint64_t* bar = &bars[warp][issued % kStages];
-      const int64_t at = (head_tile + tile0 + i * kWarps) * S::kTileBytes;
-      tc::bar_expect_tx(bar, S::kStageBytes);
-      bulk_load(st, a.c.k + at, S::kTileBytes, bar);
-      bulk_load(st + S::kTileBytes, a.c.v + at, S::kTileBytes, bar);
-    };
-    for (int i = 0; i < min(mine, kStages); ++i) {
-      if (lane == 0) issue(i);
+  // the run's part of a group from its unit r on; the units it takes
+  auto cut = [&](Piece& x, int64_t r, int64_t u) {
+    const int64_t n = min(units_of(x.len) - r, u1 - u);
+    x.ch0 = (int)max(r - kExtra, (int64_t)0);
+    x.take = (int)max(r + n - kExtra, (int64_t)0) - x.ch0;
+    return n;
+  };
+  Piece p;
+  p.col = s_col, p.len = s_len, p.slot = s_slot;
+  int64_t group0 = s_first;  // the group's first unit
+  {
+    const int64_t each = units_of(p.len);
+    p.sub = (int)((u0 - s_first) / each);
+    group0 += p.sub * each;
+  }
+  int64_t u = u0 + cut(p, u0 - group0, u0);  // behind the piece
+  if (p.take == 0) {  // the whole run lies before a group's first chunk
+    zero_rows();
+    return;
+  }
+  auto first_of = [&](const Piece& x) { return x.ch0 * kWarps + warp; };  // this warp's first tile
+  auto tiles_end = [&](const Piece& x) {
+    return min((x.ch0 + x.take) * kWarps, (x.len + kTile - 1) / kTile);
+  };
+  auto tiles_mine = [&](const Piece& x) {
+    const int n = tiles_end(x) - first_of(x);
+    return n > 0 ? (n + kWarps - 1) / kWarps : 0;
+  };
+  auto issue = [&](const Piece& x, int i) {  // lane 0: this warp's tile i of the piece
+    unsigned char* st = ring + (issued % kStages) * S::kStageBytes;
+    uint64_t* bar = &bars[warp][issued % kStages];
+    const int64_t at = (first_tile(a.c, x.slot, x.sub % a.c.n_kv_heads) + first_of(x) + i * kWarps) * S::kTileBytes;
+    tc::bar_expect_tx(bar, S::kStageBytes);
+    bulk_load(st, a.c.k + at, S::kTileBytes, bar);
+    bulk_load(st + S::kTileBytes, a.c.v + at, S::kTileBytes, bar);
+  };
+  auto start = [&](const Piece& x) {  // its first tiles
+    for (int i = 0; i < min(tiles_mine(x), kStages); ++i) {
+      if (lane == 0) issue(x, i);
       ++issued;
     }
+  };
+  float qx[2][NB];  // this warp's two heads of the coming piece's queries
+  auto load_q = [&](const Piece& x) {
+    const int kvh = x.sub % a.c.n_kv_heads, h0 = (x.sub / a.c.n_kv_heads) * kGroup;
+#pragma unroll
+    for (int i = 0; i < 2; ++i)
+#pragma unroll
+      for (int b = 0; b < NB; ++b) {
+        const int hh = warp * 2 + i;
+        const int64_t head = (int64_t)kvh * a.group + h0 + hh;
+        qx[i][b] = h0 + hh < a.group ? a.q[x.col * a.ldq + head * D + 32 * b + lane] : 0.0f;
+      }
+  };
+  start(p);
+  load_q(p);
+
+  while (true) {
+    const int kvh = p.sub % a.c.n_kv_heads, h0 = (p.sub / a.c.n_kv_heads) * kGroup;
+    const int n_here = min(kGroup, a.group - h0);  // heads of this group
+    const int mine = tiles_mine(p), tile0 = first_of(p), len = p.len;
+    // the next piece begins a group: of this column, or of the next with any
+    Piece nx = p;
+    int64_t behind = u;
+    nx.take = 0;
+    if (u < u1) {
+      if (++nx.sub == a.subs) {
+        nx.sub = 0;
+        do {
+          ++nx.col;
+          nx.slot = slot_of(a, nx.col);
+          nx.len = visible(a, a.lengths[nx.col], nx.slot);
+        } while (nx.len == 0);
+      }
+      behind += cut(nx, 0, u);
+    }
+    const bool more = nx.take > 0;
 
     // ---- the group's queries as A operands (high and low terms), two heads a warp
-    {
-      float x[2][NB];
 #pragma unroll
-      for (int i = 0; i < 2; ++i)
+    for (int i = 0; i < 2; ++i) {
+      const int hh = warp * 2 + i;
+      float top = 0.0f;
 #pragma unroll
-        for (int b = 0; b < NB; ++b) {
-          const int hh = warp * 2 + i;
-          const int64_t head = (int64_t)kvh * a.group + h0 + hh;
-          x[i][b] = hh < n_here ? a.q[col * a.ldq + head * D + 32 * b + lane] : 0.0f;
-        }
+      for (int b = 0; b < NB; ++b) top = fmaxf(top, fabsf(qx[i][b]));
+      top = warp_max(top);
+      // 2^-e brings the row's largest value into [2^14, 2^15)
+      const int e = top > 0.0f ? min(max(((__float_as_int(top) >> 23) & 0xff) - 141, -120), 120) : 0;
+      const bool high = lane >= 16;
+      const int jj = lane & 15, tq = jj >> 2, el = jj & 3;
 #pragma unroll
-      for (int i = 0; i < 2; ++i) {
-        const int hh = warp * 2 + i;
-        float top = 0.0f;
-#pragma unroll
-        for (int b = 0; b < NB; ++b) top = fmaxf(top, fabsf(x[i][b]));
-        top = warp_max(top);
-        // 2^-e brings the row's largest value into [2^14, 2^15)
-        const int e = top > 0.0f ? min(max(((__float_as_int(top) >> 23) & 0xff) - 141, -120), 120) : 0;
-        const bool high = lane >= 16;
-        const int jj = lane & 15, tq = jj >> 2, el = jj & 3;
-#pragma unroll
-        for (int b = 0; b < NB; ++b) {
-          // a high nibble stands for 16 (n - 8): its channel takes 1/16
-          const float v = x[i][b] * pow2f(-e) * (high ? 0.0625f : 1.0f);
-          const __half hi = __float2half_rn(v);
-          const __half lo = __float2half_rn(v - __half2float(hi));
-          __half* dst = reinterpret_cast<__half*>(&qfrag[b][el & 1][hh * 4 + tq]) + (high ? 4 : 0) + (el >> 1);
-          dst[0] = hi;
-          dst[2] = lo;
-        }
-        if (lane == 0) qscale[hh] = pow2f(e) * a.scale;
+      for (int b = 0; b < NB; ++b) {
+        // a high nibble stands for 16 (n - 8): its channel takes 1/16
+        const float v = qx[i][b] * pow2f(-e) * (high ? 0.0625f : 1.0f);
+        const __half hi = __float2half_rn(v);
+        const __half lo = __float2half_rn(v - __half2float(hi));
+        __half* dst = reinterpret_cast<__half*>(&qfrag[b][el & 1][hh * 4 + tq]) + (high ? 4 : 0) + (el >> 1);
+        dst[0] = hi;
+        dst[2] = lo;
       }
+      if (lane == 0) qscale[hh] = pow2f(e) * a.scale;
     }
     __syncthreads();
 
@@ -623,12 +663,15 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) kv_q40_attention_kernel(
       }
       __syncwarp();
       if (i + kStages < mine) {
-        if (lane == 0) issue(i + kStages);
+        if (lane == 0) issue(p, i + kStages);
         ++issued;
       }
     }
-    ok = __syncthreads_and(ok);
-    if (!ok) break;
+    // the next piece's copies and loads run while this one's sums are joined
+    if (more && ok) {
+      start(nx);
+      load_q(nx);
+    }
 
     // ---- join the warps' sums, in warp order
     l += __shfl_xor_sync(0xffffffffu, l, 1);
@@ -638,9 +681,9 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) kv_q40_attention_kernel(
       red_l[warp][g] = l;
     }
     if (lane == 0) red_e[warp] = small_scales(ev);
-    const int warps_used = min(kWarps, tile_end - ch0 * kWarps);
+    const int warps_used = min(kWarps, tiles_end(p) - p.ch0 * kWarps);
     if (mine) {
-      float* ro = reinterpret_cast<float*>(ring);  // [head][channel], this warp's ring is empty
+      float* ro = sums + warp * (kGroup * D);  // [head][channel]
 #pragma unroll
       for (int b = 0; b < NB; ++b)
 #pragma unroll
@@ -651,35 +694,44 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) kv_q40_attention_kernel(
           to[8] = make_float2(o[b][2][e] * 0.0625f, o[b][3][e] * 0.0625f);
         }
     }
-    __syncthreads();
-    const bool whole = take == chunks;
-    float* part = a.part + ((int64_t)blockIdx.x * 2 + (ch0 == 0 ? 1 : 0)) * S::kPartFloats;
-    for (int i = tid; i < n_here * D; i += kThreads) {
-      const int h = i / D;
-      float mm = -INFINITY, ll = 0.0f, acc = 0.0f;
+    ok = __syncthreads_and(ok);
+    if (!ok) break;
+    // 16 threads a head, D / 16 channels each
+    const int h = tid / 16, chunks = chunks_of(len);
+    if (h < n_here) {
+      constexpr int C = D / 16;
+      float mm = -INFINITY, ll = 0.0f, acc[C];
       for (int w = 0; w < warps_used; ++w) mm = fmaxf(mm, red_m[w][h]);
+#pragma unroll
+      for (int c = 0; c < C; ++c) acc[c] = 0.0f;
       for (int w = 0; w < warps_used; ++w) {
-        const float f = ex2(red_m[w][h] - mm);
+        const float f = ex2(red_m[w][h] - mm), fo = f * pow2f(-red_e[w]);
         ll = fmaf(red_l[w][h], f, ll);
-        const float x = reinterpret_cast<const float*>(smem + (size_t)w * kStages * S::kStageBytes)[i];
-        acc = fmaf(x * pow2f(-red_e[w]), f, acc);
+        const float* from = sums + w * (kGroup * D) + h * D + tid % 16;
+#pragma unroll
+        for (int c = 0; c < C; ++c) acc[c] = fmaf(from[16 * c], fo, acc[c]);
       }
-      if (whole) {
-        a.out[col * a.ldo + ((int64_t)kvh * a.group + h0) * D + i] = __fdiv_rn(acc, ll);
+      if (p.take == chunks) {
+        float* y = a.out + p.col * a.ldo + ((int64_t)kvh * a.group + h0 + h) * D + tid % 16;
+#pragma unroll
+        for (int c = 0; c < C; ++c) y[16 * c] = __fdiv_rn(acc[c], ll);
       } else {
-        part[i] = acc;
-        if (i % D == 0) {
+        float* part = a.part + ((int64_t)blockIdx.x * 2 + (p.ch0 == 0 ? 1 : 0)) * S::kPartFloats;
+#pragma unroll
+        for (int c = 0; c < C; ++c) part[h * D + tid % 16 + 16 * c] = acc[c];
+        if (tid % 16 == 0) {
           part[kGroup * D + h] = mm;
           part[kGroup * D + kGroup + h] = ll;
         }
       }
     }
-    if (ch0 == 0 && tid == 0)
-      a.spans[(int64_t)col * a.subs + sub] =
-          make_int2(blockIdx.x, cta_of(u + chunks - 1, total, n_ctas));
-    tc::fence_proxy_async_smem();  // the next piece's copies overwrite the sums
-    __syncthreads();
-    u += take;
+    if (p.ch0 == 0 && tid == 0)
+      a.spans[(int64_t)p.col * a.subs + p.sub] =
+          make_int2(blockIdx.x, cta_of(group0 + kExtra + chunks - 1, total, n_ctas));
+    if (!more) break;
+    group0 = u;
+    u = behind;
+    p = nx;
   }
   if (!ok) {  // a wait ran out: leave once this warp's own copies have landed or given up
     for (; used < issued; ++used) {
@@ -688,7 +740,6 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) kv_q40_attention_kernel(
         if (tc::now_ns() - t0 > tc::kWaitNs) break;
     }
   }
-  pdl_trigger();
   zero_rows();
 }
 
@@ -696,10 +747,10 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) kv_q40_attention_kernel(
 // one CTA's run.  A warp sums every kSlots-th partial of one head, then the
 // warps' sums are joined in order.  HEADS heads a CTA: 1 where there are few
 // groups and many partials of each, 8 where there are many groups.
-constexpr int kJoinThreads = 512, kJoinWarps = kJoinThreads / 32;
 template <int NB, int HEADS>
-__global__ void __launch_bounds__(kJoinThreads) kv_q40_join_kernel(const AttnQ40Args a) {
+__global__ void __launch_bounds__(HEADS == 1 ? 1024 : 512) kv_q40_join_kernel(const AttnQ40Args a) {
   using S = Shape<NB>;
+  constexpr int kJoinThreads = HEADS == 1 ? 1024 : 512, kJoinWarps = kJoinThreads / 32;
   constexpr int D = S::kD, kSlots = kJoinWarps / HEADS;
   __shared__ float acc_s[kJoinWarps][D], m_s[kJoinWarps], l_s[kJoinWarps];
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
@@ -755,11 +806,8 @@ __global__ void __launch_bounds__(kJoinThreads) kv_q40_join_kernel(const AttnQ40
 
 template <int NB>
 constexpr size_t attention_smem() {
-  return (size_t)kWarps * kStages * Shape<NB>::kStageBytes;
+  return (size_t)kWarps * (kStages * Shape<NB>::kStageBytes + kGroup * Shape<NB>::kD * sizeof(float));
 }
-static_assert(Shape<1>::kStageBytes * kStages >= kGroup * 32 * 4 &&
-                  Shape<4>::kStageBytes * kStages >= kGroup * 128 * 4,
-              "a warp's ring holds its sums");
 
 template <int NB>
 cudaError_t launch_attention_q40(const AttnQ40Args& args, int n_ctas, bool join, cudaStream_t st) {
@@ -775,10 +823,9 @@ cudaError_t launch_attention_q40(const AttnQ40Args& args, int n_ctas, bool join,
   if (e != cudaSuccess || !join) return e;
   const unsigned groups = (unsigned)(args.n_cols * args.subs);
   if (groups < 64)
-    return launch(kv_q40_join_kernel<NB, 1>, dim3(groups, kGroup), dim3(kJoinThreads), 0, st,
-                  use_pdl(), args);
-  return launch(kv_q40_join_kernel<NB, kGroup>, dim3(groups), dim3(kJoinThreads), 0, st, use_pdl(),
-                args);
+    return launch(kv_q40_join_kernel<NB, 1>, dim3(groups, kGroup), dim3(1024), 0, st, use_pdl(),
+                  args);
+  return launch(kv_q40_join_kernel<NB, kGroup>, dim3(groups), dim3(512), 0, st, use_pdl(), args);
 }
 
 // CTAs of the attention kernel: what the SMs hold at once, or the most chunks

@@ -355,24 +355,25 @@ class _There:
             g.__exit__(*exc)
 
 
-class _Here:
-    """A call on the current device and stream.  The raw handle comes from
-    torch's binding: current_stream() costs more than the launch."""
+class _There:
+    """Another device or a given stream made current for a call, so that its
+    outputs and workspace are allocated for the stream that uses them."""
 
-    def __init__(self, index):
-        self.index = index
+    def __init__(self, device, stream):
+        torch = _torch()
+        if stream is not None and not isinstance(stream, torch.cuda.Stream):
+            stream = torch.cuda.ExternalStream(stream, device=device)
+        if stream is not None and stream.device != device:
+            raise RuntimeError("stream and tensors are on different devices")
+        self.guards = (torch.cuda.device(device), torch.cuda.stream(stream))
 
     def __enter__(self):
-        return _torch()._C._cuda_getCurrentRawStream(self.index)
+        for g in self.guards:
+            g.__enter__()
 
     def __exit__(self, *exc):
-        pass
-
-
-def _on(device, stream):
-    if stream is None and device.index == _torch()._C._cuda_getDevice():
-        return _Here(device.index)
-    return _There(device, stream)
+        for g in reversed(self.guards):
+            g.__exit__(*exc)
 
 
 def _refuse(api: str, name: str, t, shape, dtype, device):
@@ -393,21 +394,29 @@ def _first(api: str, name: str, t, dims: int):
     return t.device
 
 
-def _rows(api: str, name: str, t, shape, device) -> int:
+# These checks run on every call of a decode step: few and cheap look-ups.
+def _rows(api: str, name: str, t, shape, device, f32) -> int:
     """Elements from one row to the next of a float32 [rows, heads, head_dim]
     tensor of this shape and device whose rows are contiguous."""
-    f32 = _torch().float32
-    if isinstance(t, _torch().Tensor) and t.dtype is f32 and t.shape == shape and t.device == device:
-        row, head, value = t.stride()
-        if (value == 1 or shape[2] == 1) and (head == shape[2] or shape[1] < 2):
-            return row if shape[0] > 1 else shape[1] * shape[2]
+    try:
+        if t.dtype is f32 and t.shape == shape and t.device == device:
+            if t.is_contiguous():
+                return shape[1] * shape[2]
+            row, head, value = t.stride()
+            if (value == 1 or shape[2] == 1) and (head == shape[2] or shape[1] < 2):
+                return row
+    except AttributeError:
+        pass
     _refuse(api, name, t, shape, f32, device)
 
 
-def _vector(api: str, name: str, t, n: int, device, dtype):
-    if not (isinstance(t, _torch().Tensor) and t.dtype is dtype and t.shape == (n,) and
-            t.device == device and (n < 2 or t.stride(0) == 1)):
-        _refuse(api, name, t, (n,), dtype, device)
+def _vector(api: str, name: str, t, shape, device, dtype):
+    try:
+        if t.dtype is dtype and t.shape == shape and t.device == device and t.is_contiguous():
+            return
+    except AttributeError:
+        pass
+    _refuse(api, name, t, shape, dtype, device)
 
 
 def qk_norm_rope(q, k, q_norm, k_norm, positions, theta: float, eps: float, neox: bool = True,
@@ -418,29 +427,32 @@ def qk_norm_rope(q, k, q_norm, k_norm, positions, theta: float, eps: float, neox
     q_out / k_out may be q / k (in place); by default new tensors.  Returns
     (q_out, k_out)."""
     torch = _torch()
-    api = "QkNormRope"
+    api, f32 = "QkNormRope", torch.float32
     dev = _first(api, "q", q, 3)
+    if stream is not None or dev.index != torch._C._cuda_getDevice():
+        with _There(dev, stream):
+            return qk_norm_rope(q, k, q_norm, k_norm, positions, theta, eps, neox, q_out, k_out)
     _first(api, "k", k, 3)
-    n, heads, dim = shape = q.shape
-    kv = k.shape[1]
-    ldq = _rows(api, "q", q, shape, dev)
-    ldk = _rows(api, "k", k, (n, kv, dim), dev)
-    _vector(api, "q_norm", q_norm, dim, dev, torch.float32)
-    _vector(api, "k_norm", k_norm, dim, dev, torch.float32)
-    _vector(api, "positions", positions, n, dev, torch.int32)
-    with _on(dev, stream) as s:
-        if q_out is None:
-            q_out, ldqo = q.new_empty(shape), heads * dim
-        else:
-            ldqo = _rows(api, "q_out", q_out, shape, dev)
-        if k_out is None:
-            k_out, ldko = k.new_empty((n, kv, dim)), kv * dim
-        else:
-            ldko = _rows(api, "k_out", k_out, (n, kv, dim), dev)
-        check(lib().dqmk_qk_norm_rope(
-            q.data_ptr(), ldq, k.data_ptr(), ldk, n, heads, kv, dim, q_norm.data_ptr(),
-            k_norm.data_ptr(), eps, positions.data_ptr(), theta, 1 if neox else 0,
-            q_out.data_ptr(), ldqo, k_out.data_ptr(), ldko, s))
+    shape, kshape = q.shape, k.shape
+    n, heads, dim = shape
+    kv = kshape[1]
+    ldq = _rows(api, "q", q, shape, dev, f32)
+    ldk = _rows(api, "k", k, (n, kv, dim), dev, f32)
+    _vector(api, "q_norm", q_norm, (dim,), dev, f32)
+    _vector(api, "k_norm", k_norm, (dim,), dev, f32)
+    _vector(api, "positions", positions, (n,), dev, torch.int32)
+    if q_out is None:
+        q_out, ldqo = torch.empty_like(q), heads * dim
+    else:
+        ldqo = _rows(api, "q_out", q_out, shape, dev, f32)
+    if k_out is None:
+        k_out, ldko = torch.empty_like(k), kv * dim
+    else:
+        ldko = _rows(api, "k_out", k_out, kshape, dev, f32)
+    check(lib().dqmk_qk_norm_rope(
+        q.data_ptr(), ldq, k.data_ptr(), ldk, n, heads, kv, dim, q_norm.data_ptr(),
+        k_norm.data_ptr(), eps, positions.data_ptr(), theta, 1 if neox else 0, q_out.data_ptr(),
+        ldqo, k_out.data_ptr(), ldko, torch._C._cuda_getCurrentRawStream(dev.index)))
     return q_out, k_out
 
 
@@ -450,28 +462,32 @@ def attention_prompt(q, k, v, starts, out=None, stream=None):
     device, sequence s = tokens starts[s] .. starts[s+1]-1.  Rows of `out`
     outside every sequence are left as they were (a new `out` is zero there)."""
     torch = _torch()
-    api = "AttentionPrompt"
+    api, f32 = "AttentionPrompt", torch.float32
     dev = _first(api, "q", q, 3)
+    if stream is not None or dev.index != torch._C._cuda_getDevice():
+        with _There(dev, stream):
+            return attention_prompt(q, k, v, starts, out)
     _first(api, "k", k, 3)
     _first(api, "starts", starts, 1)
     n, heads, dim = shape = q.shape
     kv, seqs = k.shape[1], starts.shape[0] - 1
     if seqs < 0:
         raise RuntimeError(f"{api}: starts must hold at least one offset")
-    ldq = _rows(api, "q", q, shape, dev)
-    ldk = _rows(api, "k", k, (n, kv, dim), dev)
-    ldv = _rows(api, "v", v, (n, kv, dim), dev)
-    _vector(api, "starts", starts, seqs + 1, dev, torch.int32)
-    with _on(dev, stream) as s:
-        if out is None:
-            out = torch.zeros(shape, dtype=torch.float32, device=dev)
-        ldo = _rows(api, "out", out, shape, dev)
-        L = lib()
-        nbytes = L.dqmk_attention_prompt_workspace(n, seqs, heads, kv, dim)
-        work = torch.empty(nbytes, dtype=torch.uint8, device=dev)
-        check(L.dqmk_attention_prompt(
-            q.data_ptr(), ldq, k.data_ptr(), ldk, v.data_ptr(), ldv, starts.data_ptr(), seqs, n,
-            heads, kv, dim, out.data_ptr(), ldo, work.data_ptr(), nbytes, s))
+    ldq = _rows(api, "q", q, shape, dev, f32)
+    ldk = _rows(api, "k", k, (n, kv, dim), dev, f32)
+    ldv = _rows(api, "v", v, (n, kv, dim), dev, f32)
+    _vector(api, "starts", starts, (seqs + 1,), dev, torch.int32)
+    if out is None:
+        out, ldo = torch.zeros_like(q), heads * dim
+    else:
+        ldo = _rows(api, "out", out, shape, dev, f32)
+    L = lib()
+    nbytes = L.dqmk_attention_prompt_workspace(n, seqs, heads, kv, dim)
+    work = torch.empty(nbytes, dtype=torch.uint8, device=dev)
+    check(L.dqmk_attention_prompt(
+        q.data_ptr(), ldq, k.data_ptr(), ldk, v.data_ptr(), ldv, starts.data_ptr(), seqs, n, heads,
+        kv, dim, out.data_ptr(), ldo, work.data_ptr(), nbytes,
+        torch._C._cuda_getCurrentRawStream(dev.index)))
     return out
 
 
@@ -500,42 +516,49 @@ class KvCacheQ40:
     def write(self, layer: int, k, v, positions, slots=None, stream=None) -> None:
         """Rows k, v [tokens, n_kv_heads, head_dim] to positions [tokens] of
         slots [tokens] (None: slot t for token t); position -1 stores nothing."""
-        api, dev, i32 = "KvQ40Write", self.device, _torch().int32
+        torch = _torch()
+        api, dev, i32 = "KvQ40Write", self.device, torch.int32
+        if stream is not None or dev.index != torch._C._cuda_getDevice():
+            with _There(dev, stream):
+                return self.write(layer, k, v, positions, slots)
         _first(api, "k", k, 3)
         n = k.shape[0]
         shape = (n, self.n_kv_heads, self.head_dim)
-        ldk = _rows(api, "k", k, shape, dev)
-        ldv = _rows(api, "v", v, shape, dev)
-        _vector(api, "positions", positions, n, dev, i32)
+        ldk = _rows(api, "k", k, shape, dev, torch.float32)
+        ldv = _rows(api, "v", v, shape, dev, torch.float32)
+        _vector(api, "positions", positions, (n,), dev, i32)
         if slots is not None:
-            _vector(api, "slots", slots, n, dev, i32)
-        with _on(dev, stream) as s:
-            check(lib().dqmk_kv_q40_write(
-                self._ref, layer, k.data_ptr(), ldk, v.data_ptr(), ldv,
-                None if slots is None else slots.data_ptr(), positions.data_ptr(), n, s))
+            _vector(api, "slots", slots, (n,), dev, i32)
+        check(lib().dqmk_kv_q40_write(
+            self._ref, layer, k.data_ptr(), ldk, v.data_ptr(), ldv,
+            None if slots is None else slots.data_ptr(), positions.data_ptr(), n,
+            torch._C._cuda_getCurrentRawStream(dev.index)))
 
     def read(self, layer: int, positions, slots=None, k_out=None, v_out=None, stream=None):
         """The values held at those rows, as (k, v) [tokens, n_kv_heads,
         head_dim]; rows of position -1 are left as they were (zero in new
         tensors)."""
         torch = _torch()
-        api, dev = "KvQ40Read", self.device
+        api, dev, i32, f32 = "KvQ40Read", self.device, torch.int32, torch.float32
+        if stream is not None or dev.index != torch._C._cuda_getDevice():
+            with _There(dev, stream):
+                return self.read(layer, positions, slots, k_out, v_out)
         _first(api, "positions", positions, 1)
         n = positions.shape[0]
         shape = (n, self.n_kv_heads, self.head_dim)
-        _vector(api, "positions", positions, n, dev, torch.int32)
+        _vector(api, "positions", positions, (n,), dev, i32)
         if slots is not None:
-            _vector(api, "slots", slots, n, dev, torch.int32)
-        with _on(dev, stream) as s:
-            if k_out is None:
-                k_out = torch.zeros(shape, dtype=torch.float32, device=dev)
-            if v_out is None:
-                v_out = torch.zeros(shape, dtype=torch.float32, device=dev)
-            ldk = _rows(api, "k_out", k_out, shape, dev)
-            ldv = _rows(api, "v_out", v_out, shape, dev)
-            check(lib().dqmk_kv_q40_read(
-                self._ref, layer, None if slots is None else slots.data_ptr(),
-                positions.data_ptr(), n, k_out.data_ptr(), ldk, v_out.data_ptr(), ldv, s))
+            _vector(api, "slots", slots, (n,), dev, i32)
+        if k_out is None:
+            k_out = torch.zeros(shape, dtype=f32, device=dev)
+        if v_out is None:
+            v_out = torch.zeros(shape, dtype=f32, device=dev)
+        ldk = _rows(api, "k_out", k_out, shape, dev, f32)
+        ldv = _rows(api, "v_out", v_out, shape, dev, f32)
+        check(lib().dqmk_kv_q40_read(
+            self._ref, layer, None if slots is None else slots.data_ptr(), positions.data_ptr(), n,
+            k_out.data_ptr(), ldk, v_out.data_ptr(), ldv,
+            torch._C._cuda_getCurrentRawStream(dev.index)))
         return k_out, v_out
 
     def attention(self, q, layer: int, lengths, slots=None, out=None, stream=None):
@@ -544,25 +567,28 @@ class KvCacheQ40:
         the device.  Length 0 gives zeros.  Returns out [columns, n_heads,
         head_dim]."""
         torch = _torch()
-        api, dev = "KvQ40Attention", self.device
+        api, dev, i32, f32 = "KvQ40Attention", self.device, torch.int32, torch.float32
+        if stream is not None or dev.index != torch._C._cuda_getDevice():
+            with _There(dev, stream):
+                return self.attention(q, layer, lengths, slots, out)
         _first(api, "q", q, 3)
         n, heads, _ = q.shape
         shape = (n, heads, self.head_dim)
-        ldq = _rows(api, "q", q, shape, dev)
-        _vector(api, "lengths", lengths, n, dev, torch.int32)
+        ldq = _rows(api, "q", q, shape, dev, f32)
+        _vector(api, "lengths", lengths, (n,), dev, i32)
         if slots is not None:
-            _vector(api, "slots", slots, n, dev, torch.int32)
-        with _on(dev, stream) as s:
-            if out is None:
-                out, ldo = q.new_empty(shape), heads * self.head_dim
-            else:
-                ldo = _rows(api, "out", out, shape, dev)
-            L = lib()
-            nbytes = L.dqmk_kv_q40_attention_workspace(self._ref, n, heads)
-            work = torch.empty(nbytes, dtype=torch.uint8, device=dev)
-            check(L.dqmk_kv_q40_attention(
-                self._ref, layer, q.data_ptr(), ldq, None if slots is None else slots.data_ptr(),
-                lengths.data_ptr(), n, heads, out.data_ptr(), ldo, work.data_ptr(), nbytes, s))
+            _vector(api, "slots", slots, (n,), dev, i32)
+        if out is None:
+            out, ldo = torch.empty_like(q), heads * self.head_dim
+        else:
+            ldo = _rows(api, "out", out, shape, dev, f32)
+        L = lib()
+        nbytes = L.dqmk_kv_q40_attention_workspace(self._ref, n, heads)
+        work = torch.empty(nbytes, dtype=torch.uint8, device=dev)
+        check(L.dqmk_kv_q40_attention(
+            self._ref, layer, q.data_ptr(), ldq, None if slots is None else slots.data_ptr(),
+            lengths.data_ptr(), n, heads, out.data_ptr(), ldo, work.data_ptr(), nbytes,
+            torch._C._cuda_getCurrentRawStream(dev.index)))
         return out
 
 

@@ -226,7 +226,7 @@ __global__ void __launch_bounds__(256) kv_q40_read_kernel(RowsArgs a) {
 // its partial sums in the workspace for a second kernel.  Each warp streams its
 // own tiles of 32 positions through a ring of bulk copies.
 constexpr int kWarps = 4, kThreads = 32 * kWarps, kChunk = kTile * kWarps;
-constexpr int kStages = 2, kGroup = 8, kCtasPerSm = 3, kExtra = 2;
+constexpr int kStages = 2, kGroup = 8, kCtasPerSm = 3, kExtra = 1;
 constexpr float kLog2e = 1.44269504088896341f;
 
 struct AttnQ40Args {

@@ -20,17 +20,23 @@
 // queries that must not see it; it is marked, and the second kernel takes it
 // in f32 straight from the inputs.
 //
-// Second kernel: a CTA takes 128 rows (token, head of the group) of one
-// sequence and KV head, row f = token * group + head: the heads that share
-// keys fill a tile also where the sequence is short, and a tile of rows spans
-// few tokens, so little of the masked triangle is computed.  Row r is TMEM lane
-// r.  One warp streams the tiles, one issues the products, eight run the
-// softmax, warps w and w + 4 on the same 32 rows and half of the columns each:
+// One more CTA of that kernel lists the second kernel's items, those with the
+// most keys first.
+//
+// Second kernel: an item is 128 rows (token, head of the group) of one sequence
+// and KV head, row f = token * group + head: the heads that share keys fill a
+// tile also where the sequence is short, and a tile of rows spans few tokens,
+// so little of the masked triangle is computed.  Row r is TMEM lane r.  A CTA
+// stays on its SM and takes items from the list.  One warp streams the tiles
+// (past the item's end, on into the next one's), one issues the products, eight
+// run the softmax, warps w and w + 4 on the same 32 rows and half of the columns
+// each:
 //   S(j) = Q K_j^T      A = Q (TMEM), B = K_j
 //   P(j) = exp2(S f - m) 2^14, two terms, over S(j)'s own columns
 //   O'(j) = P(j) V_j    A = P(j) (TMEM), B = V_j; o = o corr + O' 2^e in registers
 // S(j+1) is issued before P(j) is waited for, so the tensor cores work on the
-// next scores while the softmax runs.
+// next scores while the softmax runs, and the next item's queries go to TMEM
+// while the last O' is computed.
 #include <climits>
 
 #include "common.cuh"
@@ -56,7 +62,15 @@ struct PromptArgs {
   float scale;            // log2(e) / sqrt(D)
   unsigned char* images;  // [tile][kv_head] operand images
   float4* meta;           // [tile][kv_head]: 2^ek, 2^ev, marked, -
-  int max_tiles;
+  struct Item* items;     // row tiles, those with the most keys first
+  int* heads;             // [0]: row tiles listed, [1]: items taken
+  int max_tiles, max_items;
+};
+
+// 128 rows of one sequence: its first token, its tokens, the first row, and the
+// key tiles before the sequence.
+struct Item {
+  int first, n, row, key_tiles;
 };
 
 // DP: head_dim rounded up to 64 or 128.
@@ -68,48 +82,26 @@ struct Cfg {
   static constexpr int kStages = 3;
   static constexpr int kBufs = DP == 128 ? 3 : 2;   // score buffers
   static constexpr int kCtas = DP == 128 ? 1 : 2;   // for each SM
-  static constexpr int kSmem = kStages * kImage + 1024;
+  // an output stage of each softmax warp: 32 rows of DP / 8 columns
+  static constexpr int kOut = 32 * (DP / 8) * 4;
+  static constexpr int kSmem = kStages * kImage + 8 * kOut + 1024;
   static constexpr uint32_t kTmem = DP == 128 ? 512 : 256;
   static constexpr uint32_t kColQ = 0, kColO = DP, kColS = 2 * DP;
   static_assert(2 * DP + 64 * kBufs <= kTmem, "tensor memory plan");
-};
-
-// One sequence's place in the packed work: row tiles and key tiles of the
-// sequences before it.
-struct Place {
-  int seq, first, n;
-  int64_t row_tiles, key_tiles;  // before this sequence
 };
 
 __device__ __forceinline__ int seq_len(const PromptArgs& a, int s) {
   const int t0 = a.starts[s], t1 = a.starts[s + 1];
   return t0 >= 0 && t1 >= t0 && t1 <= a.n_tokens ? t1 - t0 : 0;
 }
-__device__ __forceinline__ int64_t row_tiles_of(const PromptArgs& a, int n) {
-  return ((int64_t)n * a.group + kRows - 1) / kRows;
+__device__ __forceinline__ int key_tiles_of(int n) { return (n + kKeys - 1) / kKeys; }
+__device__ __forceinline__ int row_tiles_of(const PromptArgs& a, int n) {
+  return (int)(((int64_t)n * a.group + kRows - 1) / kRows);
 }
-
-// The sequence that holds row tile (by_rows) or key tile `index` of the whole
-// pack; false past the end.  All threads call; `shared` is one Place.
-__device__ __forceinline__ bool find_place(const PromptArgs& a, int64_t index, bool by_rows,
-                                           int64_t* warp_sums, Place* shared) {
-  int64_t rows = 0, keys = 0;
-  if (threadIdx.x == 0) shared->seq = -1;
-  for (int s0 = 0; s0 < a.n_seqs; s0 += blockDim.x) {
-    const int s = s0 + threadIdx.x;
-    const int n = s < a.n_seqs ? seq_len(a, s) : 0;
-    const int64_t mine_r = row_tiles_of(a, n), mine_k = (n + kKeys - 1) / kKeys;
-    int64_t before;
-    const int64_t sum = block_scan(mine_r << 32 | mine_k, &before, warp_sums);
-    const int64_t br = rows + (before >> 32), bk = keys + (before & 0xffffffff);
-    const int64_t b = by_rows ? br : bk, mine = by_rows ? mine_r : mine_k;
-    if (index >= b && index < b + mine) *shared = Place{s, a.starts[s], n, br, bk};
-    rows += sum >> 32;
-    keys += sum & 0xffffffff;
-    if (index < (by_rows ? rows : keys)) break;
-  }
-  __syncthreads();
-  return shared->seq >= 0;
+// Key tiles that rows row .. row + 127 of a sequence of n tokens see.
+__device__ __forceinline__ int item_tiles(const PromptArgs& a, int n, int row) {
+  const int64_t last = min((int64_t)row + kRows, (int64_t)n * a.group) - 1;
+  return (int)(last / a.group) / kKeys + 1;
 }
 
 // Byte offset of 16-byte chunk c (8 fp16) of row r in a 128-byte-swizzled
@@ -136,25 +128,97 @@ __device__ __forceinline__ void split2(float x0, float x1, uint32_t& hi, uint32_
 constexpr int kSplitThreads = 256;
 constexpr int kMostSpread = 16;  // exponents between a tile's largest and smallest row
 
+constexpr int kBins = 1024;      // items are listed by their key tiles, up to this many
+
+// The list of row tiles, by one CTA of kSplitThreads.  Sequences whose key tiles
+// do not fit the workspace (only offsets that overlap have any) are left out.
+__device__ void list_items(const PromptArgs& a) {
+  __shared__ int bins[kBins], lens[kSplitThreads], firsts[kSplitThreads], tiles[kSplitThreads];
+  __shared__ int64_t warp_sums[kSplitThreads / 32];
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  for (int i = tid; i < kBins; i += kSplitThreads) bins[i] = 0;
+  // twice over the sequences: first the bins' sizes, then the places
+  for (int pass = 0; pass < 2; ++pass) {
+    int64_t before_chunk = 0;
+    for (int s0 = 0; s0 < a.n_seqs; s0 += kSplitThreads) {
+      const int s = s0 + tid, n = s < a.n_seqs ? seq_len(a, s) : 0;
+      int64_t before;
+      const int64_t sum = block_scan(key_tiles_of(n), &before, warp_sums);
+      before += before_chunk;
+      const bool fits = before + key_tiles_of(n) <= a.max_tiles;
+      if (pass == 0 && s < a.n_seqs) {
+        const int t0 = a.starts[s], t1 = a.starts[s + 1];
+        if (!fits || t0 < 0 || t1 < t0 || t1 > a.n_tokens) atomicOr(&g_prompt_error, kErrBadIndex);
+      }
+      lens[tid] = fits ? n : 0;
+      firsts[tid] = n ? a.starts[s] : 0;
+      tiles[tid] = fits ? (int)before : 0;
+      __syncthreads();
+      for (int i = warp; i < min(kSplitThreads, a.n_seqs - s0); i += kSplitThreads / 32) {
+        const int len = lens[i], count = row_tiles_of(a, len);
+        for (int r = lane; r < count; r += 32) {
+          const int bin = kBins - min(item_tiles(a, len, r * kRows), kBins);
+          const int at = atomicAdd(&bins[bin], 1);
+          if (pass && at < a.max_items) a.items[at] = Item{firsts[i], len, r * kRows, tiles[i]};
+        }
+      }
+      __syncthreads();
+      before_chunk += sum;
+    }
+    if (pass == 0) {
+      constexpr int kEach = kBins / kSplitThreads;
+      int own[kEach], sum = 0;
+#pragma unroll
+      for (int i = 0; i < kEach; ++i) sum += own[i] = bins[tid * kEach + i];
+      int64_t before;
+      const int64_t total = block_scan(sum, &before, warp_sums);
+#pragma unroll
+      for (int i = 0; i < kEach; ++i) {
+        bins[tid * kEach + i] = (int)before;
+        before += own[i];
+      }
+      if (tid == 0) {
+        a.heads[0] = (int)min(total, (int64_t)a.max_items);
+        a.heads[1] = 0;
+      }
+      __syncthreads();
+    }
+  }
+}
+
 template <int DP>
 __global__ void __launch_bounds__(kSplitThreads) prompt_split_kernel(const PromptArgs a) {
   using C = Cfg<DP>;
   constexpr int kF4 = DP / 4, kPer = kKeys * kF4 / kSplitThreads;  // float4s a row, a thread
   __shared__ int64_t warp_sums[kSplitThreads / 32];
-  __shared__ Place place;
+  __shared__ int place[3];  // the tile's sequence: first token, tokens, key tiles before it
   __shared__ float vt[kKeys][DP + 1];
   __shared__ int top_bits, low_bits;
   const int tid = threadIdx.x, kvh = blockIdx.y, D = a.head_dim;
-  if (blockIdx.x == 0 && kvh == 0)
-    for (int s = tid; s < a.n_seqs; s += kSplitThreads) {
-      const int t0 = a.starts[s], t1 = a.starts[s + 1];
-      if (t0 < 0 || t1 < t0 || t1 > a.n_tokens) atomicOr(&g_prompt_error, kErrBadIndex);
-    }
-  const bool found = find_place(a, blockIdx.x, false, warp_sums, &place);
   pdl_trigger();
-  if (!found) return;
-  const int64_t tile = blockIdx.x;  // < max_tiles: the grid's size
-  const int k0 = (int)(tile - place.key_tiles) * kKeys, live = min(kKeys, place.n - k0);
+  if (blockIdx.x == 0) {  // first, so that it does not end last
+    if (kvh == 0) list_items(a);
+    return;
+  }
+  const int64_t tile = (int64_t)blockIdx.x - 1;  // < max_tiles: the grid's size
+  if (tid == 0) place[1] = 0;
+  int64_t done = 0;
+  for (int s0 = 0; s0 < a.n_seqs && done <= tile; s0 += kSplitThreads) {
+    const int s = s0 + tid, n = s < a.n_seqs ? seq_len(a, s) : 0;
+    int64_t before;
+    const int64_t sum = block_scan(key_tiles_of(n), &before, warp_sums);
+    before += done;
+    if (tile >= before && tile < before + key_tiles_of(n)) {
+      place[0] = a.starts[s];
+      place[1] = n;
+      place[2] = (int)before;
+    }
+    done += sum;
+  }
+  __syncthreads();
+  if (place[1] == 0) return;
+  const int k0 = (int)(tile - place[2]) * kKeys, live = min(kKeys, place[1] - k0);
+  const int first = place[0];
   unsigned char* image = a.images + (tile * a.n_kv_heads + kvh) * C::kImage;
   float scales[2];
   bool marked = false;
@@ -164,7 +228,7 @@ __global__ void __launch_bounds__(kSplitThreads) prompt_split_kernel(const Promp
   float4 x[2][kPer];
 #pragma unroll
   for (int which = 0; which < 2; ++which) {
-    const float* base = (which ? a.v : a.k) + (int64_t)(place.first + k0) * (which ? a.ldv : a.ldk) +
+    const float* base = (which ? a.v : a.k) + (int64_t)(first + k0) * (which ? a.ldv : a.ldk) +
                         (int64_t)kvh * D;
     const int64_t ld = which ? a.ldv : a.ldk;
 #pragma unroll
@@ -258,8 +322,39 @@ __device__ __forceinline__ void bulk_load(void* dst, const void* src, uint32_t b
 __device__ __forceinline__ void pair_sync(int quarter) {
   asm volatile("bar.sync %0, 64;" ::"r"(quarter + 1) : "memory");
 }
-__device__ __forceinline__ void tmem_st_n(uint32_t addr, const uint32_t (&r)[32]) { tc::tmem_st32(addr, r); }
-__device__ __forceinline__ void tmem_st_n(uint32_t addr, const uint32_t (&r)[16]) { tc::tmem_st16(addr, r); }
+
+// The AND of a predicate over those 64 threads.
+__device__ __forceinline__ bool pair_and(int quarter, bool x) {
+  uint32_t r;
+  asm volatile(
+      "{\n\t.reg .pred p, q;\n\t"
+      "setp.ne.u32 p, %2, 0;\n\t"
+      "bar.red.and.pred q, %1, 64, p;\n\t"
+      "selp.u32 %0, 1, 0, q;\n\t}"
+      : "=r"(r)
+      : "r"(quarter + 1), "r"((uint32_t)x)
+      : "memory");
+  return r != 0;
+}
+// 16 rows of 8 columns: lane l has columns 2 (l % 4) + {0, 1} of row l / 4 in
+// r[0], r[1] and of row l / 4 + 8 in r[2], r[3].
+__device__ __forceinline__ void tmem_st_rows16(uint32_t taddr, const uint32_t (&r)[4]) {
+  asm volatile("tcgen05.st.sync.aligned.16x256b.x1.b32 [%0], {%1,%2,%3,%4};" ::"r"(taddr), "r"(r[0]),
+               "r"(r[1]), "r"(r[2]), "r"(r[3])
+               : "memory");
+}
+// 2^x; results below 2^-126 are 0.
+__device__ __forceinline__ float ex2(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+
+// An item as the roles of a CTA see it; kvh < 0: no more.
+struct Work {
+  Item it;
+  int kvh, tiles;
+};
 
 template <int DP>
 __global__ void __launch_bounds__(kThreads, Cfg<DP>::kCtas) attention_prompt_kernel(const PromptArgs a) {
@@ -268,33 +363,14 @@ __global__ void __launch_bounds__(kThreads, Cfg<DP>::kCtas) attention_prompt_ker
   extern __shared__ unsigned char raw[];
   __shared__ __align__(8) uint64_t kfull[ST], kempty[ST], vfull[ST], vempty[ST];
   __shared__ __align__(8) uint64_t s_done[NB], p_ready[NB], o_done, o_free, q_ready, fin;
+  __shared__ __align__(8) uint64_t work_full[2], work_empty[2];
+  __shared__ Work work[2];
   __shared__ uint32_t tmem_slot;
   __shared__ volatile int abort_flag;
-  __shared__ float red[2][2][kRows];
-  __shared__ int64_t warp_sums[kThreads / 32];
-  __shared__ Place place;
+  __shared__ float red[2][2][kRows], row_scale[kRows], red_l[2][kRows];
   unsigned char* smem = reinterpret_cast<unsigned char*>(
       (reinterpret_cast<uintptr_t>(raw) + 1023) & ~(uintptr_t)1023);
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
-  const int kvh = blockIdx.x % a.n_kv_heads;
-  // no such tile of rows; or its sequence has more key tiles than the workspace
-  // holds (offsets that overlap, which are recorded)
-  if (!find_place(a, blockIdx.x / a.n_kv_heads, true, warp_sums, &place) ||
-      place.key_tiles + (place.n + kKeys - 1) / kKeys > a.max_tiles) {
-    pdl_wait();  // so that this grid's end is also the first kernel's
-    return;
-  }
-  const int n = place.n, t0 = place.first;
-  const int64_t tiles_here = row_tiles_of(a, n);
-  // the last tokens see the most keys: their tiles first
-  const int64_t f0 = (tiles_here - 1 - (blockIdx.x / a.n_kv_heads - place.row_tiles)) * kRows;
-  const int64_t rows = (int64_t)n * a.group;
-  const int first_tok = (int)(f0 / a.group);
-  const int last_tok = (int)((min(f0 + kRows, rows) - 1) / a.group);
-  const int nt = last_tok / kKeys + 1;
-  const unsigned char* images = a.images + (place.key_tiles * a.n_kv_heads + kvh) * C::kImage;
-  const float4* meta = a.meta + place.key_tiles * a.n_kv_heads + kvh;
-  const size_t image_step = (size_t)a.n_kv_heads * C::kImage;
 
   if (tid == 0) {
     for (int i = 0; i < ST; ++i) {
@@ -306,6 +382,10 @@ __global__ void __launch_bounds__(kThreads, Cfg<DP>::kCtas) attention_prompt_ker
     for (int i = 0; i < NB; ++i) {
       tc::bar_init(&s_done[i], 1);
       tc::bar_init(&p_ready[i], 32 * kSoftWarps);
+    }
+    for (int i = 0; i < 2; ++i) {
+      tc::bar_init(&work_full[i], 1);
+      tc::bar_init(&work_empty[i], 1 + 32 * kSoftWarps);
     }
     tc::bar_init(&o_done, 1);
     tc::bar_init(&o_free, 32 * kSoftWarps);
@@ -322,25 +402,42 @@ __global__ void __launch_bounds__(kThreads, Cfg<DP>::kCtas) attention_prompt_ker
   auto wait = [&](uint64_t* b, int phase) {
     return tc::bar_wait(b, (uint32_t)(phase & 1), &abort_flag, &g_prompt_error);
   };
+  pdl_wait();  // the first kernel's list, images and sizes
 
+  // Tiles are counted through all items of the CTA (T, from 0): tile T uses
+  // stage T % ST and score buffer T % NB; items are counted by w.
   if (warp == kSoftWarps) {
-    // ---- the tiles, by one thread
+    // ---- the items and their tiles, by one thread
     if (lane == 0) {
-      pdl_wait();
       asm volatile("fence.proxy.async.global;" ::: "memory");
+      const int total = __ldcg(a.heads) * a.n_kv_heads;  // at most INT_MAX: the host's check
       int nk = 0, nv = 0;  // copies issued
-      for (int j = 0; j < nt; ++j) {
-        const int st = j % ST;
-        unsigned char* dst = smem + st * C::kImage;
-        const unsigned char* src = images + j * image_step;
-        if (j >= ST && !wait(&kempty[st], j / ST - 1)) break;
-        tc::bar_expect_tx(&kfull[st], C::kOperand);
-        bulk_load(dst, src, C::kOperand, &kfull[st]);
-        ++nk;
-        if (j >= ST && !wait(&vempty[st], j / ST - 1)) break;
-        tc::bar_expect_tx(&vfull[st], C::kOperand);
-        bulk_load(dst + C::kOperand, src + C::kOperand, C::kOperand, &vfull[st]);
-        ++nv;
+      for (int w = 0; !abort_flag; ++w) {
+        const int id = atomicAdd(a.heads + 1, 1);
+        Work x = {};
+        x.kvh = -1;
+        if (id < total) {
+          x.it = a.items[id / a.n_kv_heads];
+          x.kvh = id % a.n_kv_heads;
+          x.tiles = item_tiles(a, x.it.n, x.it.row);
+        }
+        if (w >= 2 && !wait(&work_empty[w & 1], (w >> 1) - 1)) break;
+        work[w & 1] = x;
+        tc::bar_arrive(&work_full[w & 1]);
+        if (x.kvh < 0) break;
+        const unsigned char* src = a.images + ((int64_t)x.it.key_tiles * a.n_kv_heads + x.kvh) * C::kImage;
+        for (int j = 0; j < x.tiles; ++j, src += (size_t)a.n_kv_heads * C::kImage) {
+          const int st = nk % ST;
+          unsigned char* dst = smem + st * C::kImage;
+          if (nk >= ST && !wait(&kempty[st], nk / ST - 1)) break;
+          tc::bar_expect_tx(&kfull[st], C::kOperand);
+          bulk_load(dst, src, C::kOperand, &kfull[st]);
+          ++nk;
+          if (nv >= ST && !wait(&vempty[st], nv / ST - 1)) break;
+          tc::bar_expect_tx(&vfull[st], C::kOperand);
+          bulk_load(dst + C::kOperand, src + C::kOperand, C::kOperand, &vfull[st]);
+          ++nv;
+        }
       }
       if (abort_flag) {  // copies in flight land before the CTA ends
         const unsigned long long begin = tc::now_ns();
@@ -359,9 +456,9 @@ __global__ void __launch_bounds__(kThreads, Cfg<DP>::kCtas) attention_prompt_ker
     // ---- the products, by one thread
     if (tc::elect_one()) {
       constexpr uint32_t kIdescS = tc::idesc_f16(kRows, kKeys), kIdescO = tc::idesc_f16(kRows, DP);
-      auto scores = [&](int j) {
-        const uint32_t d = tmem + C::kColS + 64u * (j % NB), q = tmem + C::kColQ;
-        const uint32_t base = tc::su32(smem + (j % ST) * C::kImage);
+      auto scores = [&](int T) {
+        const uint32_t d = tmem + C::kColS + 64u * (T % NB), q = tmem + C::kColQ;
+        const uint32_t base = tc::su32(smem + (T % ST) * C::kImage);
 #pragma unroll
         for (int k = 0; k < DP / 16; ++k) {
           // a K = 16 slice: 8 TMEM columns of A, 32 bytes (+2) of the descriptor
@@ -372,189 +469,269 @@ __global__ void __launch_bounds__(kThreads, Cfg<DP>::kCtas) attention_prompt_ker
           tc::mma_f16_ts(d, q + 8u * k, lo, kIdescS, 1u);
           tc::mma_f16_ts(d, q + DP / 2 + 8u * k, hi, kIdescS, 1u);
         }
-        tc::mma_commit(&s_done[j % NB]);
-        tc::mma_commit(&kempty[j % ST]);
+        tc::mma_commit(&s_done[T % NB]);
+        tc::mma_commit(&kempty[T % ST]);
       };
-      bool ok = wait(&q_ready, 0) && wait(&kfull[0], 0);
-      tc::tc_fence_after();
-      if (ok) scores(0);
-      for (int j = 0; ok && j < nt; ++j) {
-        if (j + 1 < nt) {
-          ok = wait(&kfull[(j + 1) % ST], (j + 1) / ST);
-          // S(j+1) goes over P(j+1-NB), which O'(j+1-NB) has to have read: with
-          // three buffers o_free of that product was waited for before O'(j-1)
-          if (ok && NB == 2 && j > 0) ok = wait(&o_done, j - 1);
+      bool ok = true;
+      int T = 0;
+      for (int w = 0; ok; ++w) {
+        ok = wait(&work_full[w & 1], w >> 1);
+        if (!ok) break;
+        const int kvh = work[w & 1].kvh, nt = work[w & 1].tiles;
+        tc::bar_arrive(&work_empty[w & 1]);
+        if (kvh < 0) break;
+        // the item's first scores: their buffer's last P went into a product that
+        // is over, for o_free of the one after it was waited for
+        ok = wait(&q_ready, w) && wait(&kfull[T % ST], T / ST);
+        tc::tc_fence_after();
+        if (ok) scores(T);
+        for (int j = 0; ok && j < nt; ++j, ++T) {
+          if (j + 1 < nt) {
+            ok = wait(&kfull[(T + 1) % ST], (T + 1) / ST);
+            // S(T+1) goes over P(T+1-NB), which O'(T+1-NB) has to have read: with
+            // three buffers o_free of that product was waited for before O'(T-1)
+            if (ok && NB == 2 && T > 0) ok = wait(&o_done, T - 1);
+            if (!ok) break;
+            tc::tc_fence_after();
+            scores(T + 1);
+          }
+          ok = wait(&vfull[T % ST], T / ST) && wait(&p_ready[T % NB], T / NB) &&
+               (T == 0 || wait(&o_free, T - 1));
           if (!ok) break;
           tc::tc_fence_after();
-          scores(j + 1);
-        }
-        ok = wait(&vfull[j % ST], j / ST) && wait(&p_ready[j % NB], j / NB) &&
-             (j == 0 || wait(&o_free, j - 1));
-        if (!ok) break;
-        tc::tc_fence_after();
-        const uint32_t p = tmem + C::kColS + 64u * (j % NB), d = tmem + C::kColO;
-        const uint32_t base = tc::su32(smem + (j % ST) * C::kImage + C::kOperand);
-        const uint64_t hi = tc::smem_desc(base), lo = tc::smem_desc(base + C::kPlane);
+          const uint32_t p = tmem + C::kColS + 64u * (T % NB), d = tmem + C::kColO;
+          const uint32_t base = tc::su32(smem + (T % ST) * C::kImage + C::kOperand);
+          const uint64_t hi = tc::smem_desc(base), lo = tc::smem_desc(base + C::kPlane);
 #pragma unroll
-        for (int k = 0; k < kKeys / 16; ++k) {
-          tc::mma_f16_ts(d, p + 8u * k, hi + 2u * k, kIdescO, k > 0 ? 1u : 0u);
-          tc::mma_f16_ts(d, p + 8u * k, lo + 2u * k, kIdescO, 1u);
-          tc::mma_f16_ts(d, p + 32 + 8u * k, hi + 2u * k, kIdescO, 1u);
+          for (int k = 0; k < kKeys / 16; ++k) {
+            tc::mma_f16_ts(d, p + 8u * k, hi + 2u * k, kIdescO, k > 0 ? 1u : 0u);
+            tc::mma_f16_ts(d, p + 8u * k, lo + 2u * k, kIdescO, 1u);
+            tc::mma_f16_ts(d, p + 32 + 8u * k, hi + 2u * k, kIdescO, 1u);
+          }
+          tc::mma_commit(&o_done);
+          tc::mma_commit(&vempty[T % ST]);
         }
-        tc::mma_commit(&o_done);
-        tc::mma_commit(&vempty[j % ST]);
       }
       tc::mma_commit(&fin);
     }
     __syncwarp();
   } else {
-    // ---- the softmax.  After a wait that ran out the warps go on to the end
-    // without waiting (their pairs meet at barriers) and store nothing.
+    // ---- the softmax.  After a wait that ran out the warps go on to the item's
+    // end without waiting (their pairs meet at barriers) and store nothing.
     const int quarter = warp & 3, half = warp >> 2;
     const int row = 32 * quarter + lane;
     const uint32_t lanes = (uint32_t)(32 * quarter) << 16;
-    const int64_t f = f0 + row;
-    const bool valid = f < rows;
-    const int tok = valid ? (int)(f / a.group) : -1;
-    const int head = kvh * a.group + (int)(f % a.group);
-    const float* qrow = a.q + (int64_t)(t0 + max(tok, 0)) * a.ldq + (int64_t)head * a.head_dim;
 
-    float fq;  // scores in base 2: S' fq 2^ek
-    {
-      float4 x[W / 4];
-      float top = 0.0f;
+    struct Rows {  // this thread's row of an item
+      int first_tok, tok, first, kvh, tiles, key_tiles, head;
+      float fq;  // scores in base 2: S' fq 2^ek
+    };
+    // Item w's row, and its queries scaled, split and stored to TMEM, once the
+    // last scores of item w - 1 are over; false: no more items.  For the loads to
+    // be coalesced a warp takes 16 whole rows of its quarter here, 4 lanes a row.
+    auto take_item = [&](int w, Rows& x) {
+      const bool got = wait(&work_full[w & 1], w >> 1);
+      const Work k = work[w & 1];
+      tc::bar_arrive(&work_empty[w & 1]);
+      if (!pair_and(quarter, got && k.kvh >= 0)) return false;
+      const int rows = k.it.n * a.group - k.it.row;  // rows of the item, if under 128
+      const int f = k.it.row + row;
+      x.first_tok = k.it.row / a.group;
+      x.tok = row < rows ? f / a.group : -1;
+      x.head = k.kvh * a.group + f % a.group;
+      x.first = k.it.first, x.kvh = k.kvh, x.tiles = k.tiles, x.key_tiles = k.it.key_tiles;
+
+      const int part = lane & 3;
+      const float* from[2];
 #pragma unroll
-      for (int i = 0; i < W / 4; ++i) {
-        const int d = half * W + 4 * i;
-        x[i] = valid && d < a.head_dim ? *reinterpret_cast<const float4*>(qrow + d)
-                                       : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-        top = fmaxf(top, fmaxf(fmaxf(fabsf(x[i].x), fabsf(x[i].y)), fmaxf(fabsf(x[i].z), fabsf(x[i].w))));
+      for (int i = 0; i < 2; ++i) {
+        const int r = 32 * quarter + 16 * half + (lane >> 2) + 8 * i, fr = k.it.row + r;
+        from[i] = r < rows ? a.q + (int64_t)(k.it.first + fr / a.group) * a.ldq +
+                                 (int64_t)(k.kvh * a.group + fr % a.group) * a.head_dim + 4 * part
+                           : nullptr;
       }
-      red[0][half][row] = top;
-      pair_sync(quarter);
-      top = fmaxf(red[0][0][row], red[0][1][row]);
-      const int e = pow2_ex(top);
-      const float down = pow2f(-e);
-      fq = pow2f(e) * a.scale;
-      uint32_t hi[W / 2], lo[W / 2];
+      const uint32_t at = tmem + ((uint32_t)(32 * quarter + 16 * half) << 16) + C::kColQ;
+      float top[2];
+      // queries of ordinary size keep all their bits under one scale, 2^7; others
+      // are read a second time, for a scale of their row
+      float up[2] = {128.0f, 128.0f};
+      auto pass = [&] {
+        top[0] = top[1] = 0.0f;
+#pragma unroll 4
+        for (int c = 0; c < DP / 16; ++c) {
+          uint32_t hi[4], lo[4];
 #pragma unroll
-      for (int i = 0; i < W / 4; ++i) {
-        split2(x[i].x * down, x[i].y * down, hi[2 * i], lo[2 * i]);
-        split2(x[i].z * down, x[i].w * down, hi[2 * i + 1], lo[2 * i + 1]);
+          for (int i = 0; i < 2; ++i) {
+            const float4 v = from[i] && 16 * c + 4 * part < a.head_dim
+                                 ? *reinterpret_cast<const float4*>(from[i] + 16 * c)
+                                 : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+            top[i] = fmaxf(top[i], fmaxf(fmaxf(fabsf(v.x), fabsf(v.y)), fmaxf(fabsf(v.z), fabsf(v.w))));
+            split2(v.x * up[i], v.y * up[i], hi[2 * i], lo[2 * i]);
+            split2(v.z * up[i], v.w * up[i], hi[2 * i + 1], lo[2 * i + 1]);
+          }
+          tmem_st_rows16(at + 8 * c, hi);
+          tmem_st_rows16(at + DP / 2 + 8 * c, lo);
+        }
+      };
+      pass();
+      bool fits = true;
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        top[i] = fmaxf(top[i], __shfl_xor_sync(0xffffffffu, top[i], 1));
+        top[i] = fmaxf(top[i], __shfl_xor_sync(0xffffffffu, top[i], 2));
+        if (top[i] > 0.0f && !(top[i] >= 0x1p-10f && top[i] < 256.0f)) {
+          up[i] = pow2f(-pow2_ex(top[i]));
+          fits = false;
+        }
       }
-      tmem_st_n(tmem + lanes + C::kColQ + half * (W / 2), hi);
-      tmem_st_n(tmem + lanes + C::kColQ + DP / 2 + half * (W / 2), lo);
+      if (!__all_sync(0xffffffffu, fits)) pass();
+      if (part == 0) {
+        row_scale[32 * quarter + 16 * half + (lane >> 2)] = a.scale / up[0];
+        row_scale[32 * quarter + 16 * half + (lane >> 2) + 8] = a.scale / up[1];
+      }
       tc::tmem_wait_st();
       tc::tc_fence_before();
       tc::bar_arrive(&q_ready);
-      pair_sync(quarter);  // red is written again below
-    }
-
-    pdl_wait();  // meta
-    float o[W];
-#pragma unroll
-    for (int d = 0; d < W; ++d) o[d] = 0.0f;
-    float m = -INFINITY, l = 0.0f, corr = 1.0f, vscale = 0.0f;
-    // O'(j): o = o corr(j) + O'(j) 2^ev(j)
-    auto take_output = [&](int j) {
-      wait(&o_done, j);
-      tc::tc_fence_after();
-#pragma unroll
-      for (int c = 0; c < W; c += 32) {
-        uint32_t r[32];
-        tc::tmem_ld32(tmem + lanes + C::kColO + half * W + c, r);
-        tc::tmem_wait_ld();
-#pragma unroll
-        for (int d = 0; d < 32; ++d)
-          o[c + d] = fmaf(__uint_as_float(r[d]), vscale, o[c + d] * corr);
-      }
-      tc::tc_fence_before();
-      tc::bar_arrive(&o_free);
-    };
-    float4 next = __ldcg(meta);
-    for (int j = 0; j < nt; ++j) {
-      const float4 mt = next;
-      if (j + 1 < nt) next = __ldcg(meta + (int64_t)(j + 1) * a.n_kv_heads);
-      const int kt = j * kKeys;
-      const uint32_t buf = tmem + lanes + C::kColS + 64u * (j % NB);
-      wait(&s_done[j % NB], j / NB);
-      tc::tc_fence_after();
-      uint32_t r[32];
-      tc::tmem_ld32(buf + 32 * half, r);
-      tc::tmem_wait_ld();
-      const bool slow = mt.z != 0.0f;  // the whole CTA's
-      float tmax = -INFINITY;
-      if (kt + kKeys - 1 <= first_tok) {  // every key is visible to every row
-#pragma unroll
-        for (int i = 0; i < 32; ++i) tmax = fmaxf(tmax, __uint_as_float(r[i]));
-      } else {
-#pragma unroll
-        for (int i = 0; i < 32; ++i) {
-          if (kt + 32 * half + i > tok) r[i] = 0xff800000u;  // -inf
-          tmax = fmaxf(tmax, __uint_as_float(r[i]));
-        }
-      }
-      red[j & 1][half][row] = tmax;
       pair_sync(quarter);
-      tmax = fmaxf(red[j & 1][0][row], red[j & 1][1][row]);
-      const float fs = fq * mt.x;
-      const float mnew = slow ? m : fmaxf(m, tmax * fs);
-      const float ref = mnew == -INFINITY ? 0.0f : mnew;
-      const float c = exp2f(m - ref);
-      m = mnew;
-      uint32_t ph[16], pl[16];
-      float sum = 0.0f;
+      x.fq = row_scale[row];
+      return true;
+    };
+
+    Rows cur, nxt;
+    bool have = take_item(0, cur);
+    int T = 0;
+    for (int w = 0; have; ++w) {
+      const int nt = cur.tiles;
+      const float4* meta = a.meta + (int64_t)cur.key_tiles * a.n_kv_heads + cur.kvh;
+      float o[W];
 #pragma unroll
-      for (int i = 0; i < 16; ++i) {
-        float p0 = exp2f(fmaf(__uint_as_float(r[2 * i]), fs, 14.0f - ref));
-        float p1 = exp2f(fmaf(__uint_as_float(r[2 * i + 1]), fs, 14.0f - ref));
-        if (slow) p0 = p1 = 0.0f;
-        sum += p0;
-        sum += p1;
-        split2(p0, p1, ph[i], pl[i]);
-      }
-      if (!slow) l = fmaf(l, c, sum);
-      tc::tmem_st16(buf + 16 * half, ph);
-      tc::tmem_st16(buf + 32 + 16 * half, pl);
-      tc::tmem_wait_st();
-      tc::tc_fence_before();
-      tc::bar_arrive(&p_ready[j % NB]);
-      if (j > 0) take_output(j - 1);
-      corr = slow ? 1.0f : c;
-      vscale = mt.y;
-      if (slow && valid) {
-        // the marked tile in f32, key by key, from the inputs; o is at m's scale
-        for (int key = kt; key <= min(tok, kt + kKeys - 1); ++key) {
-          const float* kr = a.k + (int64_t)(t0 + key) * a.ldk + (int64_t)kvh * a.head_dim;
-          const float* vr = a.v + (int64_t)(t0 + key) * a.ldv + (int64_t)kvh * a.head_dim;
-          float s = 0.0f;
-          for (int d = 0; d < a.head_dim; ++d) s = fmaf(qrow[d], kr[d], s);
-          s *= a.scale;
-          const float top = fmaxf(m, s), at = top == -INFINITY ? 0.0f : top;
-          const float down = exp2f(m - at), p = exp2f(s - at + 14.0f);
-          l *= down;
-          if (half == 0) l += p;
-          m = top;
+      for (int d = 0; d < W; ++d) o[d] = 0.0f;
+      float m = -INFINITY, l = 0.0f, corr = 1.0f, vscale = 0.0f;
+      // O'(T): o = o corr(T) + O'(T) 2^ev(T)
+      auto take_output = [&](int at) {
+        wait(&o_done, at);
+        tc::tc_fence_after();
 #pragma unroll
-          for (int d = 0; d < W; ++d) {
-            const int dd = half * W + d;
-            o[d] = fmaf(p, dd < a.head_dim ? vr[dd] : 0.0f, o[d] * down);
+        for (int c = 0; c < W; c += 32) {
+          uint32_t r[32];
+          tc::tmem_ld32(tmem + lanes + C::kColO + half * W + c, r);
+          tc::tmem_wait_ld();
+#pragma unroll
+          for (int d = 0; d < 32; ++d)
+            o[c + d] = fmaf(__uint_as_float(r[d]), vscale, o[c + d] * corr);
+        }
+        tc::tc_fence_before();
+        tc::bar_arrive(&o_free);
+      };
+      float4 next = __ldcg(meta);
+      for (int j = 0; j < nt; ++j, ++T) {
+        const float4 mt = next;
+        if (j + 1 < nt) next = __ldcg(meta + (int64_t)(j + 1) * a.n_kv_heads);
+        const int kt = j * kKeys;
+        const uint32_t buf = tmem + lanes + C::kColS + 64u * (T % NB);
+        wait(&s_done[T % NB], T / NB);
+        tc::tc_fence_after();
+        uint32_t r[32];
+        tc::tmem_ld32(buf + 32 * half, r);
+        tc::tmem_wait_ld();
+        const bool slow = mt.z != 0.0f;  // the whole CTA's
+        float tmax = -INFINITY;
+        if (kt + kKeys - 1 <= cur.first_tok) {  // every key is visible to every row
+#pragma unroll
+          for (int i = 0; i < 32; ++i) tmax = fmaxf(tmax, __uint_as_float(r[i]));
+        } else {
+#pragma unroll
+          for (int i = 0; i < 32; ++i) {
+            if (kt + 32 * half + i > cur.tok) r[i] = 0xff800000u;  // -inf
+            tmax = fmaxf(tmax, __uint_as_float(r[i]));
+          }
+        }
+        red[T & 1][half][row] = tmax;
+        pair_sync(quarter);
+        tmax = fmaxf(red[T & 1][0][row], red[T & 1][1][row]);
+        const float fs = cur.fq * mt.x;
+        const float mnew = slow ? m : fmaxf(m, tmax * fs);
+        const float ref = mnew == -INFINITY ? 0.0f : mnew;
+        const float c = ex2(m - ref);
+        m = mnew;
+        uint32_t ph[16], pl[16];
+        float sum = 0.0f;
+#pragma unroll
+        for (int i = 0; i < 16; ++i) {
+          float p0 = ex2(fmaf(__uint_as_float(r[2 * i]), fs, 14.0f - ref));
+          float p1 = ex2(fmaf(__uint_as_float(r[2 * i + 1]), fs, 14.0f - ref));
+          if (slow) p0 = p1 = 0.0f;
+          sum += p0;
+          sum += p1;
+          split2(p0, p1, ph[i], pl[i]);
+        }
+        if (!slow) l = fmaf(l, c, sum);
+        tc::tmem_st16(buf + 16 * half, ph);
+        tc::tmem_st16(buf + 32 + 16 * half, pl);
+        tc::tmem_wait_st();
+        tc::tc_fence_before();
+        tc::bar_arrive(&p_ready[T % NB]);
+        if (j > 0) take_output(T - 1);
+        corr = slow ? 1.0f : c;
+        vscale = mt.y;
+        if (slow && cur.tok >= 0) {
+          // the marked tile in f32, key by key, from the inputs; o is at m's scale
+          const float* qr = a.q + (int64_t)(cur.first + cur.tok) * a.ldq + (int64_t)cur.head * a.head_dim;
+          for (int key = kt; key <= min(cur.tok, kt + kKeys - 1); ++key) {
+            const float* kr = a.k + (int64_t)(cur.first + key) * a.ldk + (int64_t)cur.kvh * a.head_dim;
+            const float* vr = a.v + (int64_t)(cur.first + key) * a.ldv + (int64_t)cur.kvh * a.head_dim;
+            float s = 0.0f;
+            for (int d = 0; d < a.head_dim; ++d) s = fmaf(qr[d], kr[d], s);
+            s *= a.scale;
+            const float top = fmaxf(m, s), at = top == -INFINITY ? 0.0f : top;
+            const float down = ex2(m - at), p = ex2(s - at + 14.0f);
+            l *= down;
+            if (half == 0) l += p;
+            m = top;
+#pragma unroll
+            for (int d = 0; d < W; ++d) {
+              const int dd = half * W + d;
+              o[d] = fmaf(p, dd < a.head_dim ? vr[dd] : 0.0f, o[d] * down);
+            }
           }
         }
       }
-    }
-    take_output(nt - 1);
-    red[0][half][row] = l;
-    pair_sync(quarter);
-    l = red[0][0][row] + red[0][1][row];
-    if (valid && !abort_flag) {
-      float* y = a.out + (int64_t)(t0 + tok) * a.ldo + (int64_t)head * a.head_dim + half * W;
+      have = take_item(w + 1, nxt);
+      take_output(T - 1);
+      red_l[half][row] = l;
+      pair_sync(quarter);
+      l = red_l[0][row] + red_l[1][row];
+      // out through the warp's stage, so that the stores cover whole segments of
+      // rows: 4 N columns at a time, N lanes a row
+      constexpr int N = DP / 32, kPass = 32 / N;  // rows of a store
+      const float inv = __frcp_rn(l);
+      float4* stage = reinterpret_cast<float4*>(smem + ST * C::kImage + warp * C::kOut);
+      int64_t at[N];
 #pragma unroll
-      for (int i = 0; i < W / 4; ++i)
-        if (half * W + 4 * i < a.head_dim)
-          *reinterpret_cast<float4*>(y + 4 * i) =
-              make_float4(__fdiv_rn(o[4 * i], l), __fdiv_rn(o[4 * i + 1], l),
-                          __fdiv_rn(o[4 * i + 2], l), __fdiv_rn(o[4 * i + 3], l));
+      for (int i = 0; i < N; ++i) {
+        const int src = i * kPass + lane / N;
+        const int tok = __shfl_sync(0xffffffffu, cur.tok, src), head = __shfl_sync(0xffffffffu, cur.head, src);
+        at[i] = tok >= 0 ? (int64_t)(cur.first + tok) * a.ldo + (int64_t)head * a.head_dim : -1;
+      }
+      const int swz = N == 4 ? (lane >> 1) & 3 : (lane >> 2) & 1;  // of row `lane`: no bank twice
+#pragma unroll
+      for (int c = 0; c < W; c += 4 * N) {
+        __syncwarp();
+#pragma unroll
+        for (int j = 0; j < N; ++j)
+          stage[lane * N + (j ^ swz)] = make_float4(o[c + 4 * j] * inv, o[c + 4 * j + 1] * inv,
+                                                    o[c + 4 * j + 2] * inv, o[c + 4 * j + 3] * inv);
+        __syncwarp();
+        const int col = half * W + c + 4 * (lane % N);
+#pragma unroll
+        for (int i = 0; i < N; ++i) {
+          const int r = i * kPass + lane / N, sr = N == 4 ? (r >> 1) & 3 : (r >> 2) & 1;
+          const float4 v = stage[r * N + ((lane % N) ^ sr)];
+          if (at[i] >= 0 && col < a.head_dim && !abort_flag)
+            *reinterpret_cast<float4*>(a.out + at[i] + col) = v;
+        }
+      }
+      cur = nxt;
     }
   }
   tc::tc_fence_before();
@@ -580,25 +757,33 @@ int64_t most_tiles(int n_tokens, int n_seqs) {
 }
 
 template <int DP>
-cudaError_t launch_prompt(const PromptArgs& a, int64_t row_tiles, cudaStream_t st) {
+cudaError_t launch_prompt(const PromptArgs& a, cudaStream_t st) {
   static DeviceOnce once;
   cudaError_t e = once.run([] {
     return cudaFuncSetAttribute(attention_prompt_kernel<DP>,
                                 cudaFuncAttributeMaxDynamicSharedMemorySize, Cfg<DP>::kSmem);
   });
   if (e != cudaSuccess) return e;
-  e = launch(prompt_split_kernel<DP>, dim3(a.max_tiles, a.n_kv_heads), dim3(kSplitThreads), 0, st,
+  e = launch(prompt_split_kernel<DP>, dim3(a.max_tiles + 1, a.n_kv_heads), dim3(kSplitThreads), 0, st,
              false, a);
   if (e != cudaSuccess) return e;
-  return launch(attention_prompt_kernel<DP>, dim3((unsigned)(row_tiles * a.n_kv_heads)),
+  const int64_t items = (int64_t)a.max_items * a.n_kv_heads, most = (int64_t)Cfg<DP>::kCtas * sm_count();
+  return launch(attention_prompt_kernel<DP>, dim3((unsigned)(items < most ? items : most)),
                 dim3(kThreads), Cfg<DP>::kSmem, st, use_pdl(), a);
 }
 
 bool prompt_shape_ok(int n_heads, int n_kv_heads, int head_dim) {
   return n_heads > 0 && n_kv_heads > 0 && n_heads % n_kv_heads == 0 && head_dim > 0;
 }
+// Row tiles: a sequence's last one may be short, at most one more for each.
+int64_t most_items(int n_tokens, int n_seqs, int group) {
+  return (int64_t)n_tokens * group / kRows + (n_seqs < n_tokens ? n_seqs : n_tokens);
+}
+// The workspace: list heads, list, tile sizes, images.
+size_t up256(size_t b) { return (b + 255) / 256 * 256; }
+size_t items_bytes(int64_t items) { return 256 + up256((size_t)items * sizeof(Item)); }
 size_t meta_bytes(int64_t tiles, int n_kv_heads) {
-  return ((size_t)tiles * n_kv_heads * sizeof(float4) + 255) / 256 * 256;
+  return up256((size_t)tiles * n_kv_heads * sizeof(float4));
 }
 
 }  // namespace
@@ -624,7 +809,8 @@ extern "C" size_t dqmk_attention_prompt_workspace(int n_tokens, int n_seqs, int 
     return 0;
   const int64_t tiles = most_tiles(n_tokens, n_seqs);
   const size_t image = head_dim > 64 ? Cfg<128>::kImage : Cfg<64>::kImage;
-  return meta_bytes(tiles, n_kv_heads) + (size_t)tiles * n_kv_heads * image;
+  return items_bytes(most_items(n_tokens, n_seqs, n_heads / n_kv_heads)) +
+         meta_bytes(tiles, n_kv_heads) + (size_t)tiles * n_kv_heads * image;
 }
 
 extern "C" int dqmk_attention_prompt(const float* q, int64_t ldq, const float* k, int64_t ldk,
@@ -659,14 +845,18 @@ extern "C" int dqmk_attention_prompt(const float* q, int64_t ldq, const float* k
   a.head_dim = head_dim, a.out = out, a.ldo = ldo;
   a.scale = kLog2e / sqrtf((float)head_dim);
   a.max_tiles = (int)most_tiles(n_tokens, n_seqs);
-  a.meta = static_cast<float4*>(workspace);
-  a.images = static_cast<unsigned char*>(workspace) + meta_bytes(a.max_tiles, n_kv_heads);
-  // a sequence's last tile of rows may be short: at most one more for each
-  const int64_t row_tiles = (int64_t)n_tokens * a.group / kRows + n_seqs;
-  if (row_tiles * n_kv_heads > INT_MAX || n_kv_heads > 65535)
+  const int64_t items = most_items(n_tokens, n_seqs, a.group);
+  if (items * n_kv_heads > INT_MAX / 2 || n_kv_heads > 65535 || (int64_t)n_tokens * a.group > INT_MAX - kRows)
     return fail(DQMK_ERR_UNSUPPORTED, api + ": too many rows");
+  a.max_items = (int)items;
+  unsigned char* work = static_cast<unsigned char*>(workspace);
+  a.heads = reinterpret_cast<int*>(work);
+  a.items = reinterpret_cast<Item*>(work + 256);
+  work += items_bytes(items);
+  a.meta = reinterpret_cast<float4*>(work);
+  a.images = work + meta_bytes(a.max_tiles, n_kv_heads);
   cudaStream_t st = static_cast<cudaStream_t>(stream);
-  DQMK_CUDA_RET(api.c_str(), head_dim > 64 ? launch_prompt<128>(a, row_tiles, st)
-                                           : launch_prompt<64>(a, row_tiles, st));
+  DQMK_CUDA_RET(api.c_str(), head_dim > 64 ? launch_prompt<128>(a, st)
+                                           : launch_prompt<64>(a, st));
   return DQMK_OK;
 }

@@ -36,7 +36,10 @@
 //   O'(j) = P(j) V_j    A = P(j) (TMEM), B = V_j; o = o corr + O' 2^e in registers
 // S(j+1) is issued before P(j) is waited for, so the tensor cores work on the
 // next scores while the softmax runs, and the next item's queries go to TMEM
-// while the last O' is computed.
+// while the last O' is computed.  A row a thread would touch 32 lines with each
+// load and store and took 5 us of an item's 9 (measured), as much as 4 key tiles:
+// queries are read 4 lanes a row, outputs go through a shared-memory stage and
+// leave as one copy a row, under the next item's first tiles.
 #include <climits>
 
 #include "common.cuh"
@@ -79,12 +82,12 @@ struct Cfg {
   static constexpr int kPlane = kKeys * DP * 2;     // one term of K or V
   static constexpr int kOperand = 2 * kPlane;       // both terms
   static constexpr int kImage = 2 * kOperand;       // K, then V
-  static constexpr int kStages = 3;
+  static constexpr int kStages = 2;
   static constexpr int kBufs = DP == 128 ? 3 : 2;   // score buffers
   static constexpr int kCtas = DP == 128 ? 1 : 2;   // for each SM
-  // an output stage of each softmax warp: 32 rows of DP / 8 columns
-  static constexpr int kOut = 32 * (DP / 8) * 4;
-  static constexpr int kSmem = kStages * kImage + 8 * kOut + 1024;
+  // the stage: a row's outputs, rows 16 bytes apart modulo the 128 of all banks
+  static constexpr int kRowBytes = DP * 4 + 16;
+  static constexpr int kSmem = kStages * kImage + kRows * kRowBytes + 1024;
   static constexpr uint32_t kTmem = DP == 128 ? 512 : 256;
   static constexpr uint32_t kColQ = 0, kColO = DP, kColS = 2 * DP;
   static_assert(2 * DP + 64 * kBufs <= kTmem, "tensor memory plan");
@@ -318,6 +321,12 @@ __device__ __forceinline__ void bulk_load(void* dst, const void* src, uint32_t b
       "l"(src), "r"(bytes), "r"(tc::su32(bar))
       : "memory");
 }
+__device__ __forceinline__ void bulk_store(void* dst, const void* src, uint32_t bytes) {
+  asm volatile("cp.async.bulk.global.shared::cta.bulk_group [%0], [%1], %2;" ::"l"(dst),
+               "r"(tc::su32(src)), "r"(bytes)
+               : "memory");
+  asm volatile("cp.async.bulk.commit_group;" ::: "memory");
+}
 // The 64 threads of warps w and w + 4.
 __device__ __forceinline__ void pair_sync(int quarter) {
   asm volatile("bar.sync %0, 64;" ::"r"(quarter + 1) : "memory");
@@ -340,8 +349,7 @@ __device__ __forceinline__ bool pair_and(int quarter, bool x) {
 // r[0], r[1] and of row l / 4 + 8 in r[2], r[3].
 __device__ __forceinline__ void tmem_st_rows16(uint32_t taddr, const uint32_t (&r)[4]) {
   asm volatile("tcgen05.st.sync.aligned.16x256b.x1.b32 [%0], {%1,%2,%3,%4};" ::"r"(taddr), "r"(r[0]),
-               "r"(r[1]), "r"(r[2]), "r"(r[3])
-               : "memory");
+               "r"(r[1]), "r"(r[2]), "r"(r[3]));
 }
 // 2^x; results below 2^-126 are 0.
 __device__ __forceinline__ float ex2(float x) {
@@ -370,6 +378,7 @@ __global__ void __launch_bounds__(kThreads, Cfg<DP>::kCtas) attention_prompt_ker
   __shared__ float red[2][2][kRows], row_scale[kRows], red_l[2][kRows];
   unsigned char* smem = reinterpret_cast<unsigned char*>(
       (reinterpret_cast<uintptr_t>(raw) + 1023) & ~(uintptr_t)1023);
+  unsigned char* stage = smem + ST * C::kImage;
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
 
   if (tid == 0) {
@@ -407,24 +416,40 @@ __global__ void __launch_bounds__(kThreads, Cfg<DP>::kCtas) attention_prompt_ker
   // Tiles are counted through all items of the CTA (T, from 0): tile T uses
   // stage T % ST and score buffer T % NB; items are counted by w.
   if (warp == kSoftWarps) {
-    // ---- the items and their tiles, by one thread
-    if (lane == 0) {
-      asm volatile("fence.proxy.async.global;" ::: "memory");
-      const int total = __ldcg(a.heads) * a.n_kv_heads;  // at most INT_MAX: the host's check
-      int nk = 0, nv = 0;  // copies issued
-      for (int w = 0; !abort_flag; ++w) {
-        const int id = atomicAdd(a.heads + 1, 1);
-        Work x = {};
-        x.kvh = -1;
-        if (id < total) {
-          x.it = a.items[id / a.n_kv_heads];
-          x.kvh = id % a.n_kv_heads;
-          x.tiles = item_tiles(a, x.it.n, x.it.row);
-        }
-        if (w >= 2 && !wait(&work_empty[w & 1], (w >> 1) - 1)) break;
+    // ---- the items and their tiles
+    asm volatile("fence.proxy.async.global;" ::: "memory");
+    const int total = __ldcg(a.heads) * a.n_kv_heads;  // at most INT_MAX: the host's check
+    int nk = 0, nv = 0;  // copies issued, by lane 0
+    // The next item, posted for the other roles once the item before last's
+    // place is free; its queries start towards L2.
+    auto post = [&](int w, Work& x) {
+      int id = 0;
+      if (lane == 0) id = atomicAdd(a.heads + 1, 1);
+      id = __shfl_sync(0xffffffffu, id, 0);
+      x.kvh = -1;
+      if (id < total) {
+        x.it = a.items[id / a.n_kv_heads];
+        x.kvh = id % a.n_kv_heads;
+        x.tiles = item_tiles(a, x.it.n, x.it.row);
+        const int first = x.it.row / a.group, behind = min(x.it.n, (x.it.row + kRows - 1) / a.group + 1);
+        const uint32_t bytes = (uint32_t)min(a.group * a.head_dim, 1 << 16) * 4;
+        for (int t = first + lane; t < behind; t += 32)
+          asm volatile("cp.async.bulk.prefetch.L2.global [%0], %1;" ::"l"(
+                           a.q + (int64_t)(x.it.first + t) * a.ldq + (int64_t)x.kvh * a.group * a.head_dim),
+                       "r"(bytes));
+      }
+      const bool ok = __all_sync(0xffffffffu, w < 2 || wait(&work_empty[w & 1], (w >> 1) - 1));
+      if (ok && lane == 0) {
         work[w & 1] = x;
         tc::bar_arrive(&work_full[w & 1]);
-        if (x.kvh < 0) break;
+      }
+      return ok;
+    };
+    Work x = {}, ahead = {};
+    bool ok = post(0, x);
+    for (int w = 0; ok && x.kvh >= 0; ++w, x = ahead) {
+      ok = post(w + 1, ahead);
+      if (lane == 0 && ok) {
         const unsigned char* src = a.images + ((int64_t)x.it.key_tiles * a.n_kv_heads + x.kvh) * C::kImage;
         for (int j = 0; j < x.tiles; ++j, src += (size_t)a.n_kv_heads * C::kImage) {
           const int st = nk % ST;
@@ -439,17 +464,16 @@ __global__ void __launch_bounds__(kThreads, Cfg<DP>::kCtas) attention_prompt_ker
           ++nv;
         }
       }
-      if (abort_flag) {  // copies in flight land before the CTA ends
-        const unsigned long long begin = tc::now_ns();
-        for (int j = max(0, nk - ST); j < nk; ++j)
-          while (!tc::bar_try(&kfull[j % ST], (uint32_t)(j / ST) & 1) &&
-                 tc::now_ns() - begin < tc::kWaitNs) {
-          }
-        for (int j = max(0, nv - ST); j < nv; ++j)
-          while (!tc::bar_try(&vfull[j % ST], (uint32_t)(j / ST) & 1) &&
-                 tc::now_ns() - begin < tc::kWaitNs) {
-          }
-      }
+      ok = !__any_sync(0xffffffffu, abort_flag);
+    }
+    if (lane == 0 && abort_flag) {  // copies in flight land before the CTA ends
+      const unsigned long long begin = tc::now_ns();
+      auto landed = [&](uint64_t* b, int n) {
+        while (!tc::bar_try(b, (uint32_t)n & 1) && tc::now_ns() - begin < tc::kWaitNs) {
+        }
+      };
+      for (int j = max(0, nk - ST); j < nk; ++j) landed(&kfull[j % ST], j / ST);
+      for (int j = max(0, nv - ST); j < nv; ++j) landed(&vfull[j % ST], j / ST);
     }
     __syncwarp();
   } else if (warp == kSoftWarps + 1) {
@@ -527,8 +551,8 @@ __global__ void __launch_bounds__(kThreads, Cfg<DP>::kCtas) attention_prompt_ker
       float fq;  // scores in base 2: S' fq 2^ek
     };
     // Item w's row, and its queries scaled, split and stored to TMEM, once the
-    // last scores of item w - 1 are over; false: no more items.  For the loads to
-    // be coalesced a warp takes 16 whole rows of its quarter here, 4 lanes a row.
+    // last scores of item w - 1 are over; false: no more items.  A warp takes 16
+    // whole rows of its quarter here, 4 lanes a row.
     auto take_item = [&](int w, Rows& x) {
       const bool got = wait(&work_full[w & 1], w >> 1);
       const Work k = work[w & 1];
@@ -541,36 +565,45 @@ __global__ void __launch_bounds__(kThreads, Cfg<DP>::kCtas) attention_prompt_ker
       x.head = k.kvh * a.group + f % a.group;
       x.first = k.it.first, x.kvh = k.kvh, x.tiles = k.tiles, x.key_tiles = k.it.key_tiles;
 
-      const int part = lane & 3;
+      const int part = lane & 3, r0 = 32 * quarter + 16 * half + (lane >> 2);
+      const uint32_t at = tmem + ((uint32_t)(32 * quarter + 16 * half) << 16) + C::kColQ;
       const float* from[2];
 #pragma unroll
       for (int i = 0; i < 2; ++i) {
-        const int r = 32 * quarter + 16 * half + (lane >> 2) + 8 * i, fr = k.it.row + r;
-        from[i] = r < rows ? a.q + (int64_t)(k.it.first + fr / a.group) * a.ldq +
-                                 (int64_t)(k.kvh * a.group + fr % a.group) * a.head_dim + 4 * part
-                           : nullptr;
+        const int fr = k.it.row + r0 + 8 * i;
+        from[i] = r0 + 8 * i < rows ? a.q + (int64_t)(k.it.first + fr / a.group) * a.ldq +
+                                          (int64_t)(k.kvh * a.group + fr % a.group) * a.head_dim + 4 * part
+                                    : nullptr;
       }
-      const uint32_t at = tmem + ((uint32_t)(32 * quarter + 16 * half) << 16) + C::kColQ;
       float top[2];
       // queries of ordinary size keep all their bits under one scale, 2^7; others
       // are read a second time, for a scale of their row
       float up[2] = {128.0f, 128.0f};
       auto pass = [&] {
         top[0] = top[1] = 0.0f;
-#pragma unroll 4
-        for (int c = 0; c < DP / 16; ++c) {
-          uint32_t hi[4], lo[4];
 #pragma unroll
-          for (int i = 0; i < 2; ++i) {
-            const float4 v = from[i] && 16 * c + 4 * part < a.head_dim
-                                 ? *reinterpret_cast<const float4*>(from[i] + 16 * c)
-                                 : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-            top[i] = fmaxf(top[i], fmaxf(fmaxf(fabsf(v.x), fabsf(v.y)), fmaxf(fabsf(v.z), fabsf(v.w))));
-            split2(v.x * up[i], v.y * up[i], hi[2 * i], lo[2 * i]);
-            split2(v.z * up[i], v.w * up[i], hi[2 * i + 1], lo[2 * i + 1]);
+        for (int c0 = 0; c0 < DP / 16; c0 += 4) {
+          float4 v[4][2];  // 8 loads at a time
+#pragma unroll
+          for (int c = 0; c < 4; ++c)
+#pragma unroll
+            for (int i = 0; i < 2; ++i)
+              v[c][i] = from[i] && 16 * (c0 + c) + 4 * part < a.head_dim
+                            ? __ldg(reinterpret_cast<const float4*>(from[i] + 16 * (c0 + c)))
+                            : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+#pragma unroll
+          for (int c = 0; c < 4; ++c) {
+            uint32_t hi[4], lo[4];
+#pragma unroll
+            for (int i = 0; i < 2; ++i) {
+              const float4 x4 = v[c][i];
+              top[i] = fmaxf(top[i], fmaxf(fmaxf(fabsf(x4.x), fabsf(x4.y)), fmaxf(fabsf(x4.z), fabsf(x4.w))));
+              split2(x4.x * up[i], x4.y * up[i], hi[2 * i], lo[2 * i]);
+              split2(x4.z * up[i], x4.w * up[i], hi[2 * i + 1], lo[2 * i + 1]);
+            }
+            tmem_st_rows16(at + 8 * (c0 + c), hi);
+            tmem_st_rows16(at + DP / 2 + 8 * (c0 + c), lo);
           }
-          tmem_st_rows16(at + 8 * c, hi);
-          tmem_st_rows16(at + DP / 2 + 8 * c, lo);
         }
       };
       pass();
@@ -586,8 +619,8 @@ __global__ void __launch_bounds__(kThreads, Cfg<DP>::kCtas) attention_prompt_ker
       }
       if (!__all_sync(0xffffffffu, fits)) pass();
       if (part == 0) {
-        row_scale[32 * quarter + 16 * half + (lane >> 2)] = a.scale / up[0];
-        row_scale[32 * quarter + 16 * half + (lane >> 2) + 8] = a.scale / up[1];
+        row_scale[r0] = a.scale / up[0];
+        row_scale[r0 + 8] = a.scale / up[1];
       }
       tc::tmem_wait_st();
       tc::tc_fence_before();
@@ -699,40 +732,26 @@ __global__ void __launch_bounds__(kThreads, Cfg<DP>::kCtas) attention_prompt_ker
       have = take_item(w + 1, nxt);
       take_output(T - 1);
       red_l[half][row] = l;
+      // the last item's outputs have left the stage
+      asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory");
       pair_sync(quarter);
       l = red_l[0][row] + red_l[1][row];
-      // out through the warp's stage, so that the stores cover whole segments of
-      // rows: 4 N columns at a time, N lanes a row
-      constexpr int N = DP / 32, kPass = 32 / N;  // rows of a store
       const float inv = __frcp_rn(l);
-      float4* stage = reinterpret_cast<float4*>(smem + ST * C::kImage + warp * C::kOut);
-      int64_t at[N];
+      float4* to = reinterpret_cast<float4*>(stage + row * C::kRowBytes) + half * (W / 4);
 #pragma unroll
-      for (int i = 0; i < N; ++i) {
-        const int src = i * kPass + lane / N;
-        const int tok = __shfl_sync(0xffffffffu, cur.tok, src), head = __shfl_sync(0xffffffffu, cur.head, src);
-        at[i] = tok >= 0 ? (int64_t)(cur.first + tok) * a.ldo + (int64_t)head * a.head_dim : -1;
-      }
-      const int swz = N == 4 ? (lane >> 1) & 3 : (lane >> 2) & 1;  // of row `lane`: no bank twice
-#pragma unroll
-      for (int c = 0; c < W; c += 4 * N) {
-        __syncwarp();
-#pragma unroll
-        for (int j = 0; j < N; ++j)
-          stage[lane * N + (j ^ swz)] = make_float4(o[c + 4 * j] * inv, o[c + 4 * j + 1] * inv,
-                                                    o[c + 4 * j + 2] * inv, o[c + 4 * j + 3] * inv);
-        __syncwarp();
-        const int col = half * W + c + 4 * (lane % N);
-#pragma unroll
-        for (int i = 0; i < N; ++i) {
-          const int r = i * kPass + lane / N, sr = N == 4 ? (r >> 1) & 3 : (r >> 2) & 1;
-          const float4 v = stage[r * N + ((lane % N) ^ sr)];
-          if (at[i] >= 0 && col < a.head_dim && !abort_flag)
-            *reinterpret_cast<float4*>(a.out + at[i] + col) = v;
-        }
-      }
+      for (int i = 0; i < W / 4; ++i)
+        to[i] = make_float4(o[4 * i] * inv, o[4 * i + 1] * inv, o[4 * i + 2] * inv, o[4 * i + 3] * inv);
+      tc::fence_proxy_async_smem();
+      pair_sync(quarter);
+      // a copy takes 60 cycles to issue: 16 rows a warp
+      const int tok = __shfl_sync(0xffffffffu, cur.tok, 16 * half + (lane & 15));
+      const int head = __shfl_sync(0xffffffffu, cur.head, 16 * half + (lane & 15));
+      if (lane < 16 && tok >= 0 && !abort_flag)
+        bulk_store(a.out + (int64_t)(cur.first + tok) * a.ldo + (int64_t)head * a.head_dim,
+                   stage + (32 * quarter + 16 * half + lane) * C::kRowBytes, (uint32_t)a.head_dim * 4);
       cur = nxt;
     }
+    asm volatile("cp.async.bulk.wait_group 0;" ::: "memory");
   }
   tc::tc_fence_before();
   __syncthreads();

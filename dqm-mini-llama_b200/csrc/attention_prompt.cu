@@ -85,6 +85,8 @@ struct Cfg {
   static constexpr int kStages = 2;
   static constexpr int kBufs = DP == 128 ? 3 : 2;   // score buffers
   static constexpr int kCtas = DP == 128 ? 1 : 2;   // for each SM
+  static constexpr int kParts = 2;  // softmax warps on the same rows
+  static constexpr int kSoftWarps = 4 * kParts, kThreads = 32 * (kSoftWarps + 2);
   // the stage: a row's outputs, rows 16 bytes apart modulo the 128 of all banks
   static constexpr int kRowBytes = DP * 4 + 16;
   static constexpr int kSmem = kStages * kImage + kRows * kRowBytes + 1024;
@@ -312,8 +314,6 @@ __global__ void __launch_bounds__(kSplitThreads) prompt_split_kernel(const Promp
 }
 
 // ------------------------------------------------------------ second kernel
-constexpr int kSoftWarps = 8, kThreads = 32 * (kSoftWarps + 2);
-
 __device__ __forceinline__ void bulk_load(void* dst, const void* src, uint32_t bytes, uint64_t* bar) {
   asm volatile(
       "cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(
@@ -327,24 +327,27 @@ __device__ __forceinline__ void bulk_store(void* dst, const void* src, uint32_t 
                : "memory");
   asm volatile("cp.async.bulk.commit_group;" ::: "memory");
 }
-// The 64 threads of warps w and w + 4.
-__device__ __forceinline__ void pair_sync(int quarter) {
-  asm volatile("bar.sync %0, 64;" ::"r"(quarter + 1) : "memory");
+// The warps w, w + 4, .. that share 32 rows: a barrier, and the AND of a predicate.
+template <int N>
+__device__ __forceinline__ void rows_sync(int quarter) {
+  asm volatile("bar.sync %0, %1;" ::"r"(quarter + 1), "n"(N) : "memory");
 }
-
-// The AND of a predicate over those 64 threads.
-__device__ __forceinline__ bool pair_and(int quarter, bool x) {
+template <int N>
+__device__ __forceinline__ bool rows_and(int quarter, bool x) {
   uint32_t r;
   asm volatile(
       "{\n\t.reg .pred p, q;\n\t"
       "setp.ne.u32 p, %2, 0;\n\t"
-      "bar.red.and.pred q, %1, 64, p;\n\t"
+      "bar.red.and.pred q, %1, %3, p;\n\t"
       "selp.u32 %0, 1, 0, q;\n\t}"
       : "=r"(r)
-      : "r"(quarter + 1), "r"((uint32_t)x)
+      : "r"(quarter + 1), "r"((uint32_t)x), "n"(N)
       : "memory");
   return r != 0;
 }
+// 32 columns of this warp's 32 rows to registers; 16 from registers.
+__device__ __forceinline__ void tmem_ld_n(uint32_t taddr, uint32_t (&r)[32]) { tc::tmem_ld32(taddr, r); }
+__device__ __forceinline__ void tmem_st_n(uint32_t taddr, const uint32_t (&r)[16]) { tc::tmem_st16(taddr, r); }
 // 16 rows of 8 columns: lane l has columns 2 (l % 4) + {0, 1} of row l / 4 in
 // r[0], r[1] and of row l / 4 + 8 in r[2], r[3].
 __device__ __forceinline__ void tmem_st_rows16(uint32_t taddr, const uint32_t (&r)[4]) {
@@ -361,13 +364,18 @@ __device__ __forceinline__ float ex2(float x) {
 // An item as the roles of a CTA see it; kvh < 0: no more.
 struct Work {
   Item it;
-  int kvh, tiles;
+  int kvh, tiles, first_tok, first_head;  // of the item's first row
 };
+// x / d for 0 <= x < 2^21, inv = 1 / d: (x + 1/2) / d is at least 1 / 2d from a
+// whole number, more than the roundings move it.
+__device__ __forceinline__ int small_div(int x, float inv) { return (int)(((float)x + 0.5f) * inv); }
 
 template <int DP>
-__global__ void __launch_bounds__(kThreads, Cfg<DP>::kCtas) attention_prompt_kernel(const PromptArgs a) {
+__global__ void __launch_bounds__(Cfg<DP>::kThreads, Cfg<DP>::kCtas) attention_prompt_kernel(const PromptArgs a) {
   using C = Cfg<DP>;
-  constexpr int ST = C::kStages, NB = C::kBufs, W = DP / 2;  // W: output columns of a thread
+  constexpr int ST = C::kStages, NB = C::kBufs, kSoftWarps = C::kSoftWarps;
+  constexpr int P = C::kParts, kShare = 32 * P;  // threads that share 32 rows
+  constexpr int W = DP / P, K = kKeys / P;       // output columns and keys of a thread
   extern __shared__ unsigned char raw[];
   __shared__ __align__(8) uint64_t kfull[ST], kempty[ST], vfull[ST], vempty[ST];
   __shared__ __align__(8) uint64_t s_done[NB], p_ready[NB], o_done, o_free, q_ready, fin;
@@ -375,7 +383,7 @@ __global__ void __launch_bounds__(kThreads, Cfg<DP>::kCtas) attention_prompt_ker
   __shared__ Work work[2];
   __shared__ uint32_t tmem_slot;
   __shared__ volatile int abort_flag;
-  __shared__ float red[2][2][kRows], row_scale[kRows], red_l[2][kRows];
+  __shared__ float red[2][P][kRows], red_q[2][kRows], red_l[P][kRows];
   unsigned char* smem = reinterpret_cast<unsigned char*>(
       (reinterpret_cast<uintptr_t>(raw) + 1023) & ~(uintptr_t)1023);
   unsigned char* stage = smem + ST * C::kImage;
@@ -431,7 +439,10 @@ __global__ void __launch_bounds__(kThreads, Cfg<DP>::kCtas) attention_prompt_ker
         x.it = a.items[id / a.n_kv_heads];
         x.kvh = id % a.n_kv_heads;
         x.tiles = item_tiles(a, x.it.n, x.it.row);
-        const int first = x.it.row / a.group, behind = min(x.it.n, (x.it.row + kRows - 1) / a.group + 1);
+        const int first = x.it.row / a.group;
+        x.first_tok = first;
+        x.first_head = x.it.row - first * a.group;
+        const int behind = min(x.it.n, (x.it.row + kRows - 1) / a.group + 1);
         const uint32_t bytes = (uint32_t)min(a.group * a.head_dim, 1 << 16) * 4;
         for (int t = first + lane; t < behind; t += 32)
           asm volatile("cp.async.bulk.prefetch.L2.global [%0], %1;" ::"l"(
@@ -542,53 +553,65 @@ __global__ void __launch_bounds__(kThreads, Cfg<DP>::kCtas) attention_prompt_ker
   } else {
     // ---- the softmax.  After a wait that ran out the warps go on to the item's
     // end without waiting (their pairs meet at barriers) and store nothing.
-    const int quarter = warp & 3, half = warp >> 2;
+    const int quarter = warp & 3, part = warp >> 2;
     const int row = 32 * quarter + lane;
     const uint32_t lanes = (uint32_t)(32 * quarter) << 16;
+    const float inv_group = 1.0f / (float)a.group;
 
     struct Rows {  // this thread's row of an item
       int first_tok, tok, first, kvh, tiles, key_tiles, head;
       float fq;  // scores in base 2: S' fq 2^ek
+      float4 meta;  // of the item's first key tile
     };
     // Item w's row, and its queries scaled, split and stored to TMEM, once the
-    // last scores of item w - 1 are over; false: no more items.  A warp takes 16
-    // whole rows of its quarter here, 4 lanes a row.
+    // last scores of item w - 1 are over; false: no more items.  For the loads to
+    // be coalesced a warp takes 16 rows of its quarter here, 4 lanes a row, and
+    // with four warps to a quarter half of the columns.
     auto take_item = [&](int w, Rows& x) {
       const bool got = wait(&work_full[w & 1], w >> 1);
       const Work k = work[w & 1];
       tc::bar_arrive(&work_empty[w & 1]);
-      if (!pair_and(quarter, got && k.kvh >= 0)) return false;
+      if (!rows_and<kShare>(quarter, got && k.kvh >= 0)) return false;
+      x.meta = __ldcg(a.meta + (int64_t)k.it.key_tiles * a.n_kv_heads + k.kvh);
       const int rows = k.it.n * a.group - k.it.row;  // rows of the item, if under 128
-      const int f = k.it.row + row;
-      x.first_tok = k.it.row / a.group;
-      x.tok = row < rows ? f / a.group : -1;
-      x.head = k.kvh * a.group + f % a.group;
+      auto token = [&](int r, int& head) {  // of row r: counted from the first token
+        const int i = k.first_head + r, t = small_div(i, inv_group);
+        head = k.kvh * a.group + i - t * a.group;
+        return t;
+      };
+      x.first_tok = k.first_tok;
+      x.tok = token(row, x.head) + k.first_tok;
+      if (row >= rows) x.tok = -1;
       x.first = k.it.first, x.kvh = k.kvh, x.tiles = k.tiles, x.key_tiles = k.it.key_tiles;
 
-      const int part = lane & 3, r0 = 32 * quarter + 16 * half + (lane >> 2);
-      const uint32_t at = tmem + ((uint32_t)(32 * quarter + 16 * half) << 16) + C::kColQ;
+      constexpr int kCols = DP * 2 / P;  // columns of a warp
+      const int col0 = (part >> 1) * kCols + 4 * (lane & 3), r0 = 32 * quarter + 16 * (part & 1) + (lane >> 2);
+      const uint32_t at = tmem + ((uint32_t)(32 * quarter + 16 * (part & 1)) << 16) + C::kColQ +
+                          (part >> 1) * (kCols / 2);
       const float* from[2];
 #pragma unroll
       for (int i = 0; i < 2; ++i) {
-        const int fr = k.it.row + r0 + 8 * i;
-        from[i] = r0 + 8 * i < rows ? a.q + (int64_t)(k.it.first + fr / a.group) * a.ldq +
-                                          (int64_t)(k.kvh * a.group + fr % a.group) * a.head_dim + 4 * part
+        int head;
+        const int t = token(r0 + 8 * i, head) + k.first_tok;
+        from[i] = r0 + 8 * i < rows ? a.q + (int64_t)(k.it.first + t) * a.ldq + (int64_t)head * a.head_dim + col0
                                     : nullptr;
       }
       float top[2];
       // queries of ordinary size keep all their bits under one scale, 2^7; others
       // are read a second time, for a scale of their row
-      float up[2] = {128.0f, 128.0f};
+      constexpr int kUsual = -7;
+      auto unusual = [](float t) { return t > 0.0f && !(t >= 0x1p-10f && t < 256.0f); };
+      float up[2] = {pow2f(-kUsual), pow2f(-kUsual)};
       auto pass = [&] {
         top[0] = top[1] = 0.0f;
 #pragma unroll
-        for (int c0 = 0; c0 < DP / 16; c0 += 4) {
+        for (int c0 = 0; c0 < kCols / 16; c0 += 4) {
           float4 v[4][2];  // 8 loads at a time
 #pragma unroll
           for (int c = 0; c < 4; ++c)
 #pragma unroll
             for (int i = 0; i < 2; ++i)
-              v[c][i] = from[i] && 16 * (c0 + c) + 4 * part < a.head_dim
+              v[c][i] = from[i] && 16 * (c0 + c) + col0 < a.head_dim
                             ? __ldg(reinterpret_cast<const float4*>(from[i] + 16 * (c0 + c)))
                             : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
 #pragma unroll
@@ -607,26 +630,24 @@ __global__ void __launch_bounds__(kThreads, Cfg<DP>::kCtas) attention_prompt_ker
         }
       };
       pass();
-      bool fits = true;
 #pragma unroll
       for (int i = 0; i < 2; ++i) {
         top[i] = fmaxf(top[i], __shfl_xor_sync(0xffffffffu, top[i], 1));
         top[i] = fmaxf(top[i], __shfl_xor_sync(0xffffffffu, top[i], 2));
-        if (top[i] > 0.0f && !(top[i] >= 0x1p-10f && top[i] < 256.0f)) {
-          up[i] = pow2f(-pow2_ex(top[i]));
-          fits = false;
-        }
+        if ((lane & 3) == 0) red_q[part >> 1][r0 + 8 * i] = top[i];
       }
-      if (!__all_sync(0xffffffffu, fits)) pass();
-      if (part == 0) {
-        row_scale[r0] = a.scale / up[0];
-        row_scale[r0 + 8] = a.scale / up[1];
+      rows_sync<kShare>(quarter);
+      auto row_top = [&](int r) { return P == 4 ? fmaxf(red_q[0][r], red_q[1][r]) : red_q[0][r]; };
+      const float t0 = row_top(r0), t1 = row_top(r0 + 8), mine = row_top(row);
+      if (__any_sync(0xffffffffu, unusual(t0) || unusual(t1))) {
+        if (unusual(t0)) up[0] = pow2f(-pow2_ex(t0));
+        if (unusual(t1)) up[1] = pow2f(-pow2_ex(t1));
+        pass();
       }
       tc::tmem_wait_st();
       tc::tc_fence_before();
       tc::bar_arrive(&q_ready);
-      pair_sync(quarter);
-      x.fq = row_scale[row];
+      x.fq = a.scale * pow2f(unusual(mine) ? pow2_ex(mine) : kUsual);
       return true;
     };
 
@@ -644,19 +665,24 @@ __global__ void __launch_bounds__(kThreads, Cfg<DP>::kCtas) attention_prompt_ker
       auto take_output = [&](int at) {
         wait(&o_done, at);
         tc::tc_fence_after();
+        if (__any_sync(0xffffffffu, corr != 1.0f)) {
+#pragma unroll
+          for (int d = 0; d < W; ++d) o[d] *= corr;
+        }
 #pragma unroll
         for (int c = 0; c < W; c += 32) {
           uint32_t r[32];
-          tc::tmem_ld32(tmem + lanes + C::kColO + half * W + c, r);
+          tc::tmem_ld32(tmem + lanes + C::kColO + part * W + c, r);
           tc::tmem_wait_ld();
+          if (c + 32 == W) {
+            tc::tc_fence_before();
+            tc::bar_arrive(&o_free);
+          }
 #pragma unroll
-          for (int d = 0; d < 32; ++d)
-            o[c + d] = fmaf(__uint_as_float(r[d]), vscale, o[c + d] * corr);
+          for (int d = 0; d < 32; ++d) o[c + d] = fmaf(__uint_as_float(r[d]), vscale, o[c + d]);
         }
-        tc::tc_fence_before();
-        tc::bar_arrive(&o_free);
       };
-      float4 next = __ldcg(meta);
+      float4 next = cur.meta;
       for (int j = 0; j < nt; ++j, ++T) {
         const float4 mt = next;
         if (j + 1 < nt) next = __ldcg(meta + (int64_t)(j + 1) * a.n_kv_heads);
@@ -664,33 +690,34 @@ __global__ void __launch_bounds__(kThreads, Cfg<DP>::kCtas) attention_prompt_ker
         const uint32_t buf = tmem + lanes + C::kColS + 64u * (T % NB);
         wait(&s_done[T % NB], T / NB);
         tc::tc_fence_after();
-        uint32_t r[32];
-        tc::tmem_ld32(buf + 32 * half, r);
+        uint32_t r[K];
+        tmem_ld_n(buf + K * part, r);
         tc::tmem_wait_ld();
         const bool slow = mt.z != 0.0f;  // the whole CTA's
         float tmax = -INFINITY;
         if (kt + kKeys - 1 <= cur.first_tok) {  // every key is visible to every row
 #pragma unroll
-          for (int i = 0; i < 32; ++i) tmax = fmaxf(tmax, __uint_as_float(r[i]));
+          for (int i = 0; i < K; ++i) tmax = fmaxf(tmax, __uint_as_float(r[i]));
         } else {
 #pragma unroll
-          for (int i = 0; i < 32; ++i) {
-            if (kt + 32 * half + i > cur.tok) r[i] = 0xff800000u;  // -inf
+          for (int i = 0; i < K; ++i) {
+            if (kt + K * part + i > cur.tok) r[i] = 0xff800000u;  // -inf
             tmax = fmaxf(tmax, __uint_as_float(r[i]));
           }
         }
-        red[T & 1][half][row] = tmax;
-        pair_sync(quarter);
-        tmax = fmaxf(red[T & 1][0][row], red[T & 1][1][row]);
+        red[T & 1][part][row] = tmax;
+        rows_sync<kShare>(quarter);
+#pragma unroll
+        for (int i = 0; i < P; ++i) tmax = fmaxf(tmax, red[T & 1][i][row]);
         const float fs = cur.fq * mt.x;
         const float mnew = slow ? m : fmaxf(m, tmax * fs);
         const float ref = mnew == -INFINITY ? 0.0f : mnew;
         const float c = ex2(m - ref);
         m = mnew;
-        uint32_t ph[16], pl[16];
+        uint32_t ph[K / 2], pl[K / 2];
         float sum = 0.0f;
 #pragma unroll
-        for (int i = 0; i < 16; ++i) {
+        for (int i = 0; i < K / 2; ++i) {
           float p0 = ex2(fmaf(__uint_as_float(r[2 * i]), fs, 14.0f - ref));
           float p1 = ex2(fmaf(__uint_as_float(r[2 * i + 1]), fs, 14.0f - ref));
           if (slow) p0 = p1 = 0.0f;
@@ -699,8 +726,8 @@ __global__ void __launch_bounds__(kThreads, Cfg<DP>::kCtas) attention_prompt_ker
           split2(p0, p1, ph[i], pl[i]);
         }
         if (!slow) l = fmaf(l, c, sum);
-        tc::tmem_st16(buf + 16 * half, ph);
-        tc::tmem_st16(buf + 32 + 16 * half, pl);
+        tmem_st_n(buf + K / 2 * part, ph);
+        tmem_st_n(buf + 32 + K / 2 * part, pl);
         tc::tmem_wait_st();
         tc::tc_fence_before();
         tc::bar_arrive(&p_ready[T % NB]);
@@ -719,11 +746,11 @@ __global__ void __launch_bounds__(kThreads, Cfg<DP>::kCtas) attention_prompt_ker
             const float top = fmaxf(m, s), at = top == -INFINITY ? 0.0f : top;
             const float down = ex2(m - at), p = ex2(s - at + 14.0f);
             l *= down;
-            if (half == 0) l += p;
+            if (part == 0) l += p;
             m = top;
 #pragma unroll
             for (int d = 0; d < W; ++d) {
-              const int dd = half * W + d;
+              const int dd = part * W + d;
               o[d] = fmaf(p, dd < a.head_dim ? vr[dd] : 0.0f, o[d] * down);
             }
           }
@@ -731,24 +758,27 @@ __global__ void __launch_bounds__(kThreads, Cfg<DP>::kCtas) attention_prompt_ker
       }
       have = take_item(w + 1, nxt);
       take_output(T - 1);
-      red_l[half][row] = l;
+      red_l[part][row] = l;
       // the last item's outputs have left the stage
       asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory");
-      pair_sync(quarter);
-      l = red_l[0][row] + red_l[1][row];
+      rows_sync<kShare>(quarter);
+      l = red_l[0][row];
+#pragma unroll
+      for (int i = 1; i < P; ++i) l += red_l[i][row];
       const float inv = __frcp_rn(l);
-      float4* to = reinterpret_cast<float4*>(stage + row * C::kRowBytes) + half * (W / 4);
+      float4* to = reinterpret_cast<float4*>(stage + row * C::kRowBytes) + part * (W / 4);
 #pragma unroll
       for (int i = 0; i < W / 4; ++i)
         to[i] = make_float4(o[4 * i] * inv, o[4 * i + 1] * inv, o[4 * i + 2] * inv, o[4 * i + 3] * inv);
       tc::fence_proxy_async_smem();
-      pair_sync(quarter);
-      // a copy takes 60 cycles to issue: 16 rows a warp
-      const int tok = __shfl_sync(0xffffffffu, cur.tok, 16 * half + (lane & 15));
-      const int head = __shfl_sync(0xffffffffu, cur.head, 16 * half + (lane & 15));
-      if (lane < 16 && tok >= 0 && !abort_flag)
+      rows_sync<kShare>(quarter);
+      // a copy takes 60 cycles to issue: 32 / P rows a warp
+      constexpr int kEach = 32 / P;
+      const int src = kEach * part + lane % kEach;
+      const int tok = __shfl_sync(0xffffffffu, cur.tok, src), head = __shfl_sync(0xffffffffu, cur.head, src);
+      if (lane < kEach && tok >= 0 && !abort_flag)
         bulk_store(a.out + (int64_t)(cur.first + tok) * a.ldo + (int64_t)head * a.head_dim,
-                   stage + (32 * quarter + 16 * half + lane) * C::kRowBytes, (uint32_t)a.head_dim * 4);
+                   stage + (32 * quarter + src) * C::kRowBytes, (uint32_t)a.head_dim * 4);
       cur = nxt;
     }
     asm volatile("cp.async.bulk.wait_group 0;" ::: "memory");
@@ -788,7 +818,7 @@ cudaError_t launch_prompt(const PromptArgs& a, cudaStream_t st) {
   if (e != cudaSuccess) return e;
   const int64_t items = (int64_t)a.max_items * a.n_kv_heads, most = (int64_t)Cfg<DP>::kCtas * sm_count();
   return launch(attention_prompt_kernel<DP>, dim3((unsigned)(items < most ? items : most)),
-                dim3(kThreads), Cfg<DP>::kSmem, st, use_pdl(), a);
+                dim3(Cfg<DP>::kThreads), Cfg<DP>::kSmem, st, use_pdl(), a);
 }
 
 bool prompt_shape_ok(int n_heads, int n_kv_heads, int head_dim) {

@@ -83,105 +83,111 @@ __device__ __forceinline__ int64_t token_row(const RowsArgs& a, int token, int h
   return first_tile(a.c, slot, head) * kTile + pos;
 }
 
-// 8 lanes take one block, 4 values each.  VEC: 16-byte accesses to the f32
-// rows.
-template <bool VEC>
-__global__ void __launch_bounds__(256) kv_q40_write_kernel(RowsArgs a) {
-  const int nb = a.c.nb, lane = threadIdx.x & 31, i8 = lane & 7;
-  const int64_t per_token = (int64_t)2 * a.c.n_kv_heads * nb;  // blocks of K, then of V
-  const int64_t total = per_token * a.n_tokens;
-  const int64_t stride = (int64_t)gridDim.x * (blockDim.x / 8);
-  int64_t item = ((int64_t)blockIdx.x * blockDim.x + threadIdx.x) / 8;
+// A CTA takes kTokens tokens; 8 lanes take one block of a token's rows (K's
+// heads, then V's), 4 values each, the same block of all its tokens, whose loads
+// are in flight together.  VEC: 16-byte accesses to the f32 rows.  Bound by
+// memory: 4 bytes a value in, 0.56 out.
+constexpr int kRowThreads = 256, kTokens = 2;
+
+template <int NB, bool VEC>
+__global__ void __launch_bounds__(kRowThreads) kv_q40_write_kernel(const RowsArgs a) {
+  const int i8 = threadIdx.x & 7, blocks = a.c.n_kv_heads * NB;
+  const int64_t token0 = (int64_t)blockIdx.x * kTokens;
   // whole warps stay in the loop: the shuffles name every lane
-  for (; item - (lane >> 3) < total; item += stride) {
-    const bool live = item < total;
-    const int token = live ? (int)(item / per_token) : 0;
-    int r = live ? (int)(item % per_token) : 0;
-    const bool is_v = r >= a.c.n_kv_heads * nb;
-    if (is_v) r -= a.c.n_kv_heads * nb;
-    const int head = r / nb, b = r % nb;
-    float x[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-    if (live) {
-      const float* src = (is_v ? a.v + token * a.ldv : a.k + token * a.ldk) +
-                         ((int64_t)head * nb + b) * 32 + 4 * i8;
+  for (int u0 = (threadIdx.x & ~31) >> 3; u0 < 2 * blocks; u0 += kRowThreads / 8) {
+    const int u = u0 + ((threadIdx.x & 31) >> 3);
+    const bool live = u < 2 * blocks, is_v = u >= blocks;
+    const int r = is_v ? u - blocks : u, head = r / NB, b = r % NB;
+    const float* src = is_v ? a.v : a.k;
+    const int64_t ld = is_v ? a.ldv : a.ldk;
+    float x[kTokens][4];
+    int64_t row[kTokens];
+#pragma unroll
+    for (int n = 0; n < kTokens; ++n) {
+      const bool in = live && token0 + n < a.n_tokens;
+      const float* p = src + (token0 + n) * ld + r * 32 + 4 * i8;
       if constexpr (VEC) {
-        const float4 f = ldg_f4_stream(src);
-        x[0] = f.x, x[1] = f.y, x[2] = f.z, x[3] = f.w;
+        const float4 f = in ? ldg_f4_stream(p) : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+        x[n][0] = f.x, x[n][1] = f.y, x[n][2] = f.z, x[n][3] = f.w;
       } else {
 #pragma unroll
-        for (int e = 0; e < 4; ++e) x[e] = src[e];
+        for (int e = 0; e < 4; ++e) x[n][e] = in ? p[e] : 0.0f;
       }
+      row[n] = in ? token_row(a, (int)(token0 + n), head) : -1;
     }
-    float top = fmaxf(fmaxf(fabsf(x[0]), fabsf(x[1])), fmaxf(fabsf(x[2]), fabsf(x[3])));
 #pragma unroll
-    for (int o = 1; o < 8; o <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
-    uint16_t d = 0;
-    uint32_t codes = 0;  // byte e: the code of value 4 i8 + e
-    if (top > 0.0f) {
-      d = f2h_ref(__fdiv_rn(top, 7.0f));
-      const float stored = h2f(d);
-      const float inv = stored == 0.0f ? 0.0f : __fdiv_rn(1.0f, stored);
+    for (int n = 0; n < kTokens; ++n) {
+      float top = fmaxf(fmaxf(fabsf(x[n][0]), fabsf(x[n][1])), fmaxf(fabsf(x[n][2]), fabsf(x[n][3])));
 #pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        int q = (int)roundf(__fadd_rn(__fmul_rn(x[e], inv), 8.0f));
-        q = q < 0 ? 0 : (q > 15 ? 15 : q);
-        codes |= (uint32_t)q << (8 * e);
+      for (int o = 1; o < 8; o <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+      uint16_t d = 0;
+      uint32_t codes = 0;  // byte e: the code of value 4 i8 + e
+      if (top > 0.0f) {
+        d = f2h_ref(__fdiv_rn(top, 7.0f));
+        const float stored = h2f(d);
+        const float inv = stored == 0.0f ? 0.0f : __fdiv_rn(1.0f, stored);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          int q = (int)roundf(__fadd_rn(__fmul_rn(x[n][e], inv), 8.0f));
+          q = q < 0 ? 0 : (q > 15 ? 15 : q);
+          codes |= (uint32_t)q << (8 * e);
+        }
       }
-    }
-    // lanes 0-3 hold values 0..15 of the block, lanes 4-7 values 16..31
-    const uint32_t high = __shfl_down_sync(0xffffffffu, codes, 4, 8);
-    const int64_t row = live ? token_row(a, token, head) : -1;
-    if (row < 0) continue;
-    const uint32_t word = codes | high << 4;
-    unsigned char* base = is_v ? a.c.v : a.c.k;
-    if (i8 < 4) {
-      if (is_v) {
-        *reinterpret_cast<uint16_t*>(base + value_at(row, 2 * i8, b, nb)) = (uint16_t)word;
-        *reinterpret_cast<uint16_t*>(base + value_at(row, 2 * i8 + 1, b, nb)) = (uint16_t)(word >> 16);
-      } else {
-        *reinterpret_cast<uint32_t*>(base + key_at(row, i8, b, nb)) = word;
+      // lanes 0-3 hold values 0..15 of the block, lanes 4-7 values 16..31
+      const uint32_t word = codes | __shfl_down_sync(0xffffffffu, codes, 4, 8) << 4;
+      if (row[n] < 0) continue;
+      unsigned char* base = is_v ? a.c.v : a.c.k;
+      if (i8 < 4) {
+        if (is_v) {
+          *reinterpret_cast<uint16_t*>(base + value_at(row[n], 2 * i8, b, NB)) = (uint16_t)word;
+          *reinterpret_cast<uint16_t*>(base + value_at(row[n], 2 * i8 + 1, b, NB)) = (uint16_t)(word >> 16);
+        } else {
+          *reinterpret_cast<uint32_t*>(base + key_at(row[n], i8, b, NB)) = word;
+        }
       }
+      if (i8 == 4) *reinterpret_cast<uint16_t*>(base + scale_at(row[n], b, NB)) = d;
     }
-    if (i8 == 0) *reinterpret_cast<uint16_t*>(base + scale_at(row, b, nb)) = d;
   }
 }
 
-template <bool VEC>
-__global__ void __launch_bounds__(256) kv_q40_read_kernel(RowsArgs a) {
-  const int nb = a.c.nb;
-  const int64_t per_token = (int64_t)2 * a.c.n_kv_heads * nb;
-  const int64_t total = per_token * a.n_tokens * 8;
-  for (int64_t i = (int64_t)blockIdx.x * blockDim.x + threadIdx.x; i < total;
-       i += (int64_t)gridDim.x * blockDim.x) {
-    const int i8 = (int)(i & 7);
-    const int64_t item = i >> 3;
-    const int token = (int)(item / per_token);
-    int r = (int)(item % per_token);
-    const bool is_v = r >= a.c.n_kv_heads * nb;
-    if (is_v) r -= a.c.n_kv_heads * nb;
-    const int head = r / nb, b = r % nb, t = i8 & 3;
-    const int64_t row = token_row(a, token, head);
-    if (row < 0) continue;
-    uint32_t word;
+template <int NB, bool VEC>
+__global__ void __launch_bounds__(kRowThreads) kv_q40_read_kernel(const RowsArgs a) {
+  const int i8 = threadIdx.x & 7, t = i8 & 3, blocks = a.c.n_kv_heads * NB;
+  const int64_t token0 = (int64_t)blockIdx.x * kTokens;
+  for (int u = threadIdx.x >> 3; u < 2 * blocks; u += kRowThreads / 8) {
+    const bool is_v = u >= blocks;
+    const int r = is_v ? u - blocks : u, head = r / NB, b = r % NB;
     const unsigned char* base = is_v ? a.c.v : a.c.k;
-    if (is_v) {
-      word = *reinterpret_cast<const uint16_t*>(base + value_at(row, 2 * t, b, nb)) |
-             (uint32_t)*reinterpret_cast<const uint16_t*>(base + value_at(row, 2 * t + 1, b, nb)) << 16;
-    } else {
-      word = *reinterpret_cast<const uint32_t*>(base + key_at(row, t, b, nb));
+    uint32_t word[kTokens];
+    float d[kTokens];
+    bool in[kTokens];
+#pragma unroll
+    for (int n = 0; n < kTokens; ++n) {
+      const int64_t row = token0 + n < a.n_tokens ? token_row(a, (int)(token0 + n), head) : -1;
+      in[n] = row >= 0;
+      word[n] = 0, d[n] = 0.0f;
+      if (!in[n]) continue;
+      if (is_v)
+        word[n] = *reinterpret_cast<const uint16_t*>(base + value_at(row, 2 * t, b, NB)) |
+                  (uint32_t)*reinterpret_cast<const uint16_t*>(base + value_at(row, 2 * t + 1, b, NB)) << 16;
+      else
+        word[n] = *reinterpret_cast<const uint32_t*>(base + key_at(row, t, b, NB));
+      d[n] = h2f(*reinterpret_cast<const uint16_t*>(base + scale_at(row, b, NB)));
     }
-    if (i8 >= 4) word >>= 4;
-    const float d = h2f(*reinterpret_cast<const uint16_t*>(base + scale_at(row, b, nb)));
-    float y[4];
 #pragma unroll
-    for (int e = 0; e < 4; ++e) y[e] = __fmul_rn(d, (float)(int)((word >> (8 * e)) & 15u) - 8.0f);
-    float* dst = (is_v ? a.vo + token * a.ldv : a.ko + token * a.ldk) +
-                 ((int64_t)head * nb + b) * 32 + 4 * i8;
-    if constexpr (VEC) {
-      *reinterpret_cast<float4*>(dst) = make_float4(y[0], y[1], y[2], y[3]);
-    } else {
+    for (int n = 0; n < kTokens; ++n) {
+      if (!in[n]) continue;
+      const uint32_t w = i8 >= 4 ? word[n] >> 4 : word[n];
+      float y[4];
 #pragma unroll
-      for (int e = 0; e < 4; ++e) dst[e] = y[e];
+      for (int e = 0; e < 4; ++e) y[e] = __fmul_rn(d[n], (float)(int)((w >> (8 * e)) & 15u) - 8.0f);
+      float* dst = (is_v ? a.vo + (token0 + n) * a.ldv : a.ko + (token0 + n) * a.ldk) + r * 32 + 4 * i8;
+      if constexpr (VEC) {
+        *reinterpret_cast<float4*>(dst) = make_float4(y[0], y[1], y[2], y[3]);
+      } else {
+#pragma unroll
+        for (int e = 0; e < 4; ++e) dst[e] = y[e];
+      }
     }
   }
 }
@@ -868,10 +874,22 @@ int check_cache(const std::string& api, const dqmk_kv_q40* kv, int layer, Plane*
   return DQMK_OK;
 }
 
-unsigned rows_grid(const Plane& c, int n_tokens) {
-  const int64_t threads = (int64_t)2 * c.n_kv_heads * c.nb * n_tokens * 8;
-  const int64_t blocks = (threads + 255) / 256, most = (int64_t)sm_count() * 32;
-  return (unsigned)(blocks < most ? blocks : most);
+template <int NB>
+cudaError_t launch_rows(bool write, bool vec, const RowsArgs& a, cudaStream_t st) {
+  const dim3 grid((unsigned)(((int64_t)a.n_tokens + kTokens - 1) / kTokens)), block(kRowThreads);
+  if (write)
+    return vec ? launch(kv_q40_write_kernel<NB, true>, grid, block, 0, st, false, a)
+               : launch(kv_q40_write_kernel<NB, false>, grid, block, 0, st, false, a);
+  return vec ? launch(kv_q40_read_kernel<NB, true>, grid, block, 0, st, false, a)
+             : launch(kv_q40_read_kernel<NB, false>, grid, block, 0, st, false, a);
+}
+cudaError_t launch_rows(bool write, bool vec, const RowsArgs& a, cudaStream_t st) {
+  switch (a.c.nb) {
+    case 1: return launch_rows<1>(write, vec, a, st);
+    case 2: return launch_rows<2>(write, vec, a, st);
+    case 3: return launch_rows<3>(write, vec, a, st);
+    default: return launch_rows<4>(write, vec, a, st);
+  }
 }
 
 bool vec_rows(const void* k, const void* v, int64_t ldk, int64_t ldv) {
@@ -922,11 +940,7 @@ extern "C" int dqmk_kv_q40_write(const dqmk_kv_q40* kv, int layer, const float* 
   if (n_tokens == 0) return DQMK_OK;
   a.k = k, a.v = v, a.ldk = ldk, a.ldv = ldv;
   a.slots = slots, a.positions = positions, a.n_tokens = n_tokens;
-  const dim3 grid(rows_grid(a.c, n_tokens)), block(256);
-  cudaStream_t st = static_cast<cudaStream_t>(stream);
-  DQMK_CUDA_RET(api.c_str(), vec_rows(k, v, ldk, ldv)
-                                 ? launch(kv_q40_write_kernel<true>, grid, block, 0, st, false, a)
-                                 : launch(kv_q40_write_kernel<false>, grid, block, 0, st, false, a));
+  DQMK_CUDA_RET(api.c_str(), launch_rows(true, vec_rows(k, v, ldk, ldv), a, static_cast<cudaStream_t>(stream)));
   return DQMK_OK;
 }
 
@@ -941,11 +955,7 @@ extern "C" int dqmk_kv_q40_read(const dqmk_kv_q40* kv, int layer, const int* slo
   if (n_tokens == 0) return DQMK_OK;
   a.ko = k, a.vo = v, a.ldk = ldk, a.ldv = ldv;
   a.slots = slots, a.positions = positions, a.n_tokens = n_tokens;
-  const dim3 grid(rows_grid(a.c, n_tokens)), block(256);
-  cudaStream_t st = static_cast<cudaStream_t>(stream);
-  DQMK_CUDA_RET(api.c_str(), vec_rows(k, v, ldk, ldv)
-                                 ? launch(kv_q40_read_kernel<true>, grid, block, 0, st, false, a)
-                                 : launch(kv_q40_read_kernel<false>, grid, block, 0, st, false, a));
+  DQMK_CUDA_RET(api.c_str(), launch_rows(false, vec_rows(k, v, ldk, ldv), a, static_cast<cudaStream_t>(stream)));
   return DQMK_OK;
 }
 

@@ -83,105 +83,140 @@ __device__ __forceinline__ int64_t token_row(const RowsArgs& a, int token, int h
   return first_tile(a.c, slot, head) * kTile + pos;
 }
 
-// A CTA takes kTokens tokens; 8 lanes take one block of a token's rows (K's
-// heads, then V's), 4 values each, the same block of all its tokens, whose loads
-// are in flight together.  VEC: 16-byte accesses to the f32 rows.  Bound by
-// memory: 4 bytes a value in, 0.56 out.
-constexpr int kRowThreads = 256, kTokens = 2;
+// 8 lanes take one block of a token's rows (K's heads, then V's), 4 values each,
+// the same block of TOK tokens, whose loads are in flight together.  With 8
+// tokens lane j also works out token j's row and scale for the other lanes: the
+// divisions and the rounding of the scale take more instructions than a block's
+// values, and with each lane repeating them the kernel was bound by its
+// instructions (21 us for 8191 tokens of 4 heads of 128 against a floor of 6).
+// VEC: 16-byte accesses to the f32 rows.
+constexpr int kRowThreads = 256;
 
-template <int NB, bool VEC>
+__device__ __forceinline__ int64_t shfl8(int64_t x, int lane) {
+  const int lo = __shfl_sync(0xffffffffu, (int)x, lane, 8), hi = __shfl_sync(0xffffffffu, (int)(x >> 32), lane, 8);
+  return (int64_t)((uint64_t)(uint32_t)hi << 32 | (uint32_t)lo);
+}
+// Element `i` of an array in registers.
+template <int N>
+__device__ __forceinline__ float pick(const float (&x)[N], int i) {
+  float y = x[0];
+#pragma unroll
+  for (int n = 1; n < N; ++n) y = i == n ? x[n] : y;
+  return y;
+}
+
+template <int NB, int TOK, bool VEC>
 __global__ void __launch_bounds__(kRowThreads) kv_q40_write_kernel(const RowsArgs a) {
   const int i8 = threadIdx.x & 7, blocks = a.c.n_kv_heads * NB;
-  const int64_t token0 = (int64_t)blockIdx.x * kTokens;
+  const int64_t token0 = (int64_t)blockIdx.x * TOK;
+  const int tokens = (int)min((int64_t)TOK, a.n_tokens - token0);
   // whole warps stay in the loop: the shuffles name every lane
   for (int u0 = (threadIdx.x & ~31) >> 3; u0 < 2 * blocks; u0 += kRowThreads / 8) {
-    const int u = u0 + ((threadIdx.x & 31) >> 3);
-    const bool live = u < 2 * blocks, is_v = u >= blocks;
+    const int u = min(u0 + (int)((threadIdx.x & 31) >> 3), 2 * blocks - 1);
+    const bool live = u == u0 + (int)((threadIdx.x & 31) >> 3), is_v = u >= blocks;
     const int r = is_v ? u - blocks : u, head = r / NB, b = r % NB;
-    const float* src = is_v ? a.v : a.k;
     const int64_t ld = is_v ? a.ldv : a.ldk;
-    float x[kTokens][4];
-    int64_t row[kTokens];
+    const float* src = (is_v ? a.v : a.k) + token0 * ld + r * 32 + 4 * i8;
+    float x[TOK][4], top[TOK];
 #pragma unroll
-    for (int n = 0; n < kTokens; ++n) {
-      const bool in = live && token0 + n < a.n_tokens;
-      const float* p = src + (token0 + n) * ld + r * 32 + 4 * i8;
+    for (int n = 0; n < TOK; ++n) {
+      const float* p = src + n * ld;
       if constexpr (VEC) {
-        const float4 f = in ? ldg_f4_stream(p) : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+        const float4 f = n < tokens ? ldg_f4_stream(p) : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
         x[n][0] = f.x, x[n][1] = f.y, x[n][2] = f.z, x[n][3] = f.w;
       } else {
 #pragma unroll
-        for (int e = 0; e < 4; ++e) x[n][e] = in ? p[e] : 0.0f;
+        for (int e = 0; e < 4; ++e) x[n][e] = n < tokens ? p[e] : 0.0f;
       }
-      row[n] = in ? token_row(a, (int)(token0 + n), head) : -1;
+    }
+    const int own = TOK == 8 ? i8 : 0;  // the token this lane works out
+    const int64_t own_row = live && own < tokens ? token_row(a, (int)(token0 + own), head) : -1;
+#pragma unroll
+    for (int n = 0; n < TOK; ++n) {
+      top[n] = fmaxf(fmaxf(fabsf(x[n][0]), fabsf(x[n][1])), fmaxf(fabsf(x[n][2]), fabsf(x[n][3])));
+#pragma unroll
+      for (int o = 1; o < 8; o <<= 1) top[n] = fmaxf(top[n], __shfl_xor_sync(0xffffffffu, top[n], o));
+    }
+    const float own_top = pick(top, own);
+    float own_inv = 0.0f;
+    if (own_top > 0.0f) {
+      const uint16_t d = f2h_ref(__fdiv_rn(own_top, 7.0f));
+      const float stored = h2f(d);
+      own_inv = stored == 0.0f ? 0.0f : __fdiv_rn(1.0f, stored);
+      if (own_row >= 0 && (TOK == 8 || i8 == 0))
+        *reinterpret_cast<uint16_t*>((is_v ? a.c.v : a.c.k) + scale_at(own_row, b, NB)) = d;
+    } else if (own_row >= 0 && (TOK == 8 || i8 == 0)) {
+      *reinterpret_cast<uint16_t*>((is_v ? a.c.v : a.c.k) + scale_at(own_row, b, NB)) = 0;
     }
 #pragma unroll
-    for (int n = 0; n < kTokens; ++n) {
-      float top = fmaxf(fmaxf(fabsf(x[n][0]), fabsf(x[n][1])), fmaxf(fabsf(x[n][2]), fabsf(x[n][3])));
+    for (int n = 0; n < TOK; ++n) {
+      const float inv = TOK == 8 ? __shfl_sync(0xffffffffu, own_inv, n, 8) : own_inv;
+      const int64_t row = TOK == 8 ? shfl8(own_row, n) : own_row;
+      // round(x inv + 8) held to 0 .. 15: with y = x inv + 8 a multiple of 2^-21
+      // below 8, y + 1/2 is exact where it could reach the next whole number, so
+      // its floor is y rounded with halves up; adding 2^23 rounded down leaves
+      // it in the low bits.  A NaN (inf times 0) is held at 0.
+      uint32_t q[4];
 #pragma unroll
-      for (int o = 1; o < 8; o <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
-      uint16_t d = 0;
-      uint32_t codes = 0;  // byte e: the code of value 4 i8 + e
-      if (top > 0.0f) {
-        d = f2h_ref(__fdiv_rn(top, 7.0f));
-        const float stored = h2f(d);
-        const float inv = stored == 0.0f ? 0.0f : __fdiv_rn(1.0f, stored);
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          int q = (int)roundf(__fadd_rn(__fmul_rn(x[n][e], inv), 8.0f));
-          q = q < 0 ? 0 : (q > 15 ? 15 : q);
-          codes |= (uint32_t)q << (8 * e);
-        }
+      for (int e = 0; e < 4; ++e) {
+        const float y = __fadd_rn(__fmul_rn(x[n][e], inv), 8.0f);
+        const float z = fminf(fmaxf(__fadd_rn(y, 0.5f), 0.0f), 15.5f);
+        q[e] = __float_as_uint(__fadd_rd(z, 8388608.0f));
       }
+      uint32_t codes = __byte_perm(__byte_perm(q[0], q[1], 0x0040), __byte_perm(q[2], q[3], 0x0040), 0x5410);
+      if (!(top[n] > 0.0f)) codes = 0;  // a block without a value above 0 (or of NaN): codes and scale 0
       // lanes 0-3 hold values 0..15 of the block, lanes 4-7 values 16..31
       const uint32_t word = codes | __shfl_down_sync(0xffffffffu, codes, 4, 8) << 4;
-      if (row[n] < 0) continue;
-      unsigned char* base = is_v ? a.c.v : a.c.k;
-      if (i8 < 4) {
-        if (is_v) {
-          *reinterpret_cast<uint16_t*>(base + value_at(row[n], 2 * i8, b, NB)) = (uint16_t)word;
-          *reinterpret_cast<uint16_t*>(base + value_at(row[n], 2 * i8 + 1, b, NB)) = (uint16_t)(word >> 16);
-        } else {
-          *reinterpret_cast<uint32_t*>(base + key_at(row[n], i8, b, NB)) = word;
-        }
+      if (row < 0 || i8 >= 4) continue;
+      if (is_v) {
+        *reinterpret_cast<uint16_t*>(a.c.v + value_at(row, 2 * i8, b, NB)) = (uint16_t)word;
+        *reinterpret_cast<uint16_t*>(a.c.v + value_at(row, 2 * i8 + 1, b, NB)) = (uint16_t)(word >> 16);
+      } else {
+        *reinterpret_cast<uint32_t*>(a.c.k + key_at(row, i8, b, NB)) = word;
       }
-      if (i8 == 4) *reinterpret_cast<uint16_t*>(base + scale_at(row[n], b, NB)) = d;
     }
   }
 }
 
-template <int NB, bool VEC>
+template <int NB, int TOK, bool VEC>
 __global__ void __launch_bounds__(kRowThreads) kv_q40_read_kernel(const RowsArgs a) {
   const int i8 = threadIdx.x & 7, t = i8 & 3, blocks = a.c.n_kv_heads * NB;
-  const int64_t token0 = (int64_t)blockIdx.x * kTokens;
-  for (int u = threadIdx.x >> 3; u < 2 * blocks; u += kRowThreads / 8) {
-    const bool is_v = u >= blocks;
+  const int64_t token0 = (int64_t)blockIdx.x * TOK;
+  const int tokens = (int)min((int64_t)TOK, a.n_tokens - token0);
+  for (int u0 = (threadIdx.x & ~31) >> 3; u0 < 2 * blocks; u0 += kRowThreads / 8) {
+    const int u = min(u0 + (int)((threadIdx.x & 31) >> 3), 2 * blocks - 1);
+    const bool live = u == u0 + (int)((threadIdx.x & 31) >> 3), is_v = u >= blocks;
     const int r = is_v ? u - blocks : u, head = r / NB, b = r % NB;
     const unsigned char* base = is_v ? a.c.v : a.c.k;
-    uint32_t word[kTokens];
-    float d[kTokens];
-    bool in[kTokens];
+    const int own = TOK == 8 ? i8 : 0;
+    const int64_t own_row = live && own < tokens ? token_row(a, (int)(token0 + own), head) : -1;
+    const float own_d =
+        own_row >= 0 ? h2f(*reinterpret_cast<const uint16_t*>(base + scale_at(own_row, b, NB))) : 0.0f;
+    uint32_t word[TOK];
+    bool in[TOK];
 #pragma unroll
-    for (int n = 0; n < kTokens; ++n) {
-      const int64_t row = token0 + n < a.n_tokens ? token_row(a, (int)(token0 + n), head) : -1;
+    for (int n = 0; n < TOK; ++n) {
+      const int64_t row = TOK == 8 ? shfl8(own_row, n) : own_row;
       in[n] = row >= 0;
-      word[n] = 0, d[n] = 0.0f;
+      word[n] = 0;
       if (!in[n]) continue;
       if (is_v)
         word[n] = *reinterpret_cast<const uint16_t*>(base + value_at(row, 2 * t, b, NB)) |
                   (uint32_t)*reinterpret_cast<const uint16_t*>(base + value_at(row, 2 * t + 1, b, NB)) << 16;
       else
         word[n] = *reinterpret_cast<const uint32_t*>(base + key_at(row, t, b, NB));
-      d[n] = h2f(*reinterpret_cast<const uint16_t*>(base + scale_at(row, b, NB)));
     }
+    const int64_t ld = is_v ? a.ldv : a.ldk;
+    float* dst0 = (is_v ? a.vo : a.ko) + token0 * ld + r * 32 + 4 * i8;
 #pragma unroll
-    for (int n = 0; n < kTokens; ++n) {
+    for (int n = 0; n < TOK; ++n) {
+      const float d = TOK == 8 ? __shfl_sync(0xffffffffu, own_d, n, 8) : own_d;
       if (!in[n]) continue;
-      const uint32_t w = i8 >= 4 ? word[n] >> 4 : word[n];
+      const uint32_t w = (i8 >= 4 ? word[n] >> 4 : word[n]) & 0x0f0f0f0fu;
       float y[4];
 #pragma unroll
-      for (int e = 0; e < 4; ++e) y[e] = __fmul_rn(d[n], (float)(int)((w >> (8 * e)) & 15u) - 8.0f);
-      float* dst = (is_v ? a.vo + (token0 + n) * a.ldv : a.ko + (token0 + n) * a.ldk) + r * 32 + 4 * i8;
+      for (int e = 0; e < 4; ++e) y[e] = __fmul_rn(d, magic_byte(w, e) - 8388616.0f);  // 2^23 + 8
+      float* dst = dst0 + n * ld;
       if constexpr (VEC) {
         *reinterpret_cast<float4*>(dst) = make_float4(y[0], y[1], y[2], y[3]);
       } else {
@@ -874,14 +909,18 @@ int check_cache(const std::string& api, const dqmk_kv_q40* kv, int layer, Plane*
   return DQMK_OK;
 }
 
+template <int NB, int TOK, bool VEC>
+cudaError_t launch_rows(bool write, const RowsArgs& a, cudaStream_t st) {
+  const dim3 grid((unsigned)(((int64_t)a.n_tokens + TOK - 1) / TOK)), block(kRowThreads);
+  return write ? launch(kv_q40_write_kernel<NB, TOK, VEC>, grid, block, 0, st, false, a)
+               : launch(kv_q40_read_kernel<NB, TOK, VEC>, grid, block, 0, st, false, a);
+}
 template <int NB>
 cudaError_t launch_rows(bool write, bool vec, const RowsArgs& a, cudaStream_t st) {
-  const dim3 grid((unsigned)(((int64_t)a.n_tokens + kTokens - 1) / kTokens)), block(kRowThreads);
-  if (write)
-    return vec ? launch(kv_q40_write_kernel<NB, true>, grid, block, 0, st, false, a)
-               : launch(kv_q40_write_kernel<NB, false>, grid, block, 0, st, false, a);
-  return vec ? launch(kv_q40_read_kernel<NB, true>, grid, block, 0, st, false, a)
-             : launch(kv_q40_read_kernel<NB, false>, grid, block, 0, st, false, a);
+  // 8 tokens a CTA once they fill the SMs: below that a token a CTA is sooner done
+  if (a.n_tokens >= 8 * sm_count())
+    return vec ? launch_rows<NB, 8, true>(write, a, st) : launch_rows<NB, 8, false>(write, a, st);
+  return vec ? launch_rows<NB, 1, true>(write, a, st) : launch_rows<NB, 1, false>(write, a, st);
 }
 cudaError_t launch_rows(bool write, bool vec, const RowsArgs& a, cudaStream_t st) {
   switch (a.c.nb) {

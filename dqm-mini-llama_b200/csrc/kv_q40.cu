@@ -91,6 +91,7 @@ __device__ __forceinline__ int64_t token_row(const RowsArgs& a, int token, int h
 // instructions (21 us for 8191 tokens of 4 heads of 128 against a floor of 6).
 // VEC: 16-byte accesses to the f32 rows.
 constexpr int kRowThreads = 256;
+constexpr int kWriteTokens = 8, kReadTokens = 4;
 
 __device__ __forceinline__ int64_t shfl8(int64_t x, int lane) {
   const int lo = __shfl_sync(0xffffffffu, (int)x, lane, 8), hi = __shfl_sync(0xffffffffu, (int)(x >> 32), lane, 8);
@@ -129,7 +130,7 @@ __global__ void __launch_bounds__(kRowThreads) kv_q40_write_kernel(const RowsArg
         for (int e = 0; e < 4; ++e) x[n][e] = n < tokens ? p[e] : 0.0f;
       }
     }
-    const int own = TOK == 8 ? i8 : 0;  // the token this lane works out
+    const int own = i8 % TOK;  // the token this lane works out
     const int64_t own_row = live && own < tokens ? token_row(a, (int)(token0 + own), head) : -1;
 #pragma unroll
     for (int n = 0; n < TOK; ++n) {
@@ -143,15 +144,15 @@ __global__ void __launch_bounds__(kRowThreads) kv_q40_write_kernel(const RowsArg
       const uint16_t d = f2h_ref(__fdiv_rn(own_top, 7.0f));
       const float stored = h2f(d);
       own_inv = stored == 0.0f ? 0.0f : __fdiv_rn(1.0f, stored);
-      if (own_row >= 0 && (TOK == 8 || i8 == 0))
+      if (own_row >= 0 && i8 < TOK)
         *reinterpret_cast<uint16_t*>((is_v ? a.c.v : a.c.k) + scale_at(own_row, b, NB)) = d;
-    } else if (own_row >= 0 && (TOK == 8 || i8 == 0)) {
+    } else if (own_row >= 0 && i8 < TOK) {
       *reinterpret_cast<uint16_t*>((is_v ? a.c.v : a.c.k) + scale_at(own_row, b, NB)) = 0;
     }
 #pragma unroll
     for (int n = 0; n < TOK; ++n) {
-      const float inv = TOK == 8 ? __shfl_sync(0xffffffffu, own_inv, n, 8) : own_inv;
-      const int64_t row = TOK == 8 ? shfl8(own_row, n) : own_row;
+      const float inv = TOK > 1 ? __shfl_sync(0xffffffffu, own_inv, n, 8) : own_inv;
+      const int64_t row = TOK > 1 ? shfl8(own_row, n) : own_row;
       // round(x inv + 8) held to 0 .. 15: with y = x inv + 8 a multiple of 2^-21
       // below 8, y + 1/2 is exact where it could reach the next whole number, so
       // its floor is y rounded with halves up; adding 2^23 rounded down leaves
@@ -188,7 +189,7 @@ __global__ void __launch_bounds__(kRowThreads) kv_q40_read_kernel(const RowsArgs
     const bool live = u == u0 + (int)((threadIdx.x & 31) >> 3), is_v = u >= blocks;
     const int r = is_v ? u - blocks : u, head = r / NB, b = r % NB;
     const unsigned char* base = is_v ? a.c.v : a.c.k;
-    const int own = TOK == 8 ? i8 : 0;
+    const int own = i8 % TOK;
     const int64_t own_row = live && own < tokens ? token_row(a, (int)(token0 + own), head) : -1;
     const float own_d =
         own_row >= 0 ? h2f(*reinterpret_cast<const uint16_t*>(base + scale_at(own_row, b, NB))) : 0.0f;
@@ -196,7 +197,7 @@ __global__ void __launch_bounds__(kRowThreads) kv_q40_read_kernel(const RowsArgs
     bool in[TOK];
 #pragma unroll
     for (int n = 0; n < TOK; ++n) {
-      const int64_t row = TOK == 8 ? shfl8(own_row, n) : own_row;
+      const int64_t row = TOK > 1 ? shfl8(own_row, n) : own_row;
       in[n] = row >= 0;
       word[n] = 0;
       if (!in[n]) continue;
@@ -210,7 +211,7 @@ __global__ void __launch_bounds__(kRowThreads) kv_q40_read_kernel(const RowsArgs
     float* dst0 = (is_v ? a.vo : a.ko) + token0 * ld + r * 32 + 4 * i8;
 #pragma unroll
     for (int n = 0; n < TOK; ++n) {
-      const float d = TOK == 8 ? __shfl_sync(0xffffffffu, own_d, n, 8) : own_d;
+      const float d = TOK > 1 ? __shfl_sync(0xffffffffu, own_d, n, 8) : own_d;
       if (!in[n]) continue;
       const uint32_t w = (i8 >= 4 ? word[n] >> 4 : word[n]) & 0x0f0f0f0fu;
       float y[4];
@@ -911,9 +912,11 @@ int check_cache(const std::string& api, const dqmk_kv_q40* kv, int layer, Plane*
 
 template <int NB, int TOK, bool VEC>
 cudaError_t launch_rows(bool write, const RowsArgs& a, cudaStream_t st) {
-  const dim3 grid((unsigned)(((int64_t)a.n_tokens + TOK - 1) / TOK)), block(kRowThreads);
-  return write ? launch(kv_q40_write_kernel<NB, TOK, VEC>, grid, block, 0, st, false, a)
-               : launch(kv_q40_read_kernel<NB, TOK, VEC>, grid, block, 0, st, false, a);
+  constexpr int RT = TOK > 1 ? kReadTokens : 1, WT = TOK > 1 ? kWriteTokens : 1;
+  const int64_t n = a.n_tokens;
+  const dim3 block(kRowThreads);
+  return write ? launch(kv_q40_write_kernel<NB, WT, VEC>, dim3((unsigned)((n + WT - 1) / WT)), block, 0, st, false, a)
+               : launch(kv_q40_read_kernel<NB, RT, VEC>, dim3((unsigned)((n + RT - 1) / RT)), block, 0, st, false, a);
 }
 template <int NB>
 cudaError_t launch_rows(bool write, bool vec, const RowsArgs& a, cudaStream_t st) {

@@ -249,6 +249,93 @@ def test_attention_prompt_one_key_is_its_value(pkg, cuda, gen):
     assert bool(((out - ref).abs() <= 6 * E * ref.abs()).all())
 
 
+def test_attention_prompt_many_sequences(pkg, cuda, gen):
+    """More sequences than a CTA has threads, most of them short or empty."""
+    torch = cuda
+    h, kv, d = 6, 2, 64
+    r = np.random.RandomState(5)
+    lengths = r.randint(0, 12, 700)
+    lengths[[3, 256, 511, 699]] = [130, 0, 70, 1]
+    starts = np.concatenate([[0], np.cumsum(lengths)]).tolist()
+    n = starts[-1]
+    q, k, v = randn(torch, gen, n, h, d), randn(torch, gen, n, kv, d), randn(torch, gen, n, kv, d)
+    out = pkg.attention_prompt(q, k, v, i32(torch, starts))
+    # one dense masked product over the whole pack
+    seq = torch.searchsorted(i32(torch, starts), torch.arange(n, device="cuda", dtype=torch.int32),
+                             right=True)
+    at = torch.arange(n, device="cuda")
+    seen = (seq[:, None] == seq[None]) & (at[None] <= at[:, None])
+    ks, vs = (x.permute(1, 0, 2).repeat_interleave(h // kv, 0) for x in (k, v))
+    ref, bound = attend(torch, q.permute(1, 0, 2), ks, vs, seen)
+    check_close(out.permute(1, 0, 2), ref, bound)
+
+
+@pytest.mark.parametrize("heads", [(130, 1), (300, 2)])
+def test_attention_prompt_wide_groups(pkg, cuda, gen, heads):
+    """Groups of more heads than an item has rows."""
+    torch = cuda
+    h, kv = heads
+    starts = [0, 3, 75]
+    q, k, v = (randn(torch, gen, 75, x, 32) for x in (h, kv, kv))
+    check_prompt(torch, pkg.attention_prompt(q, k, v, i32(torch, starts)), q, k, v, starts)
+
+
+def test_attention_prompt_not_finite(pkg, cuda, gen):
+    """An infinity or a NaN in a later token's key or value, or in another
+    sequence, leaves a token's output as it is without; a NaN query its row's."""
+    torch = cuda
+    h, kv, d = 4, 2, 64
+    starts = [0, 100, 200]
+    q, k, v = (randn(torch, gen, 200, x, d) for x in (h, kv, kv))
+    want = pkg.attention_prompt(q, k, v, i32(torch, starts))
+    for bad in (float("nan"), float("inf"), -float("inf")):
+        for which in (1, 2):
+            x = [q, k.clone(), v.clone()]
+            x[which][70, 1, 3] = bad
+            out = pkg.attention_prompt(*x, i32(torch, starts))
+            # heads of the other group and tokens before the bad one
+            check_prompt(torch, out[:70], q[:70], k[:70], v[:70], [0, 70], "before")
+            check_prompt(torch, out[:100, :2], q[:100, :2], k[:100, :1], v[:100, :1], [0, 100], "beside")
+            assert torch.equal(out[100:], want[100:])
+            if bad != bad:
+                assert bool(out[70:100, 2:, 3].isnan().all())
+    x = q.clone()
+    x[50, 2] = float("nan")
+    out = pkg.attention_prompt(x, k, v, i32(torch, starts))
+    assert bool(out[50, 2].isnan().all())
+    out[50, 2] = want[50, 2]
+    assert torch.equal(out, want)
+
+
+def test_row_strides_past_32_bits(pkg, cuda, gen):
+    """Rows so far apart that a token's offset needs more than 32 bits."""
+    torch = cuda
+    n, h, kv, d = 70, 2, 1, 64
+    step = 2 ** 31 // 64 + 4  # elements: row 64 starts past 2^31
+    if torch.cuda.mem_get_info()[0] < 40 * 2 ** 30:
+        pytest.skip("needs 28 GB of device memory")
+    flat = [torch.empty(n * step, device="cuda") for _ in range(3)]
+    q, k, v = (f.as_strided((n, x, d), (step, d, 1)) for f, x in zip(flat, (h, kv, kv)))
+    small = [randn(torch, gen, n, x, d) for x in (h, kv, kv)]
+    for a, b in zip((q, k, v), small):
+        a.copy_(b)
+    w = torch.ones(d, device="cuda")
+    pos = torch.arange(n, device="cuda", dtype=torch.int32)
+    starts = i32(torch, [0, n])
+    want = pkg.qk_norm_rope(small[0], small[1], w, w, pos, 1e6, 1e-6)
+    got = pkg.qk_norm_rope(q, k, w, w, pos, 1e6, 1e-6)
+    assert all(torch.equal(a, b) for a, b in zip(got, want))
+    assert torch.equal(pkg.attention_prompt(q, k, v, starts), pkg.attention_prompt(*small, starts))
+    caches = [pkg.KvCacheQ40(1, 1, n, kv, d) for _ in range(2)]
+    zero = torch.zeros_like(pos)
+    caches[0].write(0, k, v, pos, zero)
+    caches[1].write(0, small[1], small[2], pos, zero)
+    assert torch.equal(caches[0].keys, caches[1].keys)
+    assert torch.equal(caches[0].values, caches[1].values)
+    del flat, q, k, v
+    torch.cuda.empty_cache()
+
+
 # ------------------------------------------------------------ 4-bit cache
 def fill(pkg, torch, gen, layers, slots, room, kv, d, layer, scale=1.0, poison=True):
     """A cache with random rows at every position of one layer, every other
@@ -311,6 +398,57 @@ def test_cache_write_is_the_block_format(pkg, cuda, gen, dim, rows):
     assert float(all_k[other].abs().max()) == 0.0 and float(all_v[other].abs().max()) == 0.0
     for x in cache.read(0, every % 20, every // 20):
         assert float(x.abs().max()) == 0.0
+
+
+@pytest.mark.parametrize("dim", [32, 64, 96, 128])
+def test_cache_write_of_many_rows(pkg, cuda, gen, dim):
+    """Enough rows that a CTA takes several tokens, their number not a multiple:
+    the block format bit for bit, infinities and NaN among the values."""
+    torch = cuda
+    n, kv = 1501, 3
+    k, v = randn(torch, gen, n, kv, dim), randn(torch, gen, n, kv, dim)
+    k[5, 1, 3], k[6, 2, 31], v[7, 0, 0] = float("inf"), -float("inf"), float("nan")
+    v[8, 1] = float("nan")
+    k[9:20] *= 1e6  # scales that overflow fp16
+    cache = pkg.KvCacheQ40(1, 3, 501, kv, dim)
+    order = torch.randperm(3 * 501, generator=gen, device="cuda")[:n].to(torch.int32)
+    slots, pos = order % 3, order // 3
+    pos[[0, 700, n - 1]] = -1
+    cache.write(0, k, v, pos, slots)
+    live = pos >= 0
+    for x, y in zip((k, v), cache.read(0, pos, slots)):
+        want = pkg.DequantizeFromQ40(pkg.QuantizeToQ40(x), tuple(x.shape))
+        same = (y == want) | (y.isnan() & want.isnan())
+        assert bool(same[live].all())
+        assert float(y[~live].abs().max()) == 0.0
+
+
+def test_cache_offsets_past_32_bits(pkg, cuda, gen):
+    """A cache whose last layer starts more than 2^32 bytes in."""
+    torch = cuda
+    if torch.cuda.mem_get_info()[0] < 20 * 2 ** 30:
+        pytest.skip("needs 10 GB of device memory")
+    room, kv, d = 1 << 20, 8, 128
+    cache = pkg.KvCacheQ40(4, 2, room, kv, d)
+    assert cache.keys.numel() > 2 ** 32
+    small = pkg.KvCacheQ40(1, 1, 300, kv, d)
+    k, v = randn(torch, gen, 300, kv, d), randn(torch, gen, 300, kv, d)
+    p = torch.arange(300, device="cuda", dtype=torch.int32)
+    cache.write(3, k, v, p, torch.ones_like(p))
+    small.write(0, k, v, p, torch.zeros_like(p))
+    q = randn(torch, gen, 1, 16, d)
+    n, one = i32(torch, [300]), i32(torch, [1])
+    # other cuts of the same work: sums of 300 weighted values in another order
+    want = small.attention(q, 0, n, i32(torch, [0]))
+    got = cache.attention(q, 3, n, one)
+    assert float((got - want).abs().max()) <= 2.0 ** -20 * float(want.abs().max())
+    # positions at the end of the room
+    last = p + (room - 300)
+    cache.write(3, k, v, last, torch.ones_like(p))
+    assert all(torch.equal(a, b) for a, b in zip(cache.read(3, last, torch.ones_like(p)),
+                                                 small.read(0, p, torch.zeros_like(p))))
+    del cache
+    torch.cuda.empty_cache()
 
 
 def test_cache_rows_strides_padding_and_bad_indices(pkg, cuda, gen):
@@ -376,6 +514,40 @@ def test_cache_attention_rooms(pkg, cuda, gen, room):
     out = cache.attention(rows[:, 1:1 + h], 0, i32(torch, lengths), out=wide[:, :h])
     check_decode(torch, out, rows[:, 1:1 + h], ks, vs, lengths, range(n))
     assert bool((wide[:, h] == 3).all())
+
+
+@pytest.mark.parametrize("columns", [128, 129, 300])
+def test_cache_attention_many_columns(pkg, cuda, gen, columns):
+    """More columns than a CTA has threads, a prompt's tokens one by one among
+    them: several columns of a slot with growing lengths."""
+    torch = cuda
+    h, kv, d, room = 14, 2, 64, 700
+    cache, ks, vs = fill(pkg, torch, gen, 1, 5, room, kv, d, 0)
+    r = np.random.RandomState(columns)
+    lengths = r.randint(0, room + 1, columns)
+    lengths[:40] = np.arange(40)
+    lengths[-1] = room
+    slots = r.randint(0, 5, columns)
+    slots[:40] = 2
+    q = randn(torch, gen, columns, h, d)
+    out = cache.attention(q, 0, i32(torch, lengths.tolist()), i32(torch, slots.tolist()))
+    check_decode(torch, out, q, ks, vs, lengths.tolist(), slots.tolist())
+
+
+def test_cache_attention_not_finite(pkg, cuda, gen):
+    """A query with a NaN or an infinity spoils its own head alone."""
+    torch = cuda
+    cache, ks, vs = fill(pkg, torch, gen, 1, 2, 400, 2, 64, 0)
+    q = randn(torch, gen, 2, 14, 64)
+    n = i32(torch, [400, 33])
+    want = cache.attention(q, 0, n)
+    for bad in (float("nan"), float("inf")):
+        x = q.clone()
+        x[0, 4, 9] = bad
+        out = cache.attention(x, 0, n)
+        assert not bool(out[0, 4].isfinite().any())
+        out[0, 4] = want[0, 4]
+        assert torch.equal(out, want)
 
 
 def test_cache_attention_behind_the_length_is_never_read(pkg, cuda, gen):

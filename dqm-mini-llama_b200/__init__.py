@@ -419,6 +419,13 @@ def _vector(api: str, name: str, t, shape, device, dtype):
     _refuse(api, name, t, shape, dtype, device)
 
 
+def _heads(api: str, name: str, t) -> int:
+    try:
+        return t.shape[1]
+    except (AttributeError, IndexError):
+        raise RuntimeError(f"{api}: {name} must be a 3-dimensional CUDA tensor") from None
+
+
 def qk_norm_rope(q, k, q_norm, k_norm, positions, theta: float, eps: float, neox: bool = True,
                  q_out=None, k_out=None, stream=None):
     """RMSNorm of every head of q [tokens, n_heads, head_dim] and k [tokens,
@@ -432,12 +439,12 @@ def qk_norm_rope(q, k, q_norm, k_norm, positions, theta: float, eps: float, neox
     if stream is not None or dev.index != torch._C._cuda_getDevice():
         with _There(dev, stream):
             return qk_norm_rope(q, k, q_norm, k_norm, positions, theta, eps, neox, q_out, k_out)
-    _first(api, "k", k, 3)
-    shape, kshape = q.shape, k.shape
+    shape = q.shape
     n, heads, dim = shape
-    kv = kshape[1]
+    kv = _heads(api, "k", k)
+    kshape = (n, kv, dim)
     ldq = _rows(api, "q", q, shape, dev, f32)
-    ldk = _rows(api, "k", k, (n, kv, dim), dev, f32)
+    ldk = _rows(api, "k", k, kshape, dev, f32)
     _vector(api, "q_norm", q_norm, (dim,), dev, f32)
     _vector(api, "k_norm", k_norm, (dim,), dev, f32)
     _vector(api, "positions", positions, (n,), dev, torch.int32)
@@ -467,10 +474,9 @@ def attention_prompt(q, k, v, starts, out=None, stream=None):
     if stream is not None or dev.index != torch._C._cuda_getDevice():
         with _There(dev, stream):
             return attention_prompt(q, k, v, starts, out)
-    _first(api, "k", k, 3)
     _first(api, "starts", starts, 1)
     n, heads, dim = shape = q.shape
-    kv, seqs = k.shape[1], starts.shape[0] - 1
+    kv, seqs = _heads(api, "k", k), starts.shape[0] - 1
     if seqs < 0:
         raise RuntimeError(f"{api}: starts must hold at least one offset")
     ldq = _rows(api, "q", q, shape, dev, f32)
@@ -512,6 +518,7 @@ class KvCacheQ40:
         self._c = KvQ40(_ptr(self.keys), _ptr(self.values), self.n_layers, self.n_slots,
                         self.max_seq, self.n_kv_heads, self.head_dim)
         self._ref = C.byref(self._c)
+        self._workspace = {}  # (columns, query heads) -> bytes
 
     def write(self, layer: int, k, v, positions, slots=None, stream=None) -> None:
         """Rows k, v [tokens, n_kv_heads, head_dim] to positions [tokens] of
@@ -521,7 +528,7 @@ class KvCacheQ40:
         if stream is not None or dev.index != torch._C._cuda_getDevice():
             with _There(dev, stream):
                 return self.write(layer, k, v, positions, slots)
-        _first(api, "k", k, 3)
+        _heads(api, "k", k)
         n = k.shape[0]
         shape = (n, self.n_kv_heads, self.head_dim)
         ldk = _rows(api, "k", k, shape, dev, torch.float32)
@@ -583,7 +590,10 @@ class KvCacheQ40:
         else:
             ldo = _rows(api, "out", out, shape, dev, f32)
         L = lib()
-        nbytes = L.dqmk_kv_q40_attention_workspace(self._ref, n, heads)
+        nbytes = self._workspace.get((n, heads))
+        if nbytes is None:
+            nbytes = L.dqmk_kv_q40_attention_workspace(self._ref, n, heads)
+            self._workspace[n, heads] = nbytes
         work = torch.empty(nbytes, dtype=torch.uint8, device=dev)
         check(L.dqmk_kv_q40_attention(
             self._ref, layer, q.data_ptr(), ldq, None if slots is None else slots.data_ptr(),

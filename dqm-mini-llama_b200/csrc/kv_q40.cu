@@ -336,18 +336,17 @@ __device__ __forceinline__ void split2(float x0, float x1, __half2& hi, __half2&
   const float2 back = __half22float2(hi);
   lo = __floats2half2_rn(__fsub_rn(x0, back.x), __fsub_rn(x1, back.y));
 }
-__device__ __forceinline__ uint32_t and_or(uint32_t w, uint32_t mask, uint32_t with) {
+template <uint32_t MASK>
+__device__ __forceinline__ uint32_t and_or(uint32_t w, uint32_t with) {
   uint32_t r;
-  asm("lop3.b32 %0, %1, %2, %3, 0xea;" : "=r"(r) : "r"(w), "r"(mask), "r"(with));
+  asm("lop3.b32 %0, %1, %2, %3, 0xea;" : "=r"(r) : "r"(w), "n"(MASK), "r"(with));
   return r;
 }
-// The codes in bits 0-3 and 16-19 of a word as the halves n - 8, and those in
-// bits 4-7 and 20-23 as 16 (n - 8).
 __device__ __forceinline__ uint32_t codes_low(uint32_t w) {
-  return bits(__hadd2(as_h2(and_or(w, 0x000f000fu, 0x64006400u)), as_h2(0xe408e408u)));  // -1032
+  return bits(__hadd2(as_h2(and_or<0x000f000fu>(w, 0x64006400u)), as_h2(0xe408e408u)));  // -1032
 }
 __device__ __forceinline__ uint32_t codes_high(uint32_t w) {
-  return bits(__hadd2(as_h2(and_or(w, 0x00f000f0u, 0x64006400u)), as_h2(0xe480e480u)));  // -1152
+  return bits(__hadd2(as_h2(and_or<0x00f000f0u>(w, 0x64006400u)), as_h2(0xe480e480u)));  // -1152
 }
 __device__ __forceinline__ float pow2f(int e) { return __int_as_float((127 + e) << 23); }
 // V's scales that are all below 2^kSmall are raised by this power of two.

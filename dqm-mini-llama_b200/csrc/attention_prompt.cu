@@ -14,8 +14,8 @@
 // that start at the sequence's first token, become the shared-memory images of
 // the second kernel's operands (K rows, V columns, both terms, 128-byte
 // swizzle), so that a tile is one contiguous bulk copy and needs neither a
-// tensor map nor any alignment of the sequence's first token.  K and V take one
-// power of two a tile.  A tile whose rows differ by more than 2^16 in size, or
+// tensor map nor any alignment of the sequence's first token.  K and V each take
+// one power of two a tile.  A tile whose rows differ by more than 2^16 in size, or
 // that holds an infinity or a NaN, would lose the smaller rows' bits or reach
 // queries that must not see it; it is marked, and the second kernel takes it
 // in f32 straight from the inputs.
@@ -64,9 +64,9 @@ struct PromptArgs {
   int64_t ldo;
   float scale;            // log2(e) / sqrt(D)
   unsigned char* images;  // [tile][kv_head] operand images
-  float4* meta;           // [tile][kv_head]: 2^ek, 2^ev, marked, -
+  float4* meta;           // [tile][kv_head]: 2^ek, K marked, 2^ev, V marked
   struct Item* items;     // row tiles, those with the most keys first
-  int* heads;             // [0]: row tiles listed, [1]: items taken
+  int* heads;             // [0]: row tiles listed, [1]: items taken past each CTA's first
   int max_tiles, max_items;
 };
 
@@ -199,14 +199,18 @@ __global__ void __launch_bounds__(kSplitThreads) prompt_split_kernel(const Promp
   __shared__ int place[3];  // the tile's sequence: first token, tokens, key tiles before it
   __shared__ float vt[kKeys][DP + 1];
   __shared__ int top_bits, low_bits;
-  const int tid = threadIdx.x, kvh = blockIdx.y, D = a.head_dim;
+  const int tid = threadIdx.x, kvh = blockIdx.y >> 1, is_v = blockIdx.y & 1, D = a.head_dim;
   pdl_trigger();
   if (blockIdx.x == 0) {  // first, so that it does not end last
-    if (kvh == 0) list_items(a);
+    if (blockIdx.y == 0) list_items(a);
     return;
   }
   const int64_t tile = (int64_t)blockIdx.x - 1;  // < max_tiles: the grid's size
-  if (tid == 0) place[1] = 0;
+  if (tid == 0) {
+    place[1] = 0;
+    top_bits = 0;
+    low_bits = INT_MAX;
+  }
   int64_t done = 0;
   for (int s0 = 0; s0 < a.n_seqs && done <= tile; s0 += kSplitThreads) {
     const int s = s0 + tid, n = s < a.n_seqs ? seq_len(a, s) : 0;
@@ -223,94 +227,79 @@ __global__ void __launch_bounds__(kSplitThreads) prompt_split_kernel(const Promp
   __syncthreads();
   if (place[1] == 0) return;
   const int k0 = (int)(tile - place[2]) * kKeys, live = min(kKeys, place[1] - k0);
-  const int first = place[0];
-  unsigned char* image = a.images + (tile * a.n_kv_heads + kvh) * C::kImage;
-  float scales[2];
-  bool marked = false;
+  unsigned char* image = a.images + (tile * a.n_kv_heads + kvh) * C::kImage + (is_v ? C::kOperand : 0);
 
   // a thread's float4s of one row sit kSplitThreads / kF4 rows apart
   const int c4 = tid % kF4, r0 = tid / kF4;
-  float4 x[2][kPer];
-#pragma unroll
-  for (int which = 0; which < 2; ++which) {
-    const float* base = (which ? a.v : a.k) + (int64_t)(first + k0) * (which ? a.ldv : a.ldk) +
-                        (int64_t)kvh * D;
-    const int64_t ld = which ? a.ldv : a.ldk;
-#pragma unroll
-    for (int i = 0; i < kPer; ++i) {
-      const int r = r0 + i * (kSplitThreads / kF4);
-      x[which][i] = r < live && 4 * c4 < D ? *reinterpret_cast<const float4*>(base + r * ld + 4 * c4)
-                                           : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-    }
-  }
-#pragma unroll
-  for (int which = 0; which < 2; ++which) {
-    if (tid == 0) {
-      top_bits = 0;
-      low_bits = INT_MAX;
-    }
-    __syncthreads();
-    // sizes compare as integers; an infinity or a NaN is larger than any number
-#pragma unroll
-    for (int i = 0; i < kPer; ++i) {
-      const float4 f = x[which][i];
-      int top = max(max(__float_as_int(fabsf(f.x)), __float_as_int(fabsf(f.y))),
-                    max(__float_as_int(fabsf(f.z)), __float_as_int(fabsf(f.w))));
-#pragma unroll
-      for (int o = 1; o < (kF4 < 32 ? kF4 : 32); o <<= 1)
-        top = max(top, __shfl_xor_sync(0xffffffffu, top, o));
-      if (c4 == 0 && top > 0) {
-        atomicMax(&top_bits, top);
-        atomicMin(&low_bits, top);
-      }
-    }
-    __syncthreads();
-    const int top = top_bits, low = low_bits;
-    if (top >= 0x7f800000 || (top > 0 && (top >> 23) - (low >> 23) > kMostSpread)) marked = true;
-    const int e = pow2_ex(__int_as_float(top));
-    scales[which] = pow2f(e);
-    const float down = pow2f(-e);
-    __syncthreads();
-#pragma unroll
-    for (int i = 0; i < kPer; ++i) {
-      float4& f = x[which][i];
-      f.x *= down, f.y *= down, f.z *= down, f.w *= down;
-    }
-  }
-  if (marked) {  // the products must add nothing
-#pragma unroll
-    for (int i = 0; i < kPer; ++i)
-      x[0][i] = x[1][i] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-  }
+  const int64_t ld = is_v ? a.ldv : a.ldk;
+  const float* base = (is_v ? a.v : a.k) + (int64_t)(place[0] + k0) * ld + (int64_t)kvh * D;
+  float4 x[kPer];
 #pragma unroll
   for (int i = 0; i < kPer; ++i) {
     const int r = r0 + i * (kSplitThreads / kF4);
-    const float4 f = x[0][i];
-    uint2 hi, lo;
-    split2(f.x, f.y, hi.x, lo.x);
-    split2(f.z, f.w, hi.y, lo.y);
-    // columns 64 h ..: plane half h, 8-byte half (c4 & 1) of chunk (c4 % 16) / 2
-    unsigned char* dst = image + (c4 / 16) * (kKeys * 128) + sw128(r, (c4 % 16) >> 1) + (c4 & 1) * 8;
-    *reinterpret_cast<uint2*>(dst) = hi;
-    *reinterpret_cast<uint2*>(dst + C::kPlane) = lo;
-    const float4 g = x[1][i];
-    vt[r][4 * c4] = g.x, vt[r][4 * c4 + 1] = g.y, vt[r][4 * c4 + 2] = g.z, vt[r][4 * c4 + 3] = g.w;
+    x[i] = r < live && 4 * c4 < D ? ldg_f4_stream(base + r * ld + 4 * c4)
+                                  : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+  }
+  // sizes compare as integers; an infinity or a NaN is larger than any number
+#pragma unroll
+  for (int i = 0; i < kPer; ++i) {
+    const float4 f = x[i];
+    int top = max(max(__float_as_int(fabsf(f.x)), __float_as_int(fabsf(f.y))),
+                  max(__float_as_int(fabsf(f.z)), __float_as_int(fabsf(f.w))));
+#pragma unroll
+    for (int o = 1; o < (kF4 < 32 ? kF4 : 32); o <<= 1)
+      top = max(top, __shfl_xor_sync(0xffffffffu, top, o));
+    if (c4 == 0 && top > 0) {
+      atomicMax(&top_bits, top);
+      atomicMin(&low_bits, top);
+    }
   }
   __syncthreads();
-  // V: operand row d holds the 64 keys; a thread writes 16-byte chunks of 8 keys
-  for (int i = tid; i < DP * 8; i += kSplitThreads) {
-    const int d = i / 8, c = i % 8;
-    uint4 hi, lo;
-    split2(vt[8 * c][d], vt[8 * c + 1][d], hi.x, lo.x);
-    split2(vt[8 * c + 2][d], vt[8 * c + 3][d], hi.y, lo.y);
-    split2(vt[8 * c + 4][d], vt[8 * c + 5][d], hi.z, lo.z);
-    split2(vt[8 * c + 6][d], vt[8 * c + 7][d], hi.w, lo.w);
-    unsigned char* dst = image + C::kOperand + sw128(d, c);
-    *reinterpret_cast<uint4*>(dst) = hi;
-    *reinterpret_cast<uint4*>(dst + C::kPlane) = lo;
+  const int top = top_bits, low = low_bits;
+  const bool marked = top >= 0x7f800000 || (top > 0 && (top >> 23) - (low >> 23) > kMostSpread);
+  const int e = pow2_ex(__int_as_float(top));
+  const float down = pow2f(-e);
+#pragma unroll
+  for (int i = 0; i < kPer; ++i) {
+    float4& f = x[i];
+    f.x *= down, f.y *= down, f.z *= down, f.w *= down;
+    if (marked) f = make_float4(0.0f, 0.0f, 0.0f, 0.0f);  // the products must add nothing
+  }
+  if (!is_v) {
+#pragma unroll
+    for (int i = 0; i < kPer; ++i) {
+      const int r = r0 + i * (kSplitThreads / kF4);
+      uint2 hi, lo;
+      split2(x[i].x, x[i].y, hi.x, lo.x);
+      split2(x[i].z, x[i].w, hi.y, lo.y);
+      // columns 64 h ..: plane half h, 8-byte half (c4 & 1) of chunk (c4 % 16) / 2
+      unsigned char* dst = image + (c4 / 16) * (kKeys * 128) + sw128(r, (c4 % 16) >> 1) + (c4 & 1) * 8;
+      *reinterpret_cast<uint2*>(dst) = hi;
+      *reinterpret_cast<uint2*>(dst + C::kPlane) = lo;
+    }
+  } else {
+#pragma unroll
+    for (int i = 0; i < kPer; ++i) {
+      float* to = &vt[r0 + i * (kSplitThreads / kF4)][4 * c4];
+      to[0] = x[i].x, to[1] = x[i].y, to[2] = x[i].z, to[3] = x[i].w;
+    }
+    __syncthreads();
+    // operand row d holds the 64 keys; a thread writes 16-byte chunks of 8 keys
+#pragma unroll
+    for (int i = tid; i < DP * 8; i += kSplitThreads) {
+      const int d = i / 8, c = i % 8;
+      uint4 hi, lo;
+      split2(vt[8 * c][d], vt[8 * c + 1][d], hi.x, lo.x);
+      split2(vt[8 * c + 2][d], vt[8 * c + 3][d], hi.y, lo.y);
+      split2(vt[8 * c + 4][d], vt[8 * c + 5][d], hi.z, lo.z);
+      split2(vt[8 * c + 6][d], vt[8 * c + 7][d], hi.w, lo.w);
+      unsigned char* dst = image + sw128(d, c);
+      *reinterpret_cast<uint4*>(dst) = hi;
+      *reinterpret_cast<uint4*>(dst + C::kPlane) = lo;
+    }
   }
   if (tid == 0)
-    a.meta[tile * a.n_kv_heads + kvh] = make_float4(scales[0], scales[1], marked ? 1.0f : 0.0f, 0.0f);
+    reinterpret_cast<float2*>(a.meta + tile * a.n_kv_heads + kvh)[is_v] = make_float2(pow2f(e), marked ? 1.0f : 0.0f);
 }
 
 // ------------------------------------------------------------ second kernel
@@ -431,9 +420,11 @@ __global__ void __launch_bounds__(Cfg<DP>::kThreads, Cfg<DP>::kCtas) attention_p
     // The next item, posted for the other roles once the item before last's
     // place is free; its queries start towards L2.
     auto post = [&](int w, Work& x) {
-      int id = 0;
-      if (lane == 0) id = atomicAdd(a.heads + 1, 1);
-      id = __shfl_sync(0xffffffffu, id, 0);
+      int id = blockIdx.x;  // the first one; then from the counter
+      if (w > 0) {
+        if (lane == 0) id = gridDim.x + atomicAdd(a.heads + 1, 1);
+        id = __shfl_sync(0xffffffffu, id, 0);
+      }
       x.kvh = -1;
       if (id < total) {
         x.it = a.items[id / a.n_kv_heads];
@@ -693,7 +684,7 @@ __global__ void __launch_bounds__(Cfg<DP>::kThreads, Cfg<DP>::kCtas) attention_p
         uint32_t r[K];
         tmem_ld_n(buf + K * part, r);
         tc::tmem_wait_ld();
-        const bool slow = mt.z != 0.0f;  // the whole CTA's
+        const bool slow = mt.y + mt.w != 0.0f;  // the whole CTA's
         float tmax = -INFINITY;
         if (kt + kKeys - 1 <= cur.first_tok) {  // every key is visible to every row
 #pragma unroll
@@ -733,7 +724,7 @@ __global__ void __launch_bounds__(Cfg<DP>::kThreads, Cfg<DP>::kCtas) attention_p
         tc::bar_arrive(&p_ready[T % NB]);
         if (j > 0) take_output(T - 1);
         corr = slow ? 1.0f : c;
-        vscale = mt.y;
+        vscale = mt.z;
         if (slow && cur.tok >= 0) {
           // the marked tile in f32, key by key, from the inputs; o is at m's scale
           const float* qr = a.q + (int64_t)(cur.first + cur.tok) * a.ldq + (int64_t)cur.head * a.head_dim;
@@ -813,7 +804,7 @@ cudaError_t launch_prompt(const PromptArgs& a, cudaStream_t st) {
                                 cudaFuncAttributeMaxDynamicSharedMemorySize, Cfg<DP>::kSmem);
   });
   if (e != cudaSuccess) return e;
-  e = launch(prompt_split_kernel<DP>, dim3(a.max_tiles + 1, a.n_kv_heads), dim3(kSplitThreads), 0, st,
+  e = launch(prompt_split_kernel<DP>, dim3(a.max_tiles + 1, 2 * a.n_kv_heads), dim3(kSplitThreads), 0, st,
              false, a);
   if (e != cudaSuccess) return e;
   const int64_t items = (int64_t)a.max_items * a.n_kv_heads, most = (int64_t)Cfg<DP>::kCtas * sm_count();
@@ -895,7 +886,7 @@ extern "C" int dqmk_attention_prompt(const float* q, int64_t ldq, const float* k
   a.scale = kLog2e / sqrtf((float)head_dim);
   a.max_tiles = (int)most_tiles(n_tokens, n_seqs);
   const int64_t items = most_items(n_tokens, n_seqs, a.group);
-  if (items * n_kv_heads > INT_MAX / 2 || n_kv_heads > 65535 || (int64_t)n_tokens * a.group > INT_MAX - kRows)
+  if (items * n_kv_heads > INT_MAX / 2 || n_kv_heads > 32767 || (int64_t)n_tokens * a.group > INT_MAX - kRows)
     return fail(DQMK_ERR_UNSUPPORTED, api + ": too many rows");
   a.max_items = (int)items;
   unsigned char* work = static_cast<unsigned char*>(workspace);

@@ -334,9 +334,13 @@ __device__ __forceinline__ bool rows_and(int quarter, bool x) {
       : "memory");
   return r != 0;
 }
-// 32 columns of this warp's 32 rows to registers; 16 from registers.
+// 32 columns of this warp's 32 rows to registers; 8 from registers.
 __device__ __forceinline__ void tmem_ld_n(uint32_t taddr, uint32_t (&r)[32]) { tc::tmem_ld32(taddr, r); }
-__device__ __forceinline__ void tmem_st_n(uint32_t taddr, const uint32_t (&r)[16]) { tc::tmem_st16(taddr, r); }
+__device__ __forceinline__ void tmem_st8(uint32_t taddr, const uint32_t (&r)[8]) {
+  asm volatile("tcgen05.st.sync.aligned.32x32b.x8.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8};" ::"r"(taddr),
+               "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7])
+               : "memory");
+}
 // 16 rows of 8 columns: lane l has columns 2 (l % 4) + {0, 1} of row l / 4 in
 // r[0], r[1] and of row l / 4 + 8 in r[2], r[3].
 __device__ __forceinline__ void tmem_st_rows16(uint32_t taddr, const uint32_t (&r)[4]) {
@@ -705,20 +709,23 @@ __global__ void __launch_bounds__(Cfg<DP>::kThreads, Cfg<DP>::kCtas) attention_p
         const float ref = mnew == -INFINITY ? 0.0f : mnew;
         const float c = ex2(m - ref);
         m = mnew;
-        uint32_t ph[K / 2], pl[K / 2];
-        float sum = 0.0f;
+        const float from = slow ? INFINITY : ref - 14.0f;  // a marked tile's weights are 0 here
+        float sum[2] = {0.0f, 0.0f};
 #pragma unroll
-        for (int i = 0; i < K / 2; ++i) {
-          float p0 = ex2(fmaf(__uint_as_float(r[2 * i]), fs, 14.0f - ref));
-          float p1 = ex2(fmaf(__uint_as_float(r[2 * i + 1]), fs, 14.0f - ref));
-          if (slow) p0 = p1 = 0.0f;
-          sum += p0;
-          sum += p1;
-          split2(p0, p1, ph[i], pl[i]);
+        for (int g = 0; g < K; g += 16) {  // 16 keys at a time: few registers
+          uint32_t ph[8], pl[8];
+#pragma unroll
+          for (int i = 0; i < 8; ++i) {
+            const float p0 = ex2(fmaf(__uint_as_float(r[g + 2 * i]), fs, -from));
+            const float p1 = ex2(fmaf(__uint_as_float(r[g + 2 * i + 1]), fs, -from));
+            sum[0] += p0;
+            sum[1] += p1;
+            split2(p0, p1, ph[i], pl[i]);
+          }
+          tmem_st8(buf + K / 2 * part + g / 2, ph);
+          tmem_st8(buf + 32 + K / 2 * part + g / 2, pl);
         }
-        if (!slow) l = fmaf(l, c, sum);
-        tmem_st_n(buf + K / 2 * part, ph);
-        tmem_st_n(buf + 32 + K / 2 * part, pl);
+        if (!slow) l = fmaf(l, c, sum[0] + sum[1]);
         tc::tmem_wait_st();
         tc::tc_fence_before();
         tc::bar_arrive(&p_ready[T % NB]);

@@ -76,15 +76,15 @@ struct Item {
   int first, n, row, key_tiles;
 };
 
-// DP: head_dim rounded up to 64 or 128.
-template <int DP>
+// DP: head_dim rounded up to 64 or 128.  CTAS: CTAs of the second kernel on an SM,
+// which its registers are shared among.
+template <int DP, int CTAS = 1>
 struct Cfg {
   static constexpr int kPlane = kKeys * DP * 2;     // one term of K or V
   static constexpr int kOperand = 2 * kPlane;       // both terms
   static constexpr int kImage = 2 * kOperand;       // K, then V
   static constexpr int kStages = 2;
   static constexpr int kBufs = DP == 128 ? 3 : 2;   // score buffers
-  static constexpr int kCtas = DP == 128 ? 1 : 2;   // for each SM
   static constexpr int kParts = 2;  // softmax warps on the same rows
   static constexpr int kSoftWarps = 4 * kParts, kThreads = 32 * (kSoftWarps + 2);
   // the stage: a row's outputs, rows 16 bytes apart modulo the 128 of all banks
@@ -363,9 +363,9 @@ struct Work {
 // whole number, more than the roundings move it.
 __device__ __forceinline__ int small_div(int x, float inv) { return (int)(((float)x + 0.5f) * inv); }
 
-template <int DP>
-__global__ void __launch_bounds__(Cfg<DP>::kThreads, Cfg<DP>::kCtas) attention_prompt_kernel(const PromptArgs a) {
-  using C = Cfg<DP>;
+template <int DP, int CTAS>
+__global__ void __launch_bounds__(Cfg<DP, CTAS>::kThreads, CTAS) attention_prompt_kernel(const PromptArgs a) {
+  using C = Cfg<DP, CTAS>;
   constexpr int ST = C::kStages, NB = C::kBufs, kSoftWarps = C::kSoftWarps;
   constexpr int P = C::kParts, kShare = 32 * P;  // threads that share 32 rows
   constexpr int W = DP / P, K = kKeys / P;       // output columns and keys of a thread
@@ -803,20 +803,29 @@ int64_t most_tiles(int n_tokens, int n_seqs) {
   return t < n_tokens ? t : n_tokens;
 }
 
-template <int DP>
-cudaError_t launch_prompt(const PromptArgs& a, cudaStream_t st) {
+template <int DP, int CTAS>
+cudaError_t launch_items(const PromptArgs& a, cudaStream_t st) {
+  using C = Cfg<DP, CTAS>;
   static DeviceOnce once;
-  cudaError_t e = once.run([] {
-    return cudaFuncSetAttribute(attention_prompt_kernel<DP>,
-                                cudaFuncAttributeMaxDynamicSharedMemorySize, Cfg<DP>::kSmem);
+  const cudaError_t e = once.run([] {
+    return cudaFuncSetAttribute(attention_prompt_kernel<DP, CTAS>,
+                                cudaFuncAttributeMaxDynamicSharedMemorySize, C::kSmem);
   });
   if (e != cudaSuccess) return e;
-  e = launch(prompt_split_kernel<DP>, dim3(a.max_tiles + 1, 2 * a.n_kv_heads), dim3(kSplitThreads), 0, st,
-             false, a);
+  const int64_t items = (int64_t)a.max_items * a.n_kv_heads, most = (int64_t)CTAS * sm_count();
+  return launch(attention_prompt_kernel<DP, CTAS>, dim3((unsigned)(items < most ? items : most)),
+                dim3(C::kThreads), C::kSmem, st, use_pdl(), a);
+}
+
+template <int DP>
+cudaError_t launch_prompt(const PromptArgs& a, cudaStream_t st) {
+  const cudaError_t e = launch(prompt_split_kernel<DP>, dim3(a.max_tiles + 1, 2 * a.n_kv_heads),
+                               dim3(kSplitThreads), 0, st, false, a);
   if (e != cudaSuccess) return e;
-  const int64_t items = (int64_t)a.max_items * a.n_kv_heads, most = (int64_t)Cfg<DP>::kCtas * sm_count();
-  return launch(attention_prompt_kernel<DP>, dim3((unsigned)(items < most ? items : most)),
-                dim3(Cfg<DP>::kThreads), Cfg<DP>::kSmem, st, use_pdl(), a);
+  // at 64 two CTAs fit an SM, with fewer registers each: for more items than SMs
+  if constexpr (DP == 64)
+    if ((int64_t)a.max_items * a.n_kv_heads > sm_count()) return launch_items<DP, 2>(a, st);
+  return launch_items<DP, 1>(a, st);
 }
 
 bool prompt_shape_ok(int n_heads, int n_kv_heads, int head_dim) {

@@ -38,8 +38,9 @@
 // next scores while the softmax runs, and the next item's queries go to TMEM
 // while the last O' is computed.  A row a thread would touch 32 lines with each
 // load and store and took 5 us of an item's 9 (measured), as much as 4 key tiles:
-// queries are read 4 lanes a row, outputs go through a shared-memory stage and
-// leave as one copy a row, under the next item's first tiles.
+// queries come and outputs go in whole rows through a shared-memory stage, the
+// queries of the next item under this one's last tiles, the outputs under the
+// next one's first.
 #include <climits>
 
 #include "common.cuh"
@@ -87,7 +88,7 @@ struct Cfg {
   static constexpr int kBufs = DP == 128 ? 3 : 2;   // score buffers
   static constexpr int kParts = 2;  // softmax warps on the same rows
   static constexpr int kSoftWarps = 4 * kParts, kThreads = 32 * (kSoftWarps + 2);
-  // the stage: a row's outputs, rows 16 bytes apart modulo the 128 of all banks
+  // the stage: a row's queries or outputs, rows 16 bytes apart modulo the 128 of all banks
   static constexpr int kRowBytes = DP * 4 + 16;
   static constexpr int kSmem = kStages * kImage + kRows * kRowBytes + 1024;
   static constexpr uint32_t kTmem = DP == 128 ? 512 : 256;
@@ -376,7 +377,7 @@ __global__ void __launch_bounds__(Cfg<DP, CTAS>::kThreads, CTAS) attention_promp
   __shared__ Work work[2];
   __shared__ uint32_t tmem_slot;
   __shared__ volatile int abort_flag;
-  __shared__ float red[2][P][kRows], red_q[2][kRows], red_l[P][kRows];
+  __shared__ float red[2][P][kRows], red_q[kRows], red_l[P][kRows];
   unsigned char* smem = reinterpret_cast<unsigned char*>(
       (reinterpret_cast<uintptr_t>(raw) + 1023) & ~(uintptr_t)1023);
   unsigned char* stage = smem + ST * C::kImage;
@@ -558,70 +559,75 @@ __global__ void __launch_bounds__(Cfg<DP, CTAS>::kThreads, CTAS) attention_promp
       float fq;  // scores in base 2: S' fq 2^ek
       float4 meta;  // of the item's first key tile
     };
-    // Item w's row, and its queries scaled, split and stored to TMEM, once the
-    // last scores of item w - 1 are over; false: no more items.  For the loads to
-    // be coalesced a warp takes 16 rows of its quarter here, 4 lanes a row, and
-    // with four warps to a quarter half of the columns.
-    auto take_item = [&](int w, Rows& x) {
+    // Token (counted from the sequence's) and head of row r of an item.
+    auto place = [&](const Work& k, int r, int& head) {
+      const int i = k.first_head + r, t = small_div(i, inv_group);
+      head = k.kvh * a.group + i - t * a.group;
+      return k.first_tok + t;
+    };
+    // Item w's queries on their way to the stage, once item w - 2's outputs have
+    // left it: a warp takes the 16 rows whose outputs it sent, whole rows a copy
+    // instruction.  false: no more items.
+    auto fetch_item = [&](int w) {
       const bool got = wait(&work_full[w & 1], w >> 1);
+      const Work& k = work[w & 1];
+      if (!rows_and<kShare>(quarter, got && k.kvh >= 0)) return false;
+      asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory");
+      __syncwarp();
+      int head;
+      const int r0 = 32 * quarter + 16 * part, tok = place(k, r0 + (lane & 15), head);
+      const int64_t mine = tok < k.it.n ? (int64_t)(k.it.first + tok) * a.ldq + (int64_t)head * a.head_dim : -1;
+      constexpr int kLanes = DP / 4;  // 16 bytes a lane
+      const int col = 4 * (lane % kLanes);
+#pragma unroll 4
+      for (int i = 0; i < 16; i += 32 / kLanes) {
+        const int r = i + lane / kLanes;
+        const int64_t at = __shfl_sync(0xffffffffu, mine, r);
+        const int bytes = at >= 0 && col < a.head_dim ? 16 : 0;  // zeros where there is nothing
+        asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(
+                         tc::su32(stage + (r0 + r) * C::kRowBytes + 4 * col)),
+                     "l"(a.q + (bytes ? at + col : 0)), "r"(bytes)
+                     : "memory");
+      }
+      return true;
+    };
+    // The fetched item's row, and its queries scaled, split and stored to TMEM,
+    // once the last scores of the item before are over; 4 lanes a row.
+    auto take_item = [&](int w, Rows& x) {
       const Work k = work[w & 1];
       tc::bar_arrive(&work_empty[w & 1]);
-      if (!rows_and<kShare>(quarter, got && k.kvh >= 0)) return false;
       x.meta = __ldcg(a.meta + (int64_t)k.it.key_tiles * a.n_kv_heads + k.kvh);
-      const int rows = k.it.n * a.group - k.it.row;  // rows of the item, if under 128
-      auto token = [&](int r, int& head) {  // of row r: counted from the first token
-        const int i = k.first_head + r, t = small_div(i, inv_group);
-        head = k.kvh * a.group + i - t * a.group;
-        return t;
-      };
       x.first_tok = k.first_tok;
-      x.tok = token(row, x.head) + k.first_tok;
-      if (row >= rows) x.tok = -1;
+      x.tok = place(k, row, x.head);
+      if (x.tok >= k.it.n) x.tok = -1;
       x.first = k.it.first, x.kvh = k.kvh, x.tiles = k.tiles, x.key_tiles = k.it.key_tiles;
 
-      constexpr int kCols = DP * 2 / P;  // columns of a warp
-      const int col0 = (part >> 1) * kCols + 4 * (lane & 3), r0 = 32 * quarter + 16 * (part & 1) + (lane >> 2);
-      const uint32_t at = tmem + ((uint32_t)(32 * quarter + 16 * (part & 1)) << 16) + C::kColQ +
-                          (part >> 1) * (kCols / 2);
-      const float* from[2];
-#pragma unroll
-      for (int i = 0; i < 2; ++i) {
-        int head;
-        const int t = token(r0 + 8 * i, head) + k.first_tok;
-        from[i] = r0 + 8 * i < rows ? a.q + (int64_t)(k.it.first + t) * a.ldq + (int64_t)head * a.head_dim + col0
-                                    : nullptr;
-      }
+      asm volatile("cp.async.wait_all;" ::: "memory");
+      __syncwarp();
+      const int r0 = 32 * quarter + 16 * part + (lane >> 2);
+      const uint32_t at = tmem + ((uint32_t)(32 * quarter + 16 * part) << 16) + C::kColQ;
+      const float4* from[2] = {reinterpret_cast<const float4*>(stage + r0 * C::kRowBytes) + (lane & 3),
+                               reinterpret_cast<const float4*>(stage + (r0 + 8) * C::kRowBytes) + (lane & 3)};
       float top[2];
-      // queries of ordinary size keep all their bits under one scale, 2^7; others
-      // are read a second time, for a scale of their row
+      // queries of ordinary size keep all their bits under one scale, 2^7; with
+      // others among the 32 rows they are split again, under a scale of their row
       constexpr int kUsual = -7;
-      auto unusual = [](float t) { return t > 0.0f && !(t >= 0x1p-10f && t < 256.0f); };
+      auto usual = [](float t) { return !(t > 0.0f) || (t >= 0x1p-10f && t < 256.0f); };
       float up[2] = {pow2f(-kUsual), pow2f(-kUsual)};
       auto pass = [&] {
         top[0] = top[1] = 0.0f;
 #pragma unroll
-        for (int c0 = 0; c0 < kCols / 16; c0 += 4) {
-          float4 v[4][2];  // 8 loads at a time
+        for (int c = 0; c < DP / 16; ++c) {
+          uint32_t hi[4], lo[4];
 #pragma unroll
-          for (int c = 0; c < 4; ++c)
-#pragma unroll
-            for (int i = 0; i < 2; ++i)
-              v[c][i] = from[i] && 16 * (c0 + c) + col0 < a.head_dim
-                            ? __ldg(reinterpret_cast<const float4*>(from[i] + 16 * (c0 + c)))
-                            : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-#pragma unroll
-          for (int c = 0; c < 4; ++c) {
-            uint32_t hi[4], lo[4];
-#pragma unroll
-            for (int i = 0; i < 2; ++i) {
-              const float4 x4 = v[c][i];
-              top[i] = fmaxf(top[i], fmaxf(fmaxf(fabsf(x4.x), fabsf(x4.y)), fmaxf(fabsf(x4.z), fabsf(x4.w))));
-              split2(x4.x * up[i], x4.y * up[i], hi[2 * i], lo[2 * i]);
-              split2(x4.z * up[i], x4.w * up[i], hi[2 * i + 1], lo[2 * i + 1]);
-            }
-            tmem_st_rows16(at + 8 * (c0 + c), hi);
-            tmem_st_rows16(at + DP / 2 + 8 * (c0 + c), lo);
+          for (int i = 0; i < 2; ++i) {
+            const float4 v = from[i][4 * c];
+            top[i] = fmaxf(top[i], fmaxf(fmaxf(fabsf(v.x), fabsf(v.y)), fmaxf(fabsf(v.z), fabsf(v.w))));
+            split2(v.x * up[i], v.y * up[i], hi[2 * i], lo[2 * i]);
+            split2(v.z * up[i], v.w * up[i], hi[2 * i + 1], lo[2 * i + 1]);
           }
+          tmem_st_rows16(at + 8 * c, hi);
+          tmem_st_rows16(at + DP / 2 + 8 * c, lo);
         }
       };
       pass();
@@ -629,25 +635,28 @@ __global__ void __launch_bounds__(Cfg<DP, CTAS>::kThreads, CTAS) attention_promp
       for (int i = 0; i < 2; ++i) {
         top[i] = fmaxf(top[i], __shfl_xor_sync(0xffffffffu, top[i], 1));
         top[i] = fmaxf(top[i], __shfl_xor_sync(0xffffffffu, top[i], 2));
-        if ((lane & 3) == 0) red_q[part >> 1][r0 + 8 * i] = top[i];
+        if ((lane & 3) == 0) red_q[r0 + 8 * i] = top[i];
       }
-      rows_sync<kShare>(quarter);
-      auto row_top = [&](int r) { return P == 4 ? fmaxf(red_q[0][r], red_q[1][r]) : red_q[0][r]; };
-      const float t0 = row_top(r0), t1 = row_top(r0 + 8), mine = row_top(row);
-      if (__any_sync(0xffffffffu, unusual(t0) || unusual(t1))) {
-        if (unusual(t0)) up[0] = pow2f(-pow2_ex(t0));
-        if (unusual(t1)) up[1] = pow2f(-pow2_ex(t1));
+      // behind this barrier the stage's rows of the quarter are free, unless they
+      // are read again
+      const bool all_usual = rows_and<kShare>(quarter, usual(top[0]) && usual(top[1]));
+      const float mine = red_q[row];
+      if (!all_usual) {
+#pragma unroll
+        for (int i = 0; i < 2; ++i)
+          if (!usual(top[i])) up[i] = pow2f(-pow2_ex(top[i]));
         pass();
+        rows_sync<kShare>(quarter);
       }
       tc::tmem_wait_st();
       tc::tc_fence_before();
       tc::bar_arrive(&q_ready);
-      x.fq = a.scale * pow2f(unusual(mine) ? pow2_ex(mine) : kUsual);
-      return true;
+      x.fq = a.scale * pow2f(usual(mine) ? kUsual : pow2_ex(mine));
     };
 
     Rows cur, nxt;
-    bool have = take_item(0, cur);
+    bool have = fetch_item(0);
+    if (have) take_item(0, cur);
     int T = 0;
     for (int w = 0; have; ++w) {
       const int nt = cur.tiles;
@@ -729,6 +738,7 @@ __global__ void __launch_bounds__(Cfg<DP, CTAS>::kThreads, CTAS) attention_promp
         tc::tmem_wait_st();
         tc::tc_fence_before();
         tc::bar_arrive(&p_ready[T % NB]);
+        if (j == max(nt - 2, 0)) have = fetch_item(w + 1);
         if (j > 0) take_output(T - 1);
         corr = slow ? 1.0f : c;
         vscale = mt.z;
@@ -754,11 +764,11 @@ __global__ void __launch_bounds__(Cfg<DP, CTAS>::kThreads, CTAS) attention_promp
           }
         }
       }
-      have = take_item(w + 1, nxt);
+      if (have) take_item(w + 1, nxt);
       take_output(T - 1);
       red_l[part][row] = l;
-      // the last item's outputs have left the stage
-      asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory");
+      // without a next item the last one's outputs may still be in the stage
+      if (!have) asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory");
       rows_sync<kShare>(quarter);
       l = red_l[0][row];
 #pragma unroll

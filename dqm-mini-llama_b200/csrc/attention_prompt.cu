@@ -37,10 +37,16 @@
 // S(j+1) is issued before P(j) is waited for, so the tensor cores work on the
 // next scores while the softmax runs, and the next item's queries go to TMEM
 // while the last O' is computed.  A row a thread would touch 32 lines with each
-// load and store and took 5 us of an item's 9 (measured), as much as 4 key tiles:
-// queries come and outputs go in whole rows through a shared-memory stage, the
+// load and store: queries come and outputs go in whole rows through a shared-memory stage, the
 // queries of the next item under this one's last tiles, the outputs under the
-// next one's first.
+// next one's first (with the list, 396 -> 260 us for 33 ragged prompts of 28 / 4
+// heads of 128; the queries under the last tiles 240 -> 233).
+//
+// Bound: the tensor cores, and an item's ends where it has few keys.  28 / 4 heads
+// of 128 on one B200: 8192 tokens 1072 us, 1346 TFLOP/s of fp16 products (80% of
+// the measured 1686; 1249 us at 1477 MHz in a run of seconds, at the power limit),
+// 33 ragged prompts 230 us; 602 tokens of 14 / 2 heads of 64 20 us.  A score product
+// of 64 keys takes 44.8 cycles, 32 by its operations; one of 128 its full 64.
 #include <climits>
 
 #include "common.cuh"
@@ -54,6 +60,7 @@ __device__ unsigned int g_prompt_error;  // kErrTimeout / kErrBadIndex
 
 constexpr int kMaxDim = 128;
 constexpr int kRows = 128, kKeys = 64;
+constexpr int kMaxGroup = 1 << 20;  // small_div
 constexpr float kLog2e = 1.44269504088896341f;
 
 struct PromptArgs {
@@ -336,7 +343,6 @@ __device__ __forceinline__ bool rows_and(int quarter, bool x) {
   return r != 0;
 }
 // 32 columns of this warp's 32 rows to registers; 8 from registers.
-__device__ __forceinline__ void tmem_ld_n(uint32_t taddr, uint32_t (&r)[32]) { tc::tmem_ld32(taddr, r); }
 __device__ __forceinline__ void tmem_st8(uint32_t taddr, const uint32_t (&r)[8]) {
   asm volatile("tcgen05.st.sync.aligned.32x32b.x8.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8};" ::"r"(taddr),
                "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7])
@@ -695,7 +701,7 @@ __global__ void __launch_bounds__(Cfg<DP, CTAS>::kThreads, CTAS) attention_promp
         wait(&s_done[T % NB], T / NB);
         tc::tc_fence_after();
         uint32_t r[K];
-        tmem_ld_n(buf + K * part, r);
+        tc::tmem_ld32(buf + K * part, r);
         tc::tmem_wait_ld();
         const bool slow = mt.y + mt.w != 0.0f;  // the whole CTA's
         float tmax = -INFINITY;
@@ -890,6 +896,8 @@ extern "C" int dqmk_attention_prompt(const float* q, int64_t ldq, const float* k
     return fail(DQMK_ERR_INVALID, api + ": invalid head configuration");
   if (head_dim % 4 != 0 || head_dim > kMaxDim)
     return fail(DQMK_ERR_UNSUPPORTED, api + ": head_dim must be a multiple of 4 of at most 128");
+  if (n_heads / n_kv_heads > kMaxGroup)
+    return fail(DQMK_ERR_UNSUPPORTED, api + ": too many query heads for a key/value head");
   const int64_t wq = (int64_t)n_heads * head_dim, wk = (int64_t)n_kv_heads * head_dim;
   if (ldq < wq || ldo < wq || ldk < wk || ldv < wk)
     return fail(DQMK_ERR_INVALID, api + ": row stride shorter than the row");

@@ -322,7 +322,8 @@ int dqmk_qk_norm_rope(const float* q_dev, int64_t ldq, const float* k_dev, int64
  * were.  A sequence whose offsets are out of order or outside 0..n_tokens is
  * skipped and recorded (dqmk_device_error bit 3).  Results are within f32
  * summation order of f32 arithmetic, and the same for the same arguments every
- * time.  head_dim: a multiple of 4, at most 128; pointers 16-byte aligned,
+ * time.  head_dim: a multiple of 4, at most 128; at most 2^20 query heads to a
+ * key/value head; pointers 16-byte aligned,
  * strides multiples of 4.  workspace_dev: dqmk_attention_prompt_workspace
  * bytes, contents ignored; calls that may overlap on the GPU need one each. */
 size_t dqmk_attention_prompt_workspace(int n_tokens, int n_seqs, int n_heads, int n_kv_heads,

@@ -175,3 +175,9 @@ def test_python_wrappers_refuse_host_tensors(pkg):
         pkg.attention_prompt(x, x, x, i)
     with pytest.raises(RuntimeError, match="KvCacheQ40: unsupported shape"):
         pkg.KvCacheQ40(1, 1, 8, 1, 48)
+
+
+def test_attention_prompt_heads_that_share_keys(pkg):
+    heads = (1 << 20) + 1
+    refused(pkg, prompt(pkg, n=1, seqs=1, h=heads, kv=1, d=4, ldq=4 * heads, ldo=4 * heads,
+                        size=1 << 40), "too many query heads")

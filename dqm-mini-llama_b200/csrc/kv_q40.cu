@@ -252,14 +252,18 @@ __global__ void __launch_bounds__(kRowThreads) kv_q40_read_kernel(const RowsArgs
 // A code becomes a half by one AND/OR, (w & 0x000f) | 0x6400 = 1024 + n, and
 // one addition that centres it: n - 8 (16 (n - 8) from a high nibble; for a key
 // its channel of q takes 1/16).  The code's own bits are n 2^-24 as a subnormal
-// half and would need neither, but the products align their sums by the
-// operands' exponent fields, and 10 bits of every sum are lost.  For the same
-// reason (the accumulators round towards zero) a tile's products start from
-// zero and are added to the running sums in f32.
+// half and would need neither, but results were then off by 2.4e-6 (3e-7 with
+// centred codes).  Long chains in the accumulators cost bits as well (1.4e-6 over
+// 65536 positions): a tile's products start from zero and are added in f32.
 //
 // Bound: 18 bytes for 32 values, each used by every head of the group; at the
-// memory rate an SM has about 1.4 instruction slots a value, and the unpacking,
-// scaling and splitting above take most of them.
+// memory rate a scheduler has 3.1 lane slots a value of the cache, 1.5 for half2
+// and integer instructions, which issue at half rate, and f32 arithmetic adds its
+// time to the products'.  So it is bound by its instructions: 168 us for 16 columns
+// of 65536 positions, 28 / 4 heads of 128 (3.6 TB/s, 56% of the measured copy rate;
+// 180 us at 1860 MHz in a run of seconds, at the power limit); 64 ragged columns up
+// to 2048 22 us, 1 x 32768 14.5 us.  3 CTAs an SM with 168 registers: 4 with 128 took
+// 184 us for 168.
 //
 // Work: the positions of all columns and heads form one list of units, kExtra
 // for each (column, group), what its start and end cost, and one for each of

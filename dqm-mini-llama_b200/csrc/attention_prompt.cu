@@ -912,6 +912,8 @@ extern "C" int dqmk_attention_prompt(const float* q, int64_t ldq, const float* k
   if (workspace_bytes < need)
     return fail(DQMK_ERR_INVALID, api + ": workspace of " + std::to_string(workspace_bytes) +
                                       " bytes, needs " + std::to_string(need));
+  if (out == q || out == k || out == v)
+    return fail(DQMK_ERR_INVALID, api + ": out must not be an input");
   PromptArgs a = {};
   a.q = q, a.k = k, a.v = v, a.ldq = ldq, a.ldk = ldk, a.ldv = ldv;
   a.starts = starts, a.n_seqs = n_seqs, a.n_tokens = n_tokens;

@@ -181,3 +181,9 @@ def test_attention_prompt_heads_that_share_keys(pkg):
     heads = (1 << 20) + 1
     refused(pkg, prompt(pkg, n=1, seqs=1, h=heads, kv=1, d=4, ldq=4 * heads, ldo=4 * heads,
                         size=1 << 40), "too many query heads")
+
+
+def test_attention_prompt_output_is_no_input(pkg):
+    for name in "qkv":
+        inputs = {x: P if x == name else C.c_void_p(8192) for x in "qkv"}
+        refused(pkg, prompt(pkg, **inputs), "out must not be an input")

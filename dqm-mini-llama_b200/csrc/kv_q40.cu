@@ -893,6 +893,13 @@ bool shape_ok(int n_layers, int n_slots, int max_seq, int n_kv_heads, int head_d
          head_dim > 0 && head_dim % 32 == 0 && head_dim <= 32 * kMaxBlocks;
 }
 
+// A buffer's bytes fit 62 bits, so that no offset wraps.
+bool size_ok(int n_layers, int n_slots, int max_seq, int n_kv_heads, int head_dim) {
+  const unsigned __int128 tiles = (unsigned __int128)((uint64_t)n_layers * (uint64_t)n_slots) *
+                                  (uint64_t)n_kv_heads * (uint64_t)tiles_of(max_seq);
+  return tiles < ((uint64_t)1 << 62) / tile_bytes(head_dim / 32);
+}
+
 // The status of a cache argument; on success its layer `layer`.
 int check_cache(const std::string& api, const dqmk_kv_q40* kv, int layer, Plane* out) {
   if (!kv || !kv->keys_dev || !kv->values_dev) return fail(DQMK_ERR_INVALID, api + ": null pointer");
@@ -900,6 +907,8 @@ int check_cache(const std::string& api, const dqmk_kv_q40* kv, int layer, Plane*
     return fail(DQMK_ERR_INVALID, api + ": invalid cache shape");
   if (!shape_ok(kv->n_layers, kv->n_slots, kv->max_seq, kv->n_kv_heads, kv->head_dim))
     return fail(DQMK_ERR_UNSUPPORTED, api + ": head_dim must be a multiple of 32 of at most 128");
+  if (!size_ok(kv->n_layers, kv->n_slots, kv->max_seq, kv->n_kv_heads, kv->head_dim))
+    return fail(DQMK_ERR_UNSUPPORTED, api + ": cache too large");
   if ((reinterpret_cast<uintptr_t>(kv->keys_dev) | reinterpret_cast<uintptr_t>(kv->values_dev)) & 15u)
     return fail(DQMK_ERR_INVALID, api + ": KV cache must be 16-byte aligned");
   if (layer < 0 || layer >= kv->n_layers) return fail(DQMK_ERR_RANGE, api + ": layer out of range");
@@ -970,7 +979,9 @@ using namespace dqmk;
 
 extern "C" size_t dqmk_kv_q40_bytes(int n_layers, int n_slots, int max_seq, int n_kv_heads,
                                     int head_dim) {
-  if (!shape_ok(n_layers, n_slots, max_seq, n_kv_heads, head_dim)) return 0;
+  if (!shape_ok(n_layers, n_slots, max_seq, n_kv_heads, head_dim) ||
+      !size_ok(n_layers, n_slots, max_seq, n_kv_heads, head_dim))
+    return 0;
   return (size_t)n_layers * n_slots * n_kv_heads * tiles_of(max_seq) * tile_bytes(head_dim / 32);
 }
 

@@ -187,3 +187,12 @@ def test_attention_prompt_output_is_no_input(pkg):
     for name in "qkv":
         inputs = {x: P if x == name else C.c_void_p(8192) for x in "qkv"}
         refused(pkg, prompt(pkg, **inputs), "out must not be an input")
+
+
+def test_kv_q40_bytes_past_64_bits(pkg):
+    big, odd = 1 << 30, (1 << 30) + 1  # the product keeps low bits when it wraps
+    assert pkg.lib().dqmk_kv_q40_bytes(odd, odd, odd, 1, 32) == 0
+    kv = cache(pkg, layers=odd, slots=odd, seq=odd, kv=1, dim=32)
+    for call in (write, read, decode):
+        refused(pkg, call(pkg, kv), "too large")
+    assert pkg.lib().dqmk_kv_q40_bytes(1, 1, big, 1, 32) == 18 * big

@@ -334,28 +334,6 @@ def CudaAttentionDecodeDeviceInput(q, kv: CudaKvCache, layer: int, pos: int, n_h
 
 # ------------------------------------------------------------ attention block
 class _There:
-    """A call on another device or a given stream: both are made current, so
-    that outputs and workspaces are allocated for the stream that uses them."""
-
-    def __init__(self, device, stream):
-        torch = _torch()
-        if stream is not None and not isinstance(stream, torch.cuda.Stream):
-            stream = torch.cuda.ExternalStream(stream, device=device)
-        if stream is not None and stream.device != device:
-            raise RuntimeError("stream and tensors are on different devices")
-        self.guards = (torch.cuda.device(device), torch.cuda.stream(stream))
-
-    def __enter__(self):
-        for g in self.guards:
-            g.__enter__()
-        return _torch().cuda.current_stream().cuda_stream
-
-    def __exit__(self, *exc):
-        for g in reversed(self.guards):
-            g.__exit__(*exc)
-
-
-class _There:
     """Another device or a given stream made current for a call, so that its
     outputs and workspace are allocated for the stream that uses them."""
 
@@ -467,7 +445,8 @@ def attention_prompt(q, k, v, starts, out=None, stream=None):
     """Causal attention over packed prompts: q [tokens, n_heads, head_dim], k
     and v [tokens, n_kv_heads, head_dim], starts int32 [sequences + 1] on the
     device, sequence s = tokens starts[s] .. starts[s+1]-1.  Rows of `out`
-    outside every sequence are left as they were (a new `out` is zero there)."""
+    outside every sequence are left as they were (a new `out` is zero there);
+    `out` must not overlap the inputs."""
     torch = _torch()
     api, f32 = "AttentionPrompt", torch.float32
     dev = _first(api, "q", q, 3)
@@ -571,8 +550,8 @@ class KvCacheQ40:
     def attention(self, q, layer: int, lengths, slots=None, out=None, stream=None):
         """Decode attention: q [columns, n_heads, head_dim], column c over the
         first lengths[c] positions of slots[c] (None: slot c); int32 tensors on
-        the device.  Length 0 gives zeros.  Returns out [columns, n_heads,
-        head_dim]."""
+        the device.  Length 0 gives zeros.  out may be q.  Returns out
+        [columns, n_heads, head_dim]."""
         torch = _torch()
         api, dev, i32, f32 = "KvQ40Attention", self.device, torch.int32, torch.float32
         if stream is not None or dev.index != torch._C._cuda_getDevice():

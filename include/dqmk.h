@@ -323,9 +323,9 @@ int dqmk_qk_norm_rope(const float* q_dev, int64_t ldq, const float* k_dev, int64
  * skipped and recorded (dqmk_device_error bit 3).  Results are within f32
  * summation order of f32 arithmetic, and the same for the same arguments every
  * time.  head_dim: a multiple of 4, at most 128; at most 2^20 query heads to a
- * key/value head; pointers 16-byte aligned,
- * strides multiples of 4.  workspace_dev: dqmk_attention_prompt_workspace
- * bytes, contents ignored; calls that may overlap on the GPU need one each. */
+ * key/value head; pointers 16-byte aligned, strides multiples of 4.
+ * workspace_dev: dqmk_attention_prompt_workspace bytes, contents ignored; calls
+ * that may overlap on the GPU need one each. */
 size_t dqmk_attention_prompt_workspace(int n_tokens, int n_seqs, int n_heads, int n_kv_heads,
                                        int head_dim);
 int dqmk_attention_prompt(const float* q_dev, int64_t ldq, const float* k_dev, int64_t ldk,
@@ -335,7 +335,7 @@ int dqmk_attention_prompt(const float* q_dev, int64_t ldq, const float* k_dev, i
 
 /* A KV cache held as Q4_0 blocks: n_slots independent sequences of up to
  * max_seq positions for each of n_layers layers.  keys_dev and values_dev are
- * device buffers of dqmk_kv_q40_bytes each (16-byte aligned, contents opaque;
+ * device buffers of dqmk_kv_q40_bytes each (below 2^62; 16-byte aligned, contents opaque;
  * they need no initialisation: only written positions are read).  head_dim: a
  * multiple of 32, at most 128. */
 typedef struct dqmk_kv_q40 {
@@ -353,8 +353,8 @@ size_t dqmk_kv_q40_bytes(int n_layers, int n_slots, int max_seq, int n_kv_heads,
  * slot slots_dev[t] (slots_dev NULL: slot t) of layer `layer`.  A token with
  * position -1 is padding and stores nothing.  A slot or position outside the
  * cache stores nothing and is recorded (dqmk_device_error bit 3).  A (slot,
- * position) pair at most once in a call: of two rows it is not said which
- * blocks stay. */
+ * position) pair at most once in a call: what two rows leave there is not said
+ * (bytes of both may be mixed). */
 int dqmk_kv_q40_write(const dqmk_kv_q40* kv, int layer, const float* k_dev, int64_t ldk,
                       const float* v_dev, int64_t ldv, const int* slots_dev,
                       const int* positions_dev, int n_tokens, void* stream);
@@ -371,8 +371,9 @@ int dqmk_kv_q40_read(const dqmk_kv_q40* kv, int layer, const int* slots_dev,
  * out_dev at element c * ldo.  Query heads h use KV head h / (n_heads /
  * n_kv_heads).  Several columns may name one slot (a prompt's tokens with
  * growing lengths, once their rows are written).  Length 0 gives a row of
- * zeros, whatever its slot; so do a length outside 0..max_seq and a slot outside the cache, which
- * are recorded (dqmk_device_error bit 3).  Results are those of f32 arithmetic
+ * zeros, whatever its slot; so do a length outside 0..max_seq and a slot
+ * outside the cache, which are recorded (dqmk_device_error bit 3).  out_dev may
+ * be q_dev with the same stride; other overlap is not allowed.  Results are those of f32 arithmetic
  * on the cache's values (within f32 summation order), and the same for the
  * same arguments every time.  workspace_dev: dqmk_kv_q40_attention_workspace
  * bytes, 16-byte aligned, contents ignored; calls that may overlap on the GPU

@@ -706,3 +706,17 @@ def test_attention_block_serves_prompts_and_decodes(pkg, cuda, gen, heads):
         ks, vs = (x.view(3, 200, kv, d) for x in cache.read(1, every % 200, every // 200))
         check_decode(torch, out, qr, ks, vs, seen, range(3), f"step {step}")
     assert pkg.lib().dqmk_device_error(1) == 0
+
+
+@pytest.mark.parametrize("columns", [1, 70])
+def test_cache_attention_in_place(pkg, cuda, gen, columns):
+    """Output over the queries: groups of one CTA and of several, zero rows."""
+    torch = cuda
+    h, kv, d, room = 20, 2, 64, 3000
+    cache, _, _ = fill(pkg, torch, gen, 1, 3, room, kv, d, 0)
+    lengths = [room] if columns == 1 else [(c * 677) % (room + 1) for c in range(columns)]
+    q = randn(torch, gen, columns, h, d)
+    args = (0, i32(torch, lengths), i32(torch, [c % 3 for c in range(columns)]))
+    want = cache.attention(q, *args)
+    assert cache.attention(q, *args, out=q) is q
+    assert torch.equal(q, want)

@@ -838,9 +838,14 @@ cudaError_t launch_prompt(const PromptArgs& a, cudaStream_t st) {
   const cudaError_t e = launch(prompt_split_kernel<DP>, dim3(a.max_tiles + 1, 2 * a.n_kv_heads),
                                dim3(kSplitThreads), 0, st, false, a);
   if (e != cudaSuccess) return e;
-  // at 64 two CTAs fit an SM, with fewer registers each: for more items than SMs
+  // At 64 two CTAs fit an SM, with 96 registers each for 168.  Two hide an item's
+  // ends, one is faster while a CTA has few items, the longest of which ends last.
+  // One / two, us, items an SM: 1 x 4096 tokens of 14 / 2 heads 120 / 145 (3.0),
+  // 1 x 8192 of 8 / 8 257 / 301 (3.5); 1 x 8192 of 14 / 2 401 / 390 (6), 37 x 1024
+  // 316 / 292 (28), 148 x 64 of 8 / 8 58 / 53 (12); short prompts lose by one also
+  // with few items (148 x 16 of 14 / 2 28.0 / 26.4).
   if constexpr (DP == 64)
-    if ((int64_t)a.max_items * a.n_kv_heads > sm_count()) return launch_items<DP, 2>(a, st);
+    if ((int64_t)a.max_items * a.n_kv_heads > 4 * sm_count()) return launch_items<DP, 2>(a, st);
   return launch_items<DP, 1>(a, st);
 }
 

@@ -720,3 +720,23 @@ def test_cache_attention_in_place(pkg, cuda, gen, columns):
     want = cache.attention(q, *args)
     assert cache.attention(q, *args, out=q) is q
     assert torch.equal(q, want)
+
+
+@pytest.mark.parametrize("heads", [(14, 2, 64), (12, 3, 36), (40, 8, 32)], ids=lambda h: "h%d_kv%d_d%d" % h)
+def test_attention_prompt_full_machine(pkg, cuda, gen, heads):
+    """More items than the SMs take at once, several key tiles each, a sequence
+    whose rows differ by 2^20 and, in another, sizes of 2^20 throughout; twice."""
+    torch = cuda
+    h, kv, d = heads
+    lengths = [600] * 8 + [1, 0, 130, 64, 65] * 60
+    starts = np.concatenate([[0], np.cumsum(lengths)]).tolist()
+    n = starts[-1]
+    q, k, v = (randn(torch, gen, n, x, d) for x in (h, kv, kv))
+    v[:600] *= torch.exp2(torch.randint(-10, 11, (600, 1, 1), generator=gen, device="cuda").float())
+    v[600:1200] *= 2.0 ** 20
+    out = pkg.attention_prompt(q, k, v, i32(torch, starts))
+    for a, b in zip(starts[:40], starts[1:41]):
+        check_prompt(torch, out[a:b], q[a:b], k[a:b], v[a:b], [0, b - a], f"from {a}")
+    check_prompt(torch, out[starts[-6]:], *(x[starts[-6]:] for x in (q, k, v)),
+                 [s - starts[-6] for s in starts[-6:]])
+    assert torch.equal(out, pkg.attention_prompt(q, k, v, i32(torch, starts)))

@@ -105,6 +105,8 @@ SIGNATURES = {
     "dqmk_kv_q40_attention_workspace": ([_kvp, _i, _i], _sz),
     "dqmk_kv_q40_attention": ([_kvp, _i, _vp, _i64, _vp, _vp, _i, _i, _vp, _i64, _vp, _sz, _vp],
                               _i),
+    "dqmk_kv_q40_attention_withhold_tile": ([_kvp, _i, _vp, _i64, _vp, _vp, _i, _i, _vp, _i64, _vp,
+                                             _sz, _i, _i, _vp], _i),
     "dqmk_model_create": ([C.POINTER(ModelConfig), _i, C.POINTER(_vp)], _i),
     "dqmk_model_destroy": ([_vp], _i),
     "dqmk_model_upload": ([_vp, C.c_char_p, _i, _vp, _sz, _i, _i], _i),

@@ -286,6 +286,8 @@ struct AttnQ40Args {
   float scale;                       // log2(e) / sqrt(D)
   float* part;                       // [CTA][2][part_floats]
   int2* spans;                       // [column][sub]: first and last CTA
+  int n_ctas;                        // of the attention kernel: the partial sums there are
+  int withhold_col, withhold_tile;   // test hook: copies that are never made (-1: none)
 };
 
 template <int NB>
@@ -488,7 +490,9 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) kv_q40_attention_kernel(
   auto issue = [&](const Piece& x, int i) {  // lane 0: this warp's tile i of the piece
     unsigned char* st = ring + (issued % kStages) * S::kStageBytes;
     uint64_t* bar = &bars[warp][issued % kStages];
-    const int64_t at = (first_tile(a.c, x.slot, x.sub % a.c.n_kv_heads) + first_of(x) + i * kWarps) * S::kTileBytes;
+    const int tile = first_of(x) + i * kWarps;
+    if (x.col == a.withhold_col && tile == a.withhold_tile) return;
+    const int64_t at = (first_tile(a.c, x.slot, x.sub % a.c.n_kv_heads) + tile) * S::kTileBytes;
     tc::bar_expect_tx(bar, S::kStageBytes);
     bulk_load(st, a.c.k + at, S::kTileBytes, bar);
     bulk_load(st + S::kTileBytes, a.c.v + at, S::kTileBytes, bar);
@@ -511,6 +515,22 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) kv_q40_attention_kernel(
         qx[i][b] = h0 + hh < a.group ? a.q[x.col * a.ldq + head * D + 32 * b + lane] : 0.0f;
       }
   };
+  // the piece behind x: it begins a group, of this column or of the next with
+  // any units; no chunks of it where the run ends
+  auto next_piece = [&](const Piece& x, Piece& nx) {
+    nx = x;
+    nx.take = 0;
+    if (u >= u1) return u;
+    if (++nx.sub == a.subs) {
+      nx.sub = 0;
+      do {
+        ++nx.col;
+        nx.slot = slot_of(a, nx.col);
+        nx.len = visible(a, a.lengths[nx.col], nx.slot);
+      } while (nx.len == 0);
+    }
+    return u + cut(nx, 0, u);
+  };
   start(p);
   load_q(p);
 
@@ -518,21 +538,8 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) kv_q40_attention_kernel(
     const int kvh = p.sub % a.c.n_kv_heads, h0 = (p.sub / a.c.n_kv_heads) * kGroup;
     const int n_here = min(kGroup, a.group - h0);  // heads of this group
     const int mine = tiles_mine(p), tile0 = first_of(p), len = p.len;
-    // the next piece begins a group: of this column, or of the next with any
-    Piece nx = p;
-    int64_t behind = u;
-    nx.take = 0;
-    if (u < u1) {
-      if (++nx.sub == a.subs) {
-        nx.sub = 0;
-        do {
-          ++nx.col;
-          nx.slot = slot_of(a, nx.col);
-          nx.len = visible(a, a.lengths[nx.col], nx.slot);
-        } while (nx.len == 0);
-      }
-      behind += cut(nx, 0, u);
-    }
+    Piece nx;
+    const int64_t behind = next_piece(p, nx);
     const bool more = nx.take > 0;
 
     // ---- the group's queries as A operands (high and low terms), two heads a warp
@@ -778,7 +785,24 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) kv_q40_attention_kernel(
     u = behind;
     p = nx;
   }
-  if (!ok) {  // a wait ran out: leave once this warp's own copies have landed or given up
+  if (!ok) {
+    // A wait ran out.  Of the groups that this run leaves unfinished, the join
+    // skips those that start here; the others' sums of this run become NaN, so
+    // that nothing the workspace held before enters a result.
+    for (bool more = true; more;) {
+      if (p.ch0 == 0) {
+        if (tid == 0) a.spans[(int64_t)p.col * a.subs + p.sub] = make_int2(-1, -1);
+      } else if (tid < kGroup) {
+        float* part = a.part + (int64_t)blockIdx.x * 2 * S::kPartFloats + kGroup * D;
+        part[tid] = 0.0f;
+        part[kGroup + tid] = __int_as_float(0x7fc00000);
+      }
+      Piece nx;
+      u = next_piece(p, nx);
+      more = nx.take > 0;
+      p = nx;
+    }
+    // leave once this warp's own copies have landed or given up
     for (; used < issued; ++used) {
       const unsigned long long t0 = tc::now_ns();
       while (!tc::bar_try(&bars[warp][used % kStages], (used / kStages) & 1))
@@ -804,8 +828,10 @@ __global__ void __launch_bounds__(HEADS == 1 ? 1024 : 512) kv_q40_join_kernel(co
   const int len = visible(a, a.lengths[col], slot_of(a, col));
   pdl_wait();  // every CTA waits, so that this grid's end is also the first kernel's
   if (chunks_of(len) == 0) return;
+  // whole in one CTA, or unfinished (the partial sums' indices are checked
+  // against the workspace whatever it holds)
   const int2 span = __ldcg(a.spans + blockIdx.x);
-  if (span.x == span.y) return;
+  if (span.x < 0 || span.x >= span.y || span.y >= a.n_ctas) return;
   const int h = blockIdx.y * HEADS + warp % HEADS, slot = warp / HEADS;
   float m = -INFINITY, l = 0.0f, acc[NB];
 #pragma unroll
@@ -1028,11 +1054,13 @@ extern "C" size_t dqmk_kv_q40_attention_workspace(const dqmk_kv_q40* kv, int n_c
   return workspace_need(n_cols, subs, kv->max_seq, kv->head_dim);
 }
 
-extern "C" int dqmk_kv_q40_attention(const dqmk_kv_q40* kv, int layer, const float* q, int64_t ldq,
-                                     const int* slots, const int* lengths, int n_cols, int n_heads,
-                                     float* out, int64_t ldo, void* workspace,
-                                     size_t workspace_bytes, void* stream) {
-  const std::string api = "KvQ40Attention";
+namespace {
+
+int attention_call(const char* name, const dqmk_kv_q40* kv, int layer, const float* q, int64_t ldq,
+                   const int* slots, const int* lengths, int n_cols, int n_heads, float* out,
+                   int64_t ldo, void* workspace, size_t workspace_bytes, int withhold_col,
+                   int withhold_tile, void* stream) {
+  const std::string api = name;
   AttnQ40Args a = {};
   int rc = check_cache(api, kv, layer, &a.c);
   if (rc) return rc;
@@ -1057,10 +1085,11 @@ extern "C" int dqmk_kv_q40_attention(const dqmk_kv_q40* kv, int layer, const flo
   a.q = q, a.ldq = ldq, a.out = out, a.ldo = ldo;
   a.lengths = lengths, a.slots = slots, a.n_cols = n_cols, a.n_heads = n_heads;
   a.scale = kLog2e / sqrtf((float)kv->head_dim);
+  a.withhold_col = withhold_col, a.withhold_tile = withhold_tile;
   a.part = static_cast<float*>(workspace);
   a.spans = reinterpret_cast<int2*>(static_cast<char*>(workspace) +
                                     part_bytes(n_cols, a.subs, kv->max_seq, kv->head_dim));
-  const int n_ctas = attention_ctas(n_cols, a.subs, kv->max_seq);
+  const int n_ctas = a.n_ctas = attention_ctas(n_cols, a.subs, kv->max_seq);
   const bool join = kv->max_seq > kChunk;  // else every run ends with a whole group
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   cudaError_t e;
@@ -1072,4 +1101,23 @@ extern "C" int dqmk_kv_q40_attention(const dqmk_kv_q40* kv, int layer, const flo
   }
   DQMK_CUDA_RET(api.c_str(), e);
   return DQMK_OK;
+}
+
+}  // namespace
+
+extern "C" int dqmk_kv_q40_attention(const dqmk_kv_q40* kv, int layer, const float* q, int64_t ldq,
+                                     const int* slots, const int* lengths, int n_cols, int n_heads,
+                                     float* out, int64_t ldo, void* workspace,
+                                     size_t workspace_bytes, void* stream) {
+  return attention_call("KvQ40Attention", kv, layer, q, ldq, slots, lengths, n_cols, n_heads, out, ldo,
+                        workspace, workspace_bytes, -1, -1, stream);
+}
+
+extern "C" int dqmk_kv_q40_attention_withhold_tile(const dqmk_kv_q40* kv, int layer, const float* q,
+                                                   int64_t ldq, const int* slots, const int* lengths,
+                                                   int n_cols, int n_heads, float* out, int64_t ldo,
+                                                   void* workspace, size_t workspace_bytes, int column,
+                                                   int tile, void* stream) {
+  return attention_call("KvQ40Attention", kv, layer, q, ldq, slots, lengths, n_cols, n_heads, out, ldo,
+                        workspace, workspace_bytes, column, tile, stream);
 }

@@ -384,6 +384,17 @@ int dqmk_kv_q40_attention(const dqmk_kv_q40* kv, int layer, const float* q_dev, 
                           float* out_dev, int64_t ldo, void* workspace_dev,
                           size_t workspace_bytes, void* stream);
 
+/* Test hook for the bounded waits: dqmk_kv_q40_attention with the copies of
+ * positions 32 tile .. 32 tile + 31 of column `column` withheld, so that the
+ * waits for them run out (about a second) and the device error flag is set.
+ * The rows of a column whose work a stopped CTA held are left as they were or
+ * NaN; every other row is what it is without. */
+int dqmk_kv_q40_attention_withhold_tile(const dqmk_kv_q40* kv, int layer, const float* q_dev,
+                                        int64_t ldq, const int* slots_dev, const int* lengths_dev,
+                                        int n_cols, int n_heads, float* out_dev, int64_t ldo,
+                                        void* workspace_dev, size_t workspace_bytes, int column,
+                                        int tile, void* stream);
+
 /* ------------------------------------------------------------------ */
 /* Engine: device-resident model + context (ForwardToken / ForwardBatch)*/
 /* ------------------------------------------------------------------ */

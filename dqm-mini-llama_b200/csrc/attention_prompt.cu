@@ -719,7 +719,9 @@ __global__ void __launch_bounds__(Cfg<DP, CTAS>::kThreads, CTAS) attention_promp
         rows_sync<kShare>(quarter);
 #pragma unroll
         for (int i = 0; i < P; ++i) tmax = fmaxf(tmax, red[T & 1][i][row]);
-        const float fs = cur.fq * mt.x;
+        // held to a float's normal range: the scales' product may leave it where
+        // scores do not, and times 0 or infinity a masked key or a score of 0 is NaN
+        const float fs = slow ? 1.0f : fminf(fmaxf(cur.fq * mt.x, 0x1p-126f), 0x1.fffffep127f);
         const float mnew = slow ? m : fmaxf(m, tmax * fs);
         const float ref = mnew == -INFINITY ? 0.0f : mnew;
         const float c = ex2(m - ref);

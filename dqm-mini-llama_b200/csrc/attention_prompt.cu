@@ -5,9 +5,10 @@
 //   s_ij = q_i . k_j / sqrt(D) for j <= i, softmax over j, out_i = sum p_ij v_j
 //
 // Both products run on the tensor cores with f32 results: an operand is scaled
-// by a power of two and split into two fp16 terms (x = hi + lo + r, |r| <=
-// 2^-22 |x|), and A_hi B_hi + A_hi B_lo + A_lo B_hi accumulate in fp32 tensor
-// memory.  That is three products for one, 562 TFLOP/s of the measured 1686;
+// by a power of two that brings the largest of those that share it into [2^14,
+// 2^15) and split into two fp16 terms (x = hi + lo + r, |r| <= 2^-22 |x|, or 2^-25
+// where lo is subnormal), and A_hi B_hi + A_hi B_lo + A_lo B_hi accumulate in fp32
+// tensor memory.  That is three products for one, 562 TFLOP/s of the measured 1686;
 // f32 FMAs have an eighth of it.
 //
 // First kernel (prompt_split): K and V of every sequence, in tiles of 64 keys
@@ -15,10 +16,13 @@
 // the second kernel's operands (K rows, V columns, both terms, 128-byte
 // swizzle), so that a tile is one contiguous bulk copy and needs neither a
 // tensor map nor any alignment of the sequence's first token.  K and V each take
-// one power of two a tile.  A tile whose rows differ by more than 2^16 in size, or
-// that holds an infinity or a NaN, would lose the smaller rows' bits or reach
-// queries that must not see it; it is marked, and the second kernel takes it
-// in f32 straight from the inputs.
+// one power of two a tile.  A tile whose rows and channels differ in size by more
+// than 2^14 together would lose bits of the smaller ones, and one that holds an
+// infinity or a NaN would reach queries that must not see it; it is marked, and the
+// second kernel takes it in f32 straight from the inputs.  With r, c and t the
+// largest of an element's row, channel and tile, r c / t is then at least 2^-2 in the
+// scale of the terms, so an element is off by at most 2^-22 |x| or 2^-23 r c / t,
+// whatever sizes rows and channels have.
 //
 // One more CTA of that kernel lists the second kernel's items, those with the
 // most keys first.
@@ -128,7 +132,7 @@ __device__ __forceinline__ int pow2_ex(float top) {
   const int fe = ((__float_as_int(top) >> 23) & 0xff) - 126;
   return top > 0.0f ? min(max(fe - 15, -120), 120) : 0;
 }
-// Two values to packed fp16 pairs with x = hi + lo + r, |r| <= 2^-22 |x|.
+// Two values to packed fp16 pairs with x = hi + lo + r, |r| <= 2^-22 |x| or 2^-25.
 __device__ __forceinline__ void split2(float x0, float x1, uint32_t& hi, uint32_t& lo) {
   const __half2 h = __floats2half2_rn(x0, x1);
   const float2 back = __half22float2(h);
@@ -139,7 +143,9 @@ __device__ __forceinline__ void split2(float x0, float x1, uint32_t& hi, uint32_
 
 // ------------------------------------------------------------ first kernel
 constexpr int kSplitThreads = 256;
-constexpr int kMostSpread = 16;  // exponents between a tile's largest and smallest row
+// Exponents from a tile's largest value to its smallest row's largest, and to its
+// smallest channel's, added up (rows and channels of zeros left out).
+constexpr int kMostSpread = 14;
 
 constexpr int kBins = 1024;      // items are listed by their key tiles, up to this many
 
@@ -206,7 +212,7 @@ __global__ void __launch_bounds__(kSplitThreads) prompt_split_kernel(const Promp
   __shared__ int64_t warp_sums[kSplitThreads / 32];
   __shared__ int place[3];  // the tile's sequence: first token, tokens, key tiles before it
   __shared__ float vt[kKeys][DP + 1];
-  __shared__ int top_bits, low_bits;
+  __shared__ int top_bits, low_row, channel_bits[DP];
   const int tid = threadIdx.x, kvh = blockIdx.y >> 1, is_v = blockIdx.y & 1, D = a.head_dim;
   pdl_trigger();
   if (blockIdx.x == 0) {  // first, so that it does not end last
@@ -217,8 +223,9 @@ __global__ void __launch_bounds__(kSplitThreads) prompt_split_kernel(const Promp
   if (tid == 0) {
     place[1] = 0;
     top_bits = 0;
-    low_bits = INT_MAX;
+    low_row = INT_MAX;
   }
+  if (tid < DP) channel_bits[tid] = 0;
   int64_t done = 0;
   for (int s0 = 0; s0 < a.n_seqs && done <= tile; s0 += kSplitThreads) {
     const int s = s0 + tid, n = s < a.n_seqs ? seq_len(a, s) : 0;
@@ -249,22 +256,34 @@ __global__ void __launch_bounds__(kSplitThreads) prompt_split_kernel(const Promp
                                   : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
   }
   // sizes compare as integers; an infinity or a NaN is larger than any number
+  int channels[4] = {0, 0, 0, 0};  // of this thread's rows
 #pragma unroll
   for (int i = 0; i < kPer; ++i) {
-    const float4 f = x[i];
-    int top = max(max(__float_as_int(fabsf(f.x)), __float_as_int(fabsf(f.y))),
-                  max(__float_as_int(fabsf(f.z)), __float_as_int(fabsf(f.w))));
+    const int size[4] = {__float_as_int(fabsf(x[i].x)), __float_as_int(fabsf(x[i].y)),
+                         __float_as_int(fabsf(x[i].z)), __float_as_int(fabsf(x[i].w))};
+#pragma unroll
+    for (int e = 0; e < 4; ++e) channels[e] = max(channels[e], size[e]);
+    int top = max(max(size[0], size[1]), max(size[2], size[3]));
 #pragma unroll
     for (int o = 1; o < (kF4 < 32 ? kF4 : 32); o <<= 1)
       top = max(top, __shfl_xor_sync(0xffffffffu, top, o));
     if (c4 == 0 && top > 0) {
       atomicMax(&top_bits, top);
-      atomicMin(&low_bits, top);
+      atomicMin(&low_row, top);
     }
   }
+#pragma unroll
+  for (int e = 0; e < 4; ++e) atomicMax(&channel_bits[e * kF4 + c4], channels[e]);
   __syncthreads();
-  const int top = top_bits, low = low_bits;
-  const bool marked = top >= 0x7f800000 || (top > 0 && (top >> 23) - (low >> 23) > kMostSpread);
+  int low_channel = INT_MAX;  // by every warp
+#pragma unroll
+  for (int i = 0; i < DP; i += 32) {
+    const int size = channel_bits[i + (tid & 31)];
+    low_channel = min(low_channel, size ? size : INT_MAX);
+  }
+  low_channel = __reduce_min_sync(0xffffffffu, low_channel);
+  const int top = top_bits;
+  const bool marked = top >= 0x7f800000 || (top > 0 && 2 * (top >> 23) - (low_row >> 23) - (low_channel >> 23) > kMostSpread);
   const int e = pow2_ex(__int_as_float(top));
   const float down = pow2f(-e);
 #pragma unroll

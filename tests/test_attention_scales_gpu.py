@@ -42,3 +42,56 @@ def test_attention_prompt_large_queries_before_an_infinity(pkg, cuda, gen, heads
         check_prompt(torch, out[:at], *(y[:at] for y in x), [0, at], f"{size} before")
         g = h // kv
         check_prompt(torch, out[:, :g], x[0][:, :g], x[1][:, :1], x[2][:, :1], [0, n], f"{size} beside")
+
+
+def spread(torch, gen, n, bits):  # noqa: F811
+    """n powers of two, 2^-bits among them, and 1."""
+    e = -torch.randint(0, bits + 1, (n,), generator=gen, device="cuda").float()
+    e[n // 3], e[n // 2] = -bits, 0
+    return torch.exp2(e)
+
+
+@pytest.mark.parametrize("heads", HEADS, ids=lambda h: "h%d_kv%d_d%d" % h)
+@pytest.mark.parametrize("rows", [0, 8, 12, 15])
+@pytest.mark.parametrize("channels", [0, 5, 7, 10, 14])
+def test_attention_prompt_keys_of_many_sizes(pkg, cuda, gen, heads, rows, channels):  # noqa: F811
+    """Channels of the keys that differ in size, the queries' the other way
+    round, so that each counts the same in a score; and among the rows of a tile
+    of keys some that are 2^rows larger and weigh nothing: their scores are far
+    below the others', or they come behind the tokens that are looked at."""
+    torch = cuda
+    h, kv, d = heads
+    n = 130
+    q, k, v = (randn(torch, gen, n, x, d) for x in (h, kv, kv))
+    c = spread(torch, gen, d, channels)
+    q[..., 0] = q[..., 0].abs() + 1.0
+    for large in (20, 85):
+        k[large] *= 2.0 ** rows
+        if rows:
+            k[large] *= 0.01
+            k[large, :, 0] = -8.0 * 2.0 ** rows  # a score of about -2^rows or less
+    k[60] *= 2.0 ** rows
+    k[128] *= 2.0 ** rows
+    q, k = q / c, k * c
+    starts = [0, n]
+    out = pkg.attention_prompt(q, k, v, i32(torch, starts))
+    # tokens up to the first large key see none, those up to key 60 one of no weight
+    check_prompt(torch, out[:20], q[:20], k[:20], v[:20], [0, 20], f"{rows} {channels} first")
+    check_prompt(torch, out[:60], q[:60], k[:60], v[:60], [0, 60], f"{rows} {channels}", norm=0)
+    check_prompt(torch, out, q, k, v, starts, f"{rows} {channels} all", norm=0)
+
+
+@pytest.mark.parametrize("heads", HEADS, ids=lambda h: "h%d_kv%d_d%d" % h)
+@pytest.mark.parametrize("rows,channels", [(0, 10), (0, 14), (7, 7), (0, 20), (0, 24), (0, 40), (12, 12),
+                                           (15, 10), (15, 1)])
+def test_attention_prompt_values_of_many_sizes(pkg, cuda, gen, heads, rows, channels):  # noqa: F811
+    """Channels of the values that differ by up to 2^40, and rows: every output
+    channel to its own precision, whatever the others' size."""
+    torch = cuda
+    h, kv, d = heads
+    starts = [0, 1, 33, 163]
+    q, k, v = (randn(torch, gen, 163, x, d) for x in (h, kv, kv))
+    v *= spread(torch, gen, d, channels)
+    v *= spread(torch, gen, 163, rows)[:, None, None]
+    out = pkg.attention_prompt(q, k, v, i32(torch, starts))
+    check_prompt(torch, out, q, k, v, starts, f"{rows} {channels}")

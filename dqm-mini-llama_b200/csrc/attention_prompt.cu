@@ -634,10 +634,13 @@ __global__ void __launch_bounds__(Cfg<DP, CTAS>::kThreads, CTAS) attention_promp
       const float4* from[2] = {reinterpret_cast<const float4*>(stage + r0 * C::kRowBytes) + (lane & 3),
                                reinterpret_cast<const float4*>(stage + (r0 + 8) * C::kRowBytes) + (lane & 3)};
       float top[2];
-      // queries of ordinary size keep all their bits under one scale, 2^7; with
-      // others among the 32 rows they are split again, under a scale of their row
-      constexpr int kUsual = -7;
-      auto usual = [](float t) { return !(t > 0.0f) || (t >= 0x1p-10f && t < 256.0f); };
+      // queries whose largest value is of ordinary size are split under one scale,
+      // 2^10, which leaves elements off by at most 2^-22 of themselves or 2^-34 of
+      // that value (so that keys may outweigh them by channel); with others among
+      // the 32 rows all are split again, those under a scale of their row, 2^-39
+      // (33 ragged prompts 227 us, 237 with every row split again)
+      constexpr int kUsual = -10;
+      auto usual = [](float t) { return !(t > 0.0f) || (t >= 0.5f && t < 32.0f); };
       float up[2] = {pow2f(-kUsual), pow2f(-kUsual)};
       auto pass = [&] {
         top[0] = top[1] = 0.0f;

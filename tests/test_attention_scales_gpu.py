@@ -95,3 +95,20 @@ def test_attention_prompt_values_of_many_sizes(pkg, cuda, gen, heads, rows, chan
     v *= spread(torch, gen, 163, rows)[:, None, None]
     out = pkg.attention_prompt(q, k, v, i32(torch, starts))
     check_prompt(torch, out, q, k, v, starts, f"{rows} {channels}")
+
+
+@pytest.mark.parametrize("size", [2.0 ** -12, 2.0 ** -9, 2.0 ** -1, 1.0, 2.0 ** 4, 2.0 ** 7, 2.0 ** 12])
+@pytest.mark.parametrize("channels", [6, 10, 13])
+def test_attention_prompt_queries_of_many_sizes(pkg, cuda, gen, size, channels):  # noqa: F811
+    """Query rows of any size whose channels differ, the keys' the other way round."""
+    torch = cuda
+    n, h, kv, d = 140, 14, 2, 64
+    q, k, v = (randn(torch, gen, n, x, d) for x in (h, kv, kv))
+    c = spread(torch, gen, d, channels)
+    c[-8:] = 2.0 ** -channels
+    q = q * c * size
+    q[::7, 1:] *= 0.01  # rows whose largest channel stands out
+    k = k / c / size
+    starts = [0, n]
+    out = pkg.attention_prompt(q, k, v, i32(torch, starts))
+    check_prompt(torch, out, q, k, v, starts, f"{size} {channels}", norm=0)

@@ -773,23 +773,46 @@ __global__ void __launch_bounds__(Cfg<DP, CTAS>::kThreads, CTAS) attention_promp
         corr = slow ? 1.0f : c;
         vscale = mt.z;
         if (slow && cur.tok >= 0) {
-          // the marked tile in f32, key by key, from the inputs; o is at m's scale
+          // the marked tile in f32 from the inputs, o at m's scale; two keys at a time,
+          // as a query load takes a line a lane.  With one marked tile in sight of every
+          // row, 602 tokens of 14 / 2 heads of 64 take 135 us for 19.5, 2048 of 28 / 4
+          // of 128 990 for 85 (190 and 1390 key by key).  8 keys at a time (104, 750)
+          // slow the loop that serves the other tiles (4096 tokens of 14 / 2 heads of
+          // 64: 120 -> 130 us), as do scores and weights through tensor memory
+          // (54, 271; 33 ragged prompts 229 -> 240).
           const float* qr = a.q + (int64_t)(cur.first + cur.tok) * a.ldq + (int64_t)cur.head * a.head_dim;
-          for (int key = kt; key <= min(cur.tok, kt + kKeys - 1); ++key) {
+          const int last = min(cur.tok, kt + kKeys - 1);
+#pragma unroll 1
+          for (int key = kt; key <= last; key += 2) {
             const float* kr = a.k + (int64_t)(cur.first + key) * a.ldk + (int64_t)cur.kvh * a.head_dim;
-            const float* vr = a.v + (int64_t)(cur.first + key) * a.ldv + (int64_t)cur.kvh * a.head_dim;
-            float s = 0.0f;
-            for (int d = 0; d < a.head_dim; ++d) s = fmaf(qr[d], kr[d], s);
-            s *= a.scale;
-            const float top = fmaxf(m, s), at = top == -INFINITY ? 0.0f : top;
-            const float down = ex2(m - at), p = ex2(s - at + 14.0f);
+            const float* vr = a.v + (int64_t)(cur.first + key) * a.ldv + (int64_t)cur.kvh * a.head_dim + part * W;
+            const bool two = key < last;  // no key that the row does not see is read
+            const int64_t k_next = two ? a.ldk : 0, v_next = two ? a.ldv : 0;
+            float s0 = 0.0f, s1 = 0.0f;
+#pragma unroll 4
+            for (int d = 0; d < a.head_dim; d += 4) {
+              const float4 x = *reinterpret_cast<const float4*>(qr + d);
+              const float4 y = *reinterpret_cast<const float4*>(kr + d), z = *reinterpret_cast<const float4*>(kr + k_next + d);
+              s0 = fmaf(x.w, y.w, fmaf(x.z, y.z, fmaf(x.y, y.y, fmaf(x.x, y.x, s0))));
+              s1 = fmaf(x.w, z.w, fmaf(x.z, z.z, fmaf(x.y, z.y, fmaf(x.x, z.x, s1))));
+            }
+            s0 *= a.scale;
+            s1 = two ? s1 * a.scale : -INFINITY;
+            const float top = fmaxf(fmaxf(m, s0), s1), at = top == -INFINITY ? 0.0f : top;
+            const float down = ex2(m - at), p0 = ex2(s0 - at + 14.0f), p1 = ex2(s1 - at + 14.0f);
             l *= down;
-            if (part == 0) l += p;
+            if (part == 0) l += p0 + p1;
             m = top;
 #pragma unroll
-            for (int d = 0; d < W; ++d) {
-              const int dd = part * W + d;
-              o[d] = fmaf(p, dd < a.head_dim ? vr[dd] : 0.0f, o[d] * down);
+            for (int d = 0; d < W; d += 4) {
+              const bool in = part * W + d < a.head_dim;
+              const float4 none = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+              const float4 y = in ? *reinterpret_cast<const float4*>(vr + d) : none;
+              const float4 z = in && two ? *reinterpret_cast<const float4*>(vr + v_next + d) : none;
+              o[d] = fmaf(p1, z.x, fmaf(p0, y.x, o[d] * down));
+              o[d + 1] = fmaf(p1, z.y, fmaf(p0, y.y, o[d + 1] * down));
+              o[d + 2] = fmaf(p1, z.z, fmaf(p0, y.z, o[d + 2] * down));
+              o[d + 3] = fmaf(p1, z.w, fmaf(p0, y.w, o[d + 3] * down));
             }
           }
         }

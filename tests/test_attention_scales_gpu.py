@@ -112,3 +112,32 @@ def test_attention_prompt_queries_of_many_sizes(pkg, cuda, gen, size, channels):
     starts = [0, n]
     out = pkg.attention_prompt(q, k, v, i32(torch, starts))
     check_prompt(torch, out, q, k, v, starts, f"{size} {channels}", norm=0)
+
+
+@pytest.mark.parametrize("heads", [(14, 2, 64), (28, 4, 128), (3, 3, 36), (6, 1, 80), (130, 1, 32)],
+                         ids=lambda h: "h%d_kv%d_d%d" % h)
+@pytest.mark.parametrize("which", ["keys", "values", "both"])
+@pytest.mark.parametrize("lengths", [[300, 1, 70], [40, 64, 65, 3], [600] * 20], ids=lambda n: f"{len(n)}x{max(n)}")
+def test_attention_prompt_marked_tiles(pkg, cuda, gen, heads, which, lengths):  # noqa: F811
+    """Rows of almost nothing (not zeros) in some tiles of the keys, of the
+    values, or of both: the tiles taken in f32 between others, first and last
+    ones among them, give what the formula gives, the same each time."""
+    torch = cuda
+    h, kv, d = heads
+    starts = [0]
+    for x in lengths:
+        starts.append(starts[-1] + x)
+    n = starts[-1]
+    q, k, v = (randn(torch, gen, n, x, d) for x in (h, kv, kv))
+    for s, x in zip(starts, lengths):
+        for at in (0, 130, x - 1):
+            if at < x and x > 1:
+                if which != "values":
+                    k[s + at] *= 1e-9
+                if which != "keys":
+                    v[s + at] *= 1e-9
+    if which == "both":
+        v[starts[-2] + lengths[-1] // 2:, :, 0] *= 2.0 ** 40
+    out = pkg.attention_prompt(q, k, v, i32(torch, starts))
+    check_prompt(torch, out, q, k, v, starts)
+    assert torch.equal(out, pkg.attention_prompt(q, k, v, i32(torch, starts)))

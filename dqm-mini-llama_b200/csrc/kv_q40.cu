@@ -286,8 +286,6 @@ struct AttnQ40Args {
   float scale;                       // log2(e) / sqrt(D)
   float* part;                       // [CTA][2][part_floats]
   int2* spans;                       // [column][sub]: first and last CTA
-  int n_ctas;                        // of the attention kernel: the partial sums there are
-  int withhold_col, withhold_tile;   // test hook: copies that are never made (-1: none)
 };
 
 template <int NB>
@@ -384,8 +382,12 @@ struct Piece {
   int col, len, slot, sub, ch0, take;
 };
 
-template <int NB>
-__global__ void __launch_bounds__(kThreads, kCtasPerSm) kv_q40_attention_kernel(const AttnQ40Args a) {
+// WITHHOLD: a test hook, the copies of one tile {column, tile} are never made.  It
+// and the join's count of CTAs are arguments of their own: as members of AttnQ40Args
+// they moved the registers that are spilled (16 x 65536 167 -> 179 us).
+template <int NB, bool WITHHOLD>
+__global__ void __launch_bounds__(kThreads, kCtasPerSm)
+    kv_q40_attention_kernel(const AttnQ40Args a, const int2 withheld) {
   using S = Shape<NB>;
   constexpr int D = S::kD;
   extern __shared__ __align__(128) unsigned char smem[];  // rings, then the warps' sums
@@ -490,9 +492,9 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) kv_q40_attention_kernel(
   auto issue = [&](const Piece& x, int i) {  // lane 0: this warp's tile i of the piece
     unsigned char* st = ring + (issued % kStages) * S::kStageBytes;
     uint64_t* bar = &bars[warp][issued % kStages];
-    const int tile = first_of(x) + i * kWarps;
-    if (x.col == a.withhold_col && tile == a.withhold_tile) return;
-    const int64_t at = (first_tile(a.c, x.slot, x.sub % a.c.n_kv_heads) + tile) * S::kTileBytes;
+    if constexpr (WITHHOLD)
+      if (x.col == withheld.x && first_of(x) + i * kWarps == withheld.y) return;
+    const int64_t at = (first_tile(a.c, x.slot, x.sub % a.c.n_kv_heads) + first_of(x) + i * kWarps) * S::kTileBytes;
     tc::bar_expect_tx(bar, S::kStageBytes);
     bulk_load(st, a.c.k + at, S::kTileBytes, bar);
     bulk_load(st + S::kTileBytes, a.c.v + at, S::kTileBytes, bar);
@@ -515,31 +517,49 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) kv_q40_attention_kernel(
         qx[i][b] = h0 + hh < a.group ? a.q[x.col * a.ldq + head * D + 32 * b + lane] : 0.0f;
       }
   };
-  // the piece behind x: it begins a group, of this column or of the next with
-  // any units; no chunks of it where the run ends
-  auto next_piece = [&](const Piece& x, Piece& nx) {
-    nx = x;
-    nx.take = 0;
-    if (u >= u1) return u;
-    if (++nx.sub == a.subs) {
-      nx.sub = 0;
-      do {
-        ++nx.col;
-        nx.slot = slot_of(a, nx.col);
-        nx.len = visible(a, a.lengths[nx.col], nx.slot);
-      } while (nx.len == 0);
-    }
-    return u + cut(nx, 0, u);
-  };
   start(p);
   load_q(p);
+  // The spans of the groups that start here, before the first wait: the join then
+  // finds them also where one runs out.
+  if (tid == kThreads - 1) {
+    Piece x = p;
+    for (int64_t at = group0, r = u;;) {
+      if (x.ch0 == 0)
+        a.spans[(int64_t)x.col * a.subs + x.sub] =
+            make_int2(blockIdx.x, cta_of(at + kExtra + chunks_of(x.len) - 1, total, n_ctas));
+      if (r >= u1) break;
+      if (++x.sub == a.subs) {
+        x.sub = 0;
+        do {
+          ++x.col;
+          x.len = visible(a, a.lengths[x.col], slot_of(a, x.col));
+        } while (x.len == 0);
+      }
+      at = r;
+      r += cut(x, 0, r);
+      if (x.take == 0) break;
+    }
+  }
 
   while (true) {
     const int kvh = p.sub % a.c.n_kv_heads, h0 = (p.sub / a.c.n_kv_heads) * kGroup;
     const int n_here = min(kGroup, a.group - h0);  // heads of this group
     const int mine = tiles_mine(p), tile0 = first_of(p), len = p.len;
-    Piece nx;
-    const int64_t behind = next_piece(p, nx);
+    // the next piece begins a group: of this column, or of the next with any
+    Piece nx = p;
+    int64_t behind = u;
+    nx.take = 0;
+    if (u < u1) {
+      if (++nx.sub == a.subs) {
+        nx.sub = 0;
+        do {
+          ++nx.col;
+          nx.slot = slot_of(a, nx.col);
+          nx.len = visible(a, a.lengths[nx.col], nx.slot);
+        } while (nx.len == 0);
+      }
+      behind += cut(nx, 0, u);
+    }
     const bool more = nx.take > 0;
 
     // ---- the group's queries as A operands (high and low terms), two heads a warp
@@ -777,31 +797,16 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) kv_q40_attention_kernel(
         }
       }
     }
-    if (p.ch0 == 0 && tid == 0)
-      a.spans[(int64_t)p.col * a.subs + p.sub] =
-          make_int2(blockIdx.x, cta_of(group0 + kExtra + chunks - 1, total, n_ctas));
     if (!more) break;
-    group0 = u;
     u = behind;
     p = nx;
   }
   if (!ok) {
-    // A wait ran out.  Of the groups that this run leaves unfinished, the join
-    // skips those that start here; the others' sums of this run become NaN, so
-    // that nothing the workspace held before enters a result.
-    for (bool more = true; more;) {
-      if (p.ch0 == 0) {
-        if (tid == 0) a.spans[(int64_t)p.col * a.subs + p.sub] = make_int2(-1, -1);
-      } else if (tid < kGroup) {
-        float* part = a.part + (int64_t)blockIdx.x * 2 * S::kPartFloats + kGroup * D;
-        part[tid] = 0.0f;
-        part[kGroup + tid] = __int_as_float(0x7fc00000);
-      }
-      Piece nx;
-      u = next_piece(p, nx);
-      more = nx.take > 0;
-      p = nx;
-    }
+    // A wait ran out: the sums of weights among this run's partial sums become NaN,
+    // so that nothing the workspace held before enters a result.
+    if (tid < 2 * kGroup)
+      a.part[((int64_t)blockIdx.x * 2 + tid / kGroup) * S::kPartFloats + kGroup * (D + 1) + tid % kGroup] =
+          __int_as_float(0x7fc00000);
     // leave once this warp's own copies have landed or given up
     for (; used < issued; ++used) {
       const unsigned long long t0 = tc::now_ns();
@@ -817,7 +822,8 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) kv_q40_attention_kernel(
 // warps' sums are joined in order.  HEADS heads a CTA: 1 where there are few
 // groups and many partials of each, 8 where there are many groups.
 template <int NB, int HEADS>
-__global__ void __launch_bounds__(HEADS == 1 ? 1024 : 512) kv_q40_join_kernel(const AttnQ40Args a) {
+__global__ void __launch_bounds__(HEADS == 1 ? 1024 : 512)
+    kv_q40_join_kernel(const AttnQ40Args a, const int n_ctas) {
   using S = Shape<NB>;
   constexpr int kJoinThreads = HEADS == 1 ? 1024 : 512, kJoinWarps = kJoinThreads / 32;
   constexpr int D = S::kD, kSlots = kJoinWarps / HEADS;
@@ -828,10 +834,10 @@ __global__ void __launch_bounds__(HEADS == 1 ? 1024 : 512) kv_q40_join_kernel(co
   const int len = visible(a, a.lengths[col], slot_of(a, col));
   pdl_wait();  // every CTA waits, so that this grid's end is also the first kernel's
   if (chunks_of(len) == 0) return;
-  // whole in one CTA, or unfinished (the partial sums' indices are checked
-  // against the workspace whatever it holds)
+  // whole in one CTA; the partial sums' indices stay within the workspace
+  // whatever it holds
   const int2 span = __ldcg(a.spans + blockIdx.x);
-  if (span.x < 0 || span.x >= span.y || span.y >= a.n_ctas) return;
+  if (span.x < 0 || span.x >= span.y || span.y >= n_ctas) return;
   const int h = blockIdx.y * HEADS + warp % HEADS, slot = warp / HEADS;
   float m = -INFINITY, l = 0.0f, acc[NB];
 #pragma unroll
@@ -880,17 +886,18 @@ constexpr size_t attention_smem() {
   return (size_t)kWarps * (kStages * Shape<NB>::kStageBytes + kGroup * Shape<NB>::kD * sizeof(float));
 }
 
-template <int NB>
-cudaError_t launch_attention_q40(const AttnQ40Args& args, int n_ctas, bool join, cudaStream_t st) {
+template <int NB, bool WITHHOLD>
+cudaError_t launch_attention_q40(const AttnQ40Args& args, int n_ctas, int2 withheld, bool join,
+                                 cudaStream_t st) {
   static DeviceOnce once;
   cudaError_t e = once.run([] {
-    return cudaFuncSetAttribute(kv_q40_attention_kernel<NB>,
+    return cudaFuncSetAttribute(kv_q40_attention_kernel<NB, WITHHOLD>,
                                 cudaFuncAttributeMaxDynamicSharedMemorySize,
                                 (int)attention_smem<NB>());
   });
   if (e != cudaSuccess) return e;
-  e = launch(kv_q40_attention_kernel<NB>, dim3(n_ctas), dim3(kThreads), attention_smem<NB>(), st,
-             false, args);
+  e = launch(kv_q40_attention_kernel<NB, WITHHOLD>, dim3(n_ctas), dim3(kThreads),
+             attention_smem<NB>(), st, false, args, withheld);
   if (e != cudaSuccess || !join) return e;
   // One / 8 heads a CTA of the join, us of both kernels, 28 / 4 heads of 128: 4
   // groups of 32768 positions 14.5 / 41.7, 32 of 8192 22.1 / 23.0, 48 28.5 / 28.5,
@@ -898,8 +905,9 @@ cudaError_t launch_attention_q40(const AttnQ40Args& args, int n_ctas, bool join,
   const unsigned groups = (unsigned)(args.n_cols * args.subs);
   if (groups < 64)
     return launch(kv_q40_join_kernel<NB, 1>, dim3(groups, kGroup), dim3(1024), 0, st, use_pdl(),
-                  args);
-  return launch(kv_q40_join_kernel<NB, kGroup>, dim3(groups), dim3(512), 0, st, use_pdl(), args);
+                  args, n_ctas);
+  return launch(kv_q40_join_kernel<NB, kGroup>, dim3(groups), dim3(512), 0, st, use_pdl(), args,
+                n_ctas);
 }
 
 // CTAs of the attention kernel: what the SMs hold at once, or the most chunks
@@ -1085,19 +1093,24 @@ int attention_call(const char* name, const dqmk_kv_q40* kv, int layer, const flo
   a.q = q, a.ldq = ldq, a.out = out, a.ldo = ldo;
   a.lengths = lengths, a.slots = slots, a.n_cols = n_cols, a.n_heads = n_heads;
   a.scale = kLog2e / sqrtf((float)kv->head_dim);
-  a.withhold_col = withhold_col, a.withhold_tile = withhold_tile;
   a.part = static_cast<float*>(workspace);
   a.spans = reinterpret_cast<int2*>(static_cast<char*>(workspace) +
                                     part_bytes(n_cols, a.subs, kv->max_seq, kv->head_dim));
-  const int n_ctas = a.n_ctas = attention_ctas(n_cols, a.subs, kv->max_seq);
+  const int n_ctas = attention_ctas(n_cols, a.subs, kv->max_seq);
   const bool join = kv->max_seq > kChunk;  // else every run ends with a whole group
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   cudaError_t e;
+  const int2 withheld = make_int2(withhold_col, withhold_tile);
+  auto run = [&](auto nb) {
+    constexpr int NB = decltype(nb)::value;
+    return withhold_col < 0 ? launch_attention_q40<NB, false>(a, n_ctas, withheld, join, st)
+                            : launch_attention_q40<NB, true>(a, n_ctas, withheld, join, st);
+  };
   switch (a.c.nb) {
-    case 1: e = launch_attention_q40<1>(a, n_ctas, join, st); break;
-    case 2: e = launch_attention_q40<2>(a, n_ctas, join, st); break;
-    case 3: e = launch_attention_q40<3>(a, n_ctas, join, st); break;
-    default: e = launch_attention_q40<4>(a, n_ctas, join, st); break;
+    case 1: e = run(std::integral_constant<int, 1>()); break;
+    case 2: e = run(std::integral_constant<int, 2>()); break;
+    case 3: e = run(std::integral_constant<int, 3>()); break;
+    default: e = run(std::integral_constant<int, 4>()); break;
   }
   DQMK_CUDA_RET(api.c_str(), e);
   return DQMK_OK;

@@ -247,7 +247,11 @@ __global__ void __launch_bounds__(kRowThreads) kv_q40_read_kernel(const RowsArgs
 // scales, kept like the running maximum of the scores, and p takes 2^15 (less
 // where d is above 1) and d a power of two where it is below 2^-6.  The terms
 // of w come from p = ph + pl and d in fp16 arithmetic: hi = ph d, lo = (ph d -
-// hi) + pl d, whose first part a fused multiply-add leaves exact.
+// hi) + pl d, whose first part a fused multiply-add leaves exact.  Terms end at
+// 2^-24, so a w that is small beside the largest (at least 2^8) is off by 2^-32 of
+// that one rather than by 2^-22 of itself.  Blocks' scales far apart (2^10) would
+// need a power of two for each block; that was built and took 16 columns of 65536
+// positions from 167 to 170 us, for values that f32 rows seldom hold.
 //
 // A code becomes a half by one AND/OR, (w & 0x000f) | 0x6400 = 1024 + n, and
 // one addition that centres it: n - 8 (16 (n - 8) from a high nibble; for a key

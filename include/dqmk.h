@@ -320,12 +320,19 @@ int dqmk_qk_norm_rope(const float* q_dev, int64_t ldq, const float* k_dev, int64
  * values a token, token t at element t * ld; out_dev must not overlap the
  * inputs.  Rows outside every sequence (behind the last one) are left as they
  * were.  A sequence whose offsets are out of order or outside 0..n_tokens is
- * skipped and recorded (dqmk_device_error bit 3).  Results are within f32
- * summation order of f32 arithmetic, and the same for the same arguments every
- * time.  head_dim: a multiple of 4, at most 128; at most 2^20 query heads to a
+ * skipped and recorded (dqmk_device_error bit 3).  Results are the same for the
+ * same arguments every time.  They are those of f32 sums over operands of 22 bits:
+ * a query is off by at most 2^-22 of itself or 2^-34 of its head row's largest, a
+ * key or value by 2^-22 or 2^-23 r c / t, the largest of its row, its channel and
+ * its tile of 64 tokens, and a weight by 2^-22 or 2^-39 of its row's largest.  A
+ * tile whose rows and channels differ by more than 2^14 together, or that holds an
+ * infinity or a NaN, is taken in f32 arithmetic, which costs each 128 rows (token,
+ * head of a group) that see it 115 us at head_dim 64 and 300 at 128, in place of
+ * about 1.  head_dim: a multiple of 4, at most 128; at most 2^20 query heads to a
  * key/value head; pointers 16-byte aligned, strides multiples of 4.
- * workspace_dev: dqmk_attention_prompt_workspace bytes, contents ignored; calls
- * that may overlap on the GPU need one each. */
+ * workspace_dev: dqmk_attention_prompt_workspace bytes (as many as k and v for long
+ * sequences, up to 64 times that for sequences of one token), contents ignored;
+ * calls that may overlap on the GPU need one each. */
 size_t dqmk_attention_prompt_workspace(int n_tokens, int n_seqs, int n_heads, int n_kv_heads,
                                        int head_dim);
 int dqmk_attention_prompt(const float* q_dev, int64_t ldq, const float* k_dev, int64_t ldk,
@@ -373,9 +380,13 @@ int dqmk_kv_q40_read(const dqmk_kv_q40* kv, int layer, const int* slots_dev,
  * growing lengths, once their rows are written).  Length 0 gives a row of
  * zeros, whatever its slot; so do a length outside 0..max_seq and a slot
  * outside the cache, which are recorded (dqmk_device_error bit 3).  out_dev may
- * be q_dev with the same stride; other overlap is not allowed.  Results are those of f32 arithmetic
- * on the cache's values (within f32 summation order), and the same for the
- * same arguments every time.  workspace_dev: dqmk_kv_q40_attention_workspace
+ * be q_dev with the same stride; other overlap is not allowed.  Results are the
+ * same for the same arguments every time.  They are those of f32 sums over the
+ * cache's values with operands of 22 bits: a query is off by at most 2^-22 of itself
+ * or 2^-35 of its head's largest, and a weight times a block's scale by 2^-22 or
+ * 2^-32 of the column's largest such product (scales between 2^-14 and 2^7).
+ * More than 8 query heads to a KV head read the cache once for every 8.
+ * workspace_dev: dqmk_kv_q40_attention_workspace
  * bytes, 16-byte aligned, contents ignored; calls that may overlap on the GPU
  * need one each. */
 size_t dqmk_kv_q40_attention_workspace(const dqmk_kv_q40* kv, int n_cols, int n_heads);

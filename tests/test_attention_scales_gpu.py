@@ -3,7 +3,8 @@ References and bounds are those of the attention block's tests: a score is off
 by at most (16 + 6 D) e sum |q k| / sqrt(D), e = 2^-24, whatever the sizes."""
 import pytest
 
-from test_attention_block_gpu import check_prompt, gen, i32, randn  # noqa: F401
+from test_attention_block_gpu import (attend, check_close, check_decode, check_prompt, gen, i32,  # noqa: F401
+                                      randn)
 
 pytestmark = pytest.mark.gpu
 
@@ -141,3 +142,65 @@ def test_attention_prompt_marked_tiles(pkg, cuda, gen, heads, which, lengths):  
     out = pkg.attention_prompt(q, k, v, i32(torch, starts))
     check_prompt(torch, out, q, k, v, starts)
     assert torch.equal(out, pkg.attention_prompt(q, k, v, i32(torch, starts)))
+
+
+def blocks(torch, d, bits):
+    """A power of two for each channel, the same in a block of 32: 1, and 2^-bits in every other block."""
+    c = torch.ones(d, device="cuda")
+    c.view(-1, 32)[1::2] = 2.0 ** -bits
+    return c
+
+
+def cache_of(pkg, torch, k, v):
+    """One sequence's cache of these rows, and the values it holds."""
+    n, kv, d = k.shape
+    cache = pkg.KvCacheQ40(1, 1, n, kv, d)
+    p = torch.arange(n, device="cuda", dtype=torch.int32)
+    cache.write(0, k, v, p, torch.zeros_like(p))
+    ks, vs = cache.read(0, p, torch.zeros_like(p))
+    return cache, ks[None], vs[None]
+
+
+@pytest.mark.parametrize("heads", [(14, 2, 64), (28, 4, 128), (5, 1, 96)], ids=lambda h: "h%d_kv%d_d%d" % h)
+@pytest.mark.parametrize("bits", [6, 10, 14, 18, 22])
+@pytest.mark.parametrize("size", [1.0, 100.0, 2.0 ** -5])
+def test_cache_attention_value_blocks_of_many_sizes(pkg, cuda, gen, heads, bits, size):  # noqa: F811
+    """Blocks of the values that differ by up to 2^22, also where the large ones
+    come late or in few rows.  Beside the bound of any attention here, a
+    product of a weight and a scale is off by 2^-32 of the largest of them, and
+    a value is up to 8 times its scale (its block's largest at least 7 times)."""
+    torch = cuda
+    h, kv, d = heads
+    n = 1100
+    for late in (0, 1, 700):
+        k, v = (randn(torch, gen, n, kv, d) for _ in "kv")
+        v *= size * blocks(torch, d, bits)
+        v[:late, :, :32] *= 2.0 ** -bits  # all small at first
+        v[40:48] = 0
+        v[300:420, :, -32:] *= 2.0 ** -4
+        cache, ks, vs = cache_of(pkg, torch, k, v)
+        q = randn(torch, gen, 1, h, d)
+        for length in (1, 2, 33, 45, 140, 701, 1100):
+            out = cache.attention(q, 0, i32(torch, [length]), i32(torch, [0]))
+            kk, vv = (x[0, :length].permute(1, 0, 2).repeat_interleave(h // kv, 0).double() for x in (ks, vs))
+            seen = torch.ones(1, length, dtype=torch.bool, device="cuda")
+            ref, bound = attend(torch, q[0][:, None], kk, vv, seen)
+            p = torch.softmax(q[0].double()[:, None] @ kk.transpose(-1, -2) / d ** 0.5, -1)
+            largest = (p[:, 0] * vv.abs().amax(-1) / 7).amax(-1)[:, None, None]
+            check_close(out[0][:, None], ref, bound + 8 * length * 2.0 ** -32 * largest,
+                        f"{bits} {size} {late} {length}")
+
+
+@pytest.mark.parametrize("heads", [(14, 2, 64), (28, 4, 128)], ids=lambda h: "h%d_kv%d_d%d" % h)
+@pytest.mark.parametrize("bits", [6, 10, 12])
+def test_cache_attention_key_blocks_of_many_sizes(pkg, cuda, gen, heads, bits):  # noqa: F811
+    """Blocks of the keys that differ in size, the queries' the other way round."""
+    torch = cuda
+    h, kv, d = heads
+    k, v = (randn(torch, gen, 700, kv, d) for _ in "kv")
+    c = blocks(torch, d, bits)
+    cache, ks, vs = cache_of(pkg, torch, k * c, v)
+    q = randn(torch, gen, 1, h, d) / c
+    for length in (1, 45, 700):
+        out = cache.attention(q, 0, i32(torch, [length]), i32(torch, [0]))
+        check_decode(torch, out, q, ks, vs, [length], [0], f"{bits}")

@@ -99,6 +99,8 @@ SIGNATURES = {
     "dqmk_attention_prompt_workspace": ([_i, _i, _i, _i, _i], _sz),
     "dqmk_attention_prompt": ([_vp, _i64, _vp, _i64, _vp, _i64, _vp, _i, _i, _i, _i, _i, _vp, _i64,
                                _vp, _sz, _vp], _i),
+    "dqmk_attention_prompt_withhold_tile": ([_vp, _i64, _vp, _i64, _vp, _i64, _vp, _i, _i, _i, _i,
+                                             _i, _vp, _i64, _vp, _sz, _i, _vp], _i),
     "dqmk_kv_q40_bytes": ([_i, _i, _i, _i, _i], _sz),
     "dqmk_kv_q40_write": ([_kvp, _i, _vp, _i64, _vp, _i64, _vp, _vp, _i, _vp], _i),
     "dqmk_kv_q40_read": ([_kvp, _i, _vp, _vp, _i, _vp, _i64, _vp, _i64, _vp], _i),

@@ -52,6 +52,7 @@
 // 33 ragged prompts 230 us; 602 tokens of 14 / 2 heads of 64 20 us.  A score product
 // of 64 keys takes 44.8 cycles, 32 by its operations; one of 128 its full 64.
 #include <climits>
+#include <type_traits>
 
 #include "common.cuh"
 #include "internal.h"
@@ -389,8 +390,10 @@ struct Work {
 // whole number, more than the roundings move it.
 __device__ __forceinline__ int small_div(int x, float inv) { return (int)(((float)x + 0.5f) * inv); }
 
-template <int DP, int CTAS>
-__global__ void __launch_bounds__(Cfg<DP, CTAS>::kThreads, CTAS) attention_prompt_kernel(const PromptArgs a) {
+// WITHHOLD: a test hook, the copies of the keys of tile `withheld` are never made.
+template <int DP, int CTAS, bool WITHHOLD>
+__global__ void __launch_bounds__(Cfg<DP, CTAS>::kThreads, CTAS)
+    attention_prompt_kernel(const PromptArgs a, const int withheld) {
   using C = Cfg<DP, CTAS>;
   constexpr int ST = C::kStages, NB = C::kBufs, kSoftWarps = C::kSoftWarps;
   constexpr int P = C::kParts, kShare = 32 * P;  // threads that share 32 rows
@@ -487,8 +490,10 @@ __global__ void __launch_bounds__(Cfg<DP, CTAS>::kThreads, CTAS) attention_promp
           const int st = nk % ST;
           unsigned char* dst = smem + st * C::kImage;
           if (nk >= ST && !wait(&kempty[st], nk / ST - 1)) break;
-          tc::bar_expect_tx(&kfull[st], C::kOperand);
-          bulk_load(dst, src, C::kOperand, &kfull[st]);
+          if (!WITHHOLD || x.it.key_tiles + j != withheld) {
+            tc::bar_expect_tx(&kfull[st], C::kOperand);
+            bulk_load(dst, src, C::kOperand, &kfull[st]);
+          }
           ++nk;
           if (nv >= ST && !wait(&vempty[st], nv / ST - 1)) break;
           tc::bar_expect_tx(&vfull[st], C::kOperand);
@@ -866,22 +871,22 @@ int64_t most_tiles(int n_tokens, int n_seqs) {
   return t < n_tokens ? t : n_tokens;
 }
 
-template <int DP, int CTAS>
-cudaError_t launch_items(const PromptArgs& a, cudaStream_t st) {
+template <int DP, int CTAS, bool WITHHOLD>
+cudaError_t launch_items(const PromptArgs& a, int withheld, cudaStream_t st) {
   using C = Cfg<DP, CTAS>;
   static DeviceOnce once;
   const cudaError_t e = once.run([] {
-    return cudaFuncSetAttribute(attention_prompt_kernel<DP, CTAS>,
+    return cudaFuncSetAttribute(attention_prompt_kernel<DP, CTAS, WITHHOLD>,
                                 cudaFuncAttributeMaxDynamicSharedMemorySize, C::kSmem);
   });
   if (e != cudaSuccess) return e;
   const int64_t items = (int64_t)a.max_items * a.n_kv_heads, most = (int64_t)CTAS * sm_count();
-  return launch(attention_prompt_kernel<DP, CTAS>, dim3((unsigned)(items < most ? items : most)),
-                dim3(C::kThreads), C::kSmem, st, use_pdl(), a);
+  return launch(attention_prompt_kernel<DP, CTAS, WITHHOLD>, dim3((unsigned)(items < most ? items : most)),
+                dim3(C::kThreads), C::kSmem, st, use_pdl(), a, withheld);
 }
 
-template <int DP>
-cudaError_t launch_prompt(const PromptArgs& a, cudaStream_t st) {
+template <int DP, bool WITHHOLD>
+cudaError_t launch_prompt(const PromptArgs& a, int withheld, cudaStream_t st) {
   const cudaError_t e = launch(prompt_split_kernel<DP>, dim3(a.max_tiles + 1, 2 * a.n_kv_heads),
                                dim3(kSplitThreads), 0, st, false, a);
   if (e != cudaSuccess) return e;
@@ -892,8 +897,8 @@ cudaError_t launch_prompt(const PromptArgs& a, cudaStream_t st) {
   // 316 / 292 (28), 148 x 64 of 8 / 8 58 / 53 (12); short prompts lose by one also
   // with few items (148 x 16 of 14 / 2 28.0 / 26.4).
   if constexpr (DP == 64)
-    if ((int64_t)a.max_items * a.n_kv_heads > 4 * sm_count()) return launch_items<DP, 2>(a, st);
-  return launch_items<DP, 1>(a, st);
+    if ((int64_t)a.max_items * a.n_kv_heads > 4 * sm_count()) return launch_items<DP, 2, WITHHOLD>(a, withheld, st);
+  return launch_items<DP, 1, WITHHOLD>(a, withheld, st);
 }
 
 bool prompt_shape_ok(int n_heads, int n_kv_heads, int head_dim) {
@@ -937,11 +942,12 @@ extern "C" size_t dqmk_attention_prompt_workspace(int n_tokens, int n_seqs, int 
          meta_bytes(tiles, n_kv_heads) + (size_t)tiles * n_kv_heads * image;
 }
 
-extern "C" int dqmk_attention_prompt(const float* q, int64_t ldq, const float* k, int64_t ldk,
-                                     const float* v, int64_t ldv, const int* starts, int n_seqs,
-                                     int n_tokens, int n_heads, int n_kv_heads, int head_dim,
-                                     float* out, int64_t ldo, void* workspace,
-                                     size_t workspace_bytes, void* stream) {
+namespace {
+
+int prompt_call(const float* q, int64_t ldq, const float* k, int64_t ldk, const float* v, int64_t ldv,
+                const int* starts, int n_seqs, int n_tokens, int n_heads, int n_kv_heads, int head_dim,
+                float* out, int64_t ldo, void* workspace, size_t workspace_bytes, int withheld,
+                void* stream) {
   const std::string api = "AttentionPrompt";
   if (n_tokens < 0 || n_seqs < 0) return fail(DQMK_ERR_INVALID, api + ": counts must not be negative");
   if (!prompt_shape_ok(n_heads, n_kv_heads, head_dim))
@@ -984,7 +990,29 @@ extern "C" int dqmk_attention_prompt(const float* q, int64_t ldq, const float* k
   a.meta = reinterpret_cast<float4*>(work);
   a.images = work + meta_bytes(a.max_tiles, n_kv_heads);
   cudaStream_t st = static_cast<cudaStream_t>(stream);
-  DQMK_CUDA_RET(api.c_str(), head_dim > 64 ? launch_prompt<128>(a, st)
-                                           : launch_prompt<64>(a, st));
+  auto run = [&](auto hook) {
+    constexpr bool W = decltype(hook)::value;
+    return head_dim > 64 ? launch_prompt<128, W>(a, withheld, st) : launch_prompt<64, W>(a, withheld, st);
+  };
+  DQMK_CUDA_RET(api.c_str(), withheld < 0 ? run(std::false_type()) : run(std::true_type()));
   return DQMK_OK;
+}
+
+}  // namespace
+
+extern "C" int dqmk_attention_prompt(const float* q, int64_t ldq, const float* k, int64_t ldk,
+                                     const float* v, int64_t ldv, const int* starts, int n_seqs,
+                                     int n_tokens, int n_heads, int n_kv_heads, int head_dim,
+                                     float* out, int64_t ldo, void* workspace,
+                                     size_t workspace_bytes, void* stream) {
+  return prompt_call(q, ldq, k, ldk, v, ldv, starts, n_seqs, n_tokens, n_heads, n_kv_heads, head_dim,
+                     out, ldo, workspace, workspace_bytes, -1, stream);
+}
+
+extern "C" int dqmk_attention_prompt_withhold_tile(
+    const float* q, int64_t ldq, const float* k, int64_t ldk, const float* v, int64_t ldv,
+    const int* starts, int n_seqs, int n_tokens, int n_heads, int n_kv_heads, int head_dim, float* out,
+    int64_t ldo, void* workspace, size_t workspace_bytes, int tile, void* stream) {
+  return prompt_call(q, ldq, k, ldk, v, ldv, starts, n_seqs, n_tokens, n_heads, n_kv_heads, head_dim,
+                     out, ldo, workspace, workspace_bytes, tile, stream);
 }

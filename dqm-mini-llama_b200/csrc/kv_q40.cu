@@ -17,6 +17,7 @@
 //           bytes 2g, 2g+1 of the block; the 8 parts g of row pair r are turned
 //           by 2r, so that 4 pairs lie in different shared-memory banks
 #include <climits>
+#include <type_traits>
 
 #include "common.cuh"
 #include "internal.h"

@@ -340,6 +340,18 @@ int dqmk_attention_prompt(const float* q_dev, int64_t ldq, const float* k_dev, i
                           int n_tokens, int n_heads, int n_kv_heads, int head_dim, float* out_dev,
                           int64_t ldo, void* workspace_dev, size_t workspace_bytes, void* stream);
 
+/* Test hook for the bounded waits: dqmk_attention_prompt with the copies of the
+ * keys of tile `tile` withheld (64 tokens a tile, each sequence's from its first
+ * token on, all sequences' in a row), so that the waits for it run out (about a
+ * second) and the device error flag is set.  Rows (token, head) that a stopped
+ * CTA held are left as they were; every other row is what it is without. */
+int dqmk_attention_prompt_withhold_tile(const float* q_dev, int64_t ldq, const float* k_dev,
+                                        int64_t ldk, const float* v_dev, int64_t ldv,
+                                        const int* starts_dev, int n_seqs, int n_tokens, int n_heads,
+                                        int n_kv_heads, int head_dim, float* out_dev, int64_t ldo,
+                                        void* workspace_dev, size_t workspace_bytes, int tile,
+                                        void* stream);
+
 /* A KV cache held as Q4_0 blocks: n_slots independent sequences of up to
  * max_seq positions for each of n_layers layers.  keys_dev and values_dev are
  * device buffers of dqmk_kv_q40_bytes each (below 2^62; 16-byte aligned, contents opaque;

@@ -57,3 +57,6 @@ def test_withheld_copies_refusals(pkg):
     for layer, heads, text in ((2, 4, "layer out of range"), (1, 3, "invalid head configuration")):
         with pytest.raises(RuntimeError if heads == 3 else pkg.OutOfRange, match=text):
             pkg.check(call(C.byref(kv), layer, p, 256, p, p, 5, heads, p, 256, p, 1 << 30, 0, 0, None))
+    prompt = pkg.lib().dqmk_attention_prompt_withhold_tile
+    with pytest.raises(RuntimeError, match="AttentionPrompt: invalid head configuration"):
+        pkg.check(prompt(p, 256, p, 128, p, 128, p, 2, 10, 5, 2, 64, p, 256, p, 1 << 30, 0, None))

@@ -61,3 +61,53 @@ def test_cache_attention_wait_runs_out(pkg, cuda, lengths, column, tile, fill):
     assert int(same.sum()) >= n * h - (h if n == 3 else 60 * h)
     assert torch.equal(cache.attention(q, 0, lens), want)
     assert L.dqmk_device_error(0) == 0
+
+
+# one item a CTA; many items a CTA, two CTAs an SM; many items of the 128-wide build
+PROMPTS = [((14, 2, 64), [600, 300, 64, 5], 12, 0), ((8, 8, 64), [64] * 400, 5, 3),
+           ((28, 4, 128), [200] * 40, 4 * 7 + 2, 3)]
+
+
+@pytest.mark.parametrize("heads,lengths,tile,ahead", PROMPTS, ids=["one", "many", "wide"])
+@pytest.mark.parametrize("fill", [0x7f7f7f7f, -3])
+def test_attention_prompt_wait_runs_out(pkg, cuda, heads, lengths, tile, ahead, fill):
+    torch = cuda
+    L = pkg.lib()
+    h, kv, d = heads
+    g = torch.Generator(device="cuda").manual_seed(6)
+    starts = [0]
+    for x in lengths:
+        starts.append(starts[-1] + x)
+    n = starts[-1]
+    q, k, v = (torch.randn(n, x, d, generator=g, device="cuda") for x in (h, kv, kv))
+    st = torch.tensor(starts, dtype=torch.int32, device="cuda")
+    want = pkg.attention_prompt(q, k, v, st)
+    assert L.dqmk_device_error(1) == 0
+    out = torch.full_like(q, 7.0)
+    size = L.dqmk_attention_prompt_workspace(n, len(lengths), h, kv, d)
+    work = torch.full((size // 4,), fill, dtype=torch.int32, device="cuda")
+    torch.cuda.synchronize()
+    t0 = time.time()
+    pkg.check(L.dqmk_attention_prompt_withhold_tile(
+        q.data_ptr(), h * d, k.data_ptr(), kv * d, v.data_ptr(), kv * d, st.data_ptr(), len(lengths), n,
+        h, kv, d, out.data_ptr(), h * d, work.data_ptr(), size, tile,
+        torch.cuda.current_stream().cuda_stream))
+    torch.cuda.synchronize()
+    assert time.time() - t0 < 30
+    assert L.dqmk_device_error(1) == 1
+    same, kept = (out == want).all(-1), (out == 7.0).all(-1)
+    assert bool((same | kept).all())
+    # tokens of the withheld tile, and those behind it in its sequence
+    s, first = 0, tile
+    while first >= -(-lengths[s] // 64):
+        first -= -(-lengths[s] // 64)
+        s += 1
+    assert bool(kept[starts[s] + 64 * first:starts[s + 1]].all())
+    # a CTA that stops loses its item and those that it had taken ahead
+    items = kv * (-(-lengths[s] * (h // kv) // 128))
+    assert int(kept.sum()) <= items * (1 + ahead) * 128
+    if not ahead:
+        assert bool(same[:starts[s]].all() and same[starts[s + 1]:].all())
+        assert bool(same[starts[s]:starts[s] + 64 * first - 128 * kv // h - 1].all())
+    assert torch.equal(pkg.attention_prompt(q, k, v, st), want)
+    assert L.dqmk_device_error(0) == 0

@@ -892,10 +892,12 @@ cudaError_t launch_prompt(const PromptArgs& a, int withheld, cudaStream_t st) {
   if (e != cudaSuccess) return e;
   // At 64 two CTAs fit an SM, with 96 registers each for 168.  Two hide an item's
   // ends, one is faster while a CTA has few items, the longest of which ends last.
-  // One / two, us, items an SM: 1 x 4096 tokens of 14 / 2 heads 120 / 145 (3.0),
-  // 1 x 8192 of 8 / 8 257 / 301 (3.5); 1 x 8192 of 14 / 2 401 / 390 (6), 37 x 1024
-  // 316 / 292 (28), 148 x 64 of 8 / 8 58 / 53 (12); short prompts lose by one also
-  // with few items (148 x 16 of 14 / 2 28.0 / 26.4).
+  // One / two, us, items an SM: 1 x 4096 tokens of 14 / 2 heads 120 / 133 (3.0), 1 x
+  // 5120 176 / 180 (3.8), 1 x 8192 of 8 / 8 263 / 315 (3.5), 1 x 10240 392 / 398 (4.3);
+  // 1 x 6144 of 14 / 2 239 / 234 (4.5), 1 x 8192 403 / 390 (6), 1 x 12288 of 8 / 8 550 /
+  // 537 (5.2), 12 x 1024 of 14 / 2 115 / 110 (4.5), 37 x 1024 320 / 300 (14).  Packs of
+  // short prompts lose by two: 148 x 64 of 14 / 2 49.5 / 52 (8), 300 x 16 52 / 55.5 (4);
+  // the host does not know the lengths.
   if constexpr (DP == 64)
     if ((int64_t)a.max_items * a.n_kv_heads > 4 * sm_count()) return launch_items<DP, 2, WITHHOLD>(a, withheld, st);
   return launch_items<DP, 1, WITHHOLD>(a, withheld, st);

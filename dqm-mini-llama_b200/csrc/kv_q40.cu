@@ -904,11 +904,15 @@ cudaError_t launch_attention_q40(const AttnQ40Args& args, int n_ctas, int2 withh
   e = launch(kv_q40_attention_kernel<NB, WITHHOLD>, dim3(n_ctas), dim3(kThreads),
              attention_smem<NB>(), st, false, args, withheld);
   if (e != cudaSuccess || !join) return e;
-  // One / 8 heads a CTA of the join, us of both kernels, 28 / 4 heads of 128: 4
-  // groups of 32768 positions 14.5 / 41.7, 32 of 8192 22.1 / 23.0, 48 28.5 / 28.5,
-  // 64 34.4 / 31.7, 256 of 1024 41.5 / 23.0
+  // One head a CTA of the join where a group has many partial sums, 8 where there are
+  // many groups.  Us of both kernels, one / 8, and partial sums a group, 28 / 4 heads
+  // of 128: 1 column of 32768 14.5 / 36.5 (111), 1 of 4096 9.0 / 15.3 (32), 8 of 8192
+  // 22.3 / 22.4 (14), 12 of 8192 28.4 / 27.3 (9), 8 of 1024 13.1 / 11.8 (8), 64 of 1024
+  // 41.0 / 22.1 (2); 14 / 2 of 64: 16 of 8192 17.1 / 16.8 (14), 24 of 2048 12.8 / 11.8
+  // (9), 8 of 1024 8.2 / 8.5 (8); 40 / 8 of 128: 4 of 8192 20.9 / 21.7 (14); 5 / 1 of
+  // 64: 16 of 8192 10.8 / 16.0 (28).
   const unsigned groups = (unsigned)(args.n_cols * args.subs);
-  if (groups < 64)
+  if ((unsigned)n_ctas / 12 >= groups)
     return launch(kv_q40_join_kernel<NB, 1>, dim3(groups, kGroup), dim3(1024), 0, st, use_pdl(),
                   args, n_ctas);
   return launch(kv_q40_join_kernel<NB, kGroup>, dim3(groups), dim3(512), 0, st, use_pdl(), args,

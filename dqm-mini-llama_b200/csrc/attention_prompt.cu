@@ -122,25 +122,6 @@ __device__ __forceinline__ int item_tiles(const PromptArgs& a, int n, int row) {
   return (int)(last / a.group) / kKeys + 1;
 }
 
-// Byte offset of 16-byte chunk c (8 fp16) of row r in a 128-byte-swizzled
-// K-major operand tile (8-row atoms of 1024 bytes).
-__device__ __forceinline__ uint32_t sw128(int r, int c) {
-  return (uint32_t)((r >> 3) * 1024 + (r & 7) * 128 + ((c ^ (r & 7)) << 4));
-}
-__device__ __forceinline__ float pow2f(int e) { return __int_as_float((127 + e) << 23); }
-// e such that top 2^-e lies in [2^14, 2^15); 0 for 0.
-__device__ __forceinline__ int pow2_ex(float top) {
-  const int fe = ((__float_as_int(top) >> 23) & 0xff) - 126;
-  return top > 0.0f ? min(max(fe - 15, -120), 120) : 0;
-}
-// Two values to packed fp16 pairs with x = hi + lo + r, |r| <= 2^-22 |x| or 2^-25.
-__device__ __forceinline__ void split2(float x0, float x1, uint32_t& hi, uint32_t& lo) {
-  const __half2 h = __floats2half2_rn(x0, x1);
-  const float2 back = __half22float2(h);
-  const __half2 l = __floats2half2_rn(__fsub_rn(x0, back.x), __fsub_rn(x1, back.y));
-  hi = *reinterpret_cast<const uint32_t*>(&h);
-  lo = *reinterpret_cast<const uint32_t*>(&l);
-}
 
 // ------------------------------------------------------------ first kernel
 constexpr int kSplitThreads = 256;
@@ -301,7 +282,7 @@ __global__ void __launch_bounds__(kSplitThreads) prompt_split_kernel(const Promp
       split2(x[i].x, x[i].y, hi.x, lo.x);
       split2(x[i].z, x[i].w, hi.y, lo.y);
       // columns 64 h ..: plane half h, 8-byte half (c4 & 1) of chunk (c4 % 16) / 2
-      unsigned char* dst = image + (c4 / 16) * (kKeys * 128) + sw128(r, (c4 % 16) >> 1) + (c4 & 1) * 8;
+      unsigned char* dst = image + (c4 / 16) * (kKeys * 128) + tc::sw128(r, (c4 % 16) >> 1) + (c4 & 1) * 8;
       *reinterpret_cast<uint2*>(dst) = hi;
       *reinterpret_cast<uint2*>(dst + C::kPlane) = lo;
     }
@@ -321,7 +302,7 @@ __global__ void __launch_bounds__(kSplitThreads) prompt_split_kernel(const Promp
       split2(vt[8 * c + 2][d], vt[8 * c + 3][d], hi.y, lo.y);
       split2(vt[8 * c + 4][d], vt[8 * c + 5][d], hi.z, lo.z);
       split2(vt[8 * c + 6][d], vt[8 * c + 7][d], hi.w, lo.w);
-      unsigned char* dst = image + sw128(d, c);
+      unsigned char* dst = image + tc::sw128(d, c);
       *reinterpret_cast<uint4*>(dst) = hi;
       *reinterpret_cast<uint4*>(dst + C::kPlane) = lo;
     }
@@ -331,13 +312,6 @@ __global__ void __launch_bounds__(kSplitThreads) prompt_split_kernel(const Promp
 }
 
 // ------------------------------------------------------------ second kernel
-__device__ __forceinline__ void bulk_load(void* dst, const void* src, uint32_t bytes, uint64_t* bar) {
-  asm volatile(
-      "cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(
-          tc::su32(dst)),
-      "l"(src), "r"(bytes), "r"(tc::su32(bar))
-      : "memory");
-}
 __device__ __forceinline__ void bulk_store(void* dst, const void* src, uint32_t bytes) {
   asm volatile("cp.async.bulk.global.shared::cta.bulk_group [%0], [%1], %2;" ::"l"(dst),
                "r"(tc::su32(src)), "r"(bytes)
@@ -373,12 +347,6 @@ __device__ __forceinline__ void tmem_st8(uint32_t taddr, const uint32_t (&r)[8])
 __device__ __forceinline__ void tmem_st_rows16(uint32_t taddr, const uint32_t (&r)[4]) {
   asm volatile("tcgen05.st.sync.aligned.16x256b.x1.b32 [%0], {%1,%2,%3,%4};" ::"r"(taddr), "r"(r[0]),
                "r"(r[1]), "r"(r[2]), "r"(r[3]));
-}
-// 2^x; results below 2^-126 are 0.
-__device__ __forceinline__ float ex2(float x) {
-  float y;
-  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
-  return y;
 }
 
 // An item as the roles of a CTA see it; kvh < 0: no more.
@@ -492,12 +460,12 @@ __global__ void __launch_bounds__(Cfg<DP, CTAS>::kThreads, CTAS)
           if (nk >= ST && !wait(&kempty[st], nk / ST - 1)) break;
           if (!WITHHOLD || x.it.key_tiles + j != withheld) {
             tc::bar_expect_tx(&kfull[st], C::kOperand);
-            bulk_load(dst, src, C::kOperand, &kfull[st]);
+            tc::bulk_load(dst, src, C::kOperand, &kfull[st]);
           }
           ++nk;
           if (nv >= ST && !wait(&vempty[st], nv / ST - 1)) break;
           tc::bar_expect_tx(&vfull[st], C::kOperand);
-          bulk_load(dst + C::kOperand, src + C::kOperand, C::kOperand, &vfull[st]);
+          tc::bulk_load(dst + C::kOperand, src + C::kOperand, C::kOperand, &vfull[st]);
           ++nv;
         }
       }

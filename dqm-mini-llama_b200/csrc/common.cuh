@@ -130,6 +130,34 @@ __device__ __forceinline__ float warp_max(float v) {
   return v;
 }
 
+// 2^e for -126 <= e <= 127.
+__device__ __forceinline__ float pow2f(int e) { return __int_as_float((127 + e) << 23); }
+// e such that x 2^-e lies in [2^14, 2^15) for a normal x > 0, from its exponent
+// field; 0 for 0; held to [-120, 120].
+__device__ __forceinline__ int pow2_ex(float x) {
+  const int fe = ((__float_as_int(x) >> 23) & 0xff) - 126;
+  return x > 0.0f ? min(max(fe - 15, -120), 120) : 0;
+}
+// 2^x; results below 2^-126 are 0.
+__device__ __forceinline__ float ex2(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+// Two values to packed fp16 pairs with x = hi + lo + r, |r| <= 2^-22 |x|, or 2^-25
+// where lo is subnormal.
+__device__ __forceinline__ void split2(float x0, float x1, __half2& hi, __half2& lo) {
+  hi = __floats2half2_rn(x0, x1);
+  const float2 back = __half22float2(hi);
+  lo = __floats2half2_rn(__fsub_rn(x0, back.x), __fsub_rn(x1, back.y));
+}
+__device__ __forceinline__ void split2(float x0, float x1, uint32_t& hi, uint32_t& lo) {
+  __half2 h, l;
+  split2(x0, x1, h, l);
+  hi = *reinterpret_cast<const uint32_t*>(&h);
+  lo = *reinterpret_cast<const uint32_t*>(&l);
+}
+
 // Sum of `x` over the CTA's threads, and in *before the sum over the threads
 // before this one; warp_sums: shared memory, one entry a warp.  All threads call.
 __device__ __forceinline__ int64_t block_scan(int64_t x, int64_t* before, int64_t* warp_sums) {

@@ -330,21 +330,8 @@ __device__ __forceinline__ void mma16816_first(float (&d)[4], const uint4& a, ui
       : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3])
       : "r"(a.x), "r"(a.y), "r"(a.z), "r"(a.w), "r"(b0), "r"(b1), "f"(0.0f));
 }
-__device__ __forceinline__ void bulk_load(void* dst, const void* src, uint32_t bytes, uint64_t* bar) {
-  asm volatile(
-      "cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(
-          tc::su32(dst)),
-      "l"(src), "r"(bytes), "r"(tc::su32(bar))
-      : "memory");
-}
 __device__ __forceinline__ __half2 as_h2(uint32_t x) { return *reinterpret_cast<const __half2*>(&x); }
 __device__ __forceinline__ uint32_t bits(__half2 x) { return *reinterpret_cast<const uint32_t*>(&x); }
-// Two values to packed fp16 pairs with x = hi + lo + r, |r| <= 2^-22 |x|.
-__device__ __forceinline__ void split2(float x0, float x1, __half2& hi, __half2& lo) {
-  hi = __floats2half2_rn(x0, x1);
-  const float2 back = __half22float2(hi);
-  lo = __floats2half2_rn(__fsub_rn(x0, back.x), __fsub_rn(x1, back.y));
-}
 template <uint32_t MASK>
 __device__ __forceinline__ uint32_t and_or(uint32_t w, uint32_t with) {
   uint32_t r;
@@ -357,16 +344,9 @@ __device__ __forceinline__ uint32_t codes_low(uint32_t w) {
 __device__ __forceinline__ uint32_t codes_high(uint32_t w) {
   return bits(__hadd2(as_h2(and_or<0x00f000f0u>(w, 0x64006400u)), as_h2(0xe480e480u)));  // -1152
 }
-__device__ __forceinline__ float pow2f(int e) { return __int_as_float((127 + e) << 23); }
 // V's scales that are all below 2^kSmall are raised by this power of two.
 constexpr int kSmall = -6;
 __device__ __forceinline__ int small_scales(int ev) { return max(0, kSmall - ev); }
-// 2^x; results below 2^-126 are 0.
-__device__ __forceinline__ float ex2(float x) {
-  float y;
-  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
-  return y;
-}
 
 template <int N>
 __device__ __forceinline__ void lds_words(uint32_t (&r)[N], const void* p) {
@@ -501,8 +481,8 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm)
       if (x.col == withheld.x && first_of(x) + i * kWarps == withheld.y) return;
     const int64_t at = (first_tile(a.c, x.slot, x.sub % a.c.n_kv_heads) + first_of(x) + i * kWarps) * S::kTileBytes;
     tc::bar_expect_tx(bar, S::kStageBytes);
-    bulk_load(st, a.c.k + at, S::kTileBytes, bar);
-    bulk_load(st + S::kTileBytes, a.c.v + at, S::kTileBytes, bar);
+    tc::bulk_load(st, a.c.k + at, S::kTileBytes, bar);
+    tc::bulk_load(st + S::kTileBytes, a.c.v + at, S::kTileBytes, bar);
   };
   auto start = [&](const Piece& x) {  // its first tiles
     for (int i = 0; i < min(tiles_mine(x), kStages); ++i) {

@@ -866,30 +866,6 @@ __host__ __device__ inline void split_plan(int nt, int target, int* per, int* sp
   *splits = (nt + *per - 1) / *per;
 }
 
-// Byte offset of 16-byte chunk c (8 fp16) of row r in a 128-byte-swizzled
-// K-major operand tile (8-row atoms of 1024 bytes).
-__device__ __forceinline__ uint32_t sw128(int r, int c) {
-  return (uint32_t)((r >> 3) * 1024 + (r & 7) * 128 + ((c ^ (r & 7)) << 4));
-}
-// ex such that mx 2^-ex lies in [2^14, 2^15) for a normal mx > 0, read from
-// the exponent field (mx in [2^(fe-1), 2^fe)); 0 for mx == 0; clamped to
-// [-120, 120].
-__device__ __forceinline__ int pow2_ex(float mx) {
-  const int fe = ((__float_as_int(mx) >> 23) & 0xff) - 126;
-  return mx > 0.0f ? min(max(fe - 15, -120), 120) : 0;
-}
-// 2^e for |e| <= 126, built from its exponent field.
-__device__ __forceinline__ float pow2f(int e) { return __int_as_float((127 + e) << 23); }
-// Two values to packed fp16 pairs hi and lo with x = hi + lo + r,
-// |r| <= 2^-22 |x| (element 0 in the low half).
-__device__ __forceinline__ void split2(float x0, float x1, uint32_t& hi, uint32_t& lo) {
-  const __half2 h = __floats2half2_rn(x0, x1);
-  const float2 back = __half22float2(h);
-  const __half2 l = __floats2half2_rn(__fsub_rn(x0, back.x), __fsub_rn(x1, back.y));
-  hi = *reinterpret_cast<const uint32_t*>(&h);
-  lo = *reinterpret_cast<const uint32_t*>(&l);
-}
-
 // One 64-position tile of K and V (positions kt.., zero past `last`) into a
 // shared-memory buffer, with the per-position K scales 2^ek (sk) and the
 // per-dimension V scales 2^ev (sv); 256 threads.
@@ -926,7 +902,7 @@ __device__ __forceinline__ void load_tile(const float* kbase, const float* vbase
       uint2 hi, lo;
       split2(__fmul_rn(v[i].x, down), __fmul_rn(v[i].y, down), hi.x, lo.x);
       split2(__fmul_rn(v[i].z, down), __fmul_rn(v[i].w, down), hi.y, lo.y);
-      const uint32_t off = sw128(j, 2 * i + (p >> 1)) + (uint32_t)(p & 1) * 8;
+      const uint32_t off = tc::sw128(j, 2 * i + (p >> 1)) + (uint32_t)(p & 1) * 8;
       *reinterpret_cast<uint2*>(buf + off) = hi;
       *reinterpret_cast<uint2*>(buf + kPlane + off) = lo;
     }
@@ -968,7 +944,7 @@ __device__ __forceinline__ void load_tile(const float* kbase, const float* vbase
       uint2 hi, lo;
       split2(x[0], x[1], hi.x, lo.x);
       split2(x[2], x[3], hi.y, lo.y);
-      const uint32_t off = sw128(4 * dg + e, pg >> 1) + (uint32_t)(pg & 1) * 8;
+      const uint32_t off = tc::sw128(4 * dg + e, pg >> 1) + (uint32_t)(pg & 1) * 8;
       *reinterpret_cast<uint2*>(buf + 2 * kPlane + off) = hi;
       *reinterpret_cast<uint2*>(buf + 3 * kPlane + off) = lo;
     }

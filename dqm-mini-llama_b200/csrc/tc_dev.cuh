@@ -92,6 +92,14 @@ __device__ __forceinline__ void tma_load_2d_hint(void* dst, const CUtensorMap* m
       "l"(reinterpret_cast<uint64_t>(map)), "r"(x), "r"(y), "r"(su32(bar)), "l"(policy)
       : "memory");
 }
+// `bytes` contiguous bytes (a multiple of 16, both sides 16-byte aligned), counted at `bar`.
+__device__ __forceinline__ void bulk_load(void* dst, const void* src, uint32_t bytes, uint64_t* bar) {
+  asm volatile(
+      "cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(
+          su32(dst)),
+      "l"(src), "r"(bytes), "r"(su32(bar))
+      : "memory");
+}
 __device__ __forceinline__ void tma_prefetch_desc(const CUtensorMap* map) {
   asm volatile("prefetch.tensormap [%0];" ::"l"(reinterpret_cast<uint64_t>(map)) : "memory");
 }
@@ -102,6 +110,11 @@ __device__ __forceinline__ void fence_proxy_async_smem() {
   asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
 }
 
+// Byte offset of 16-byte chunk c (8 fp16) of row r in a 128-byte-swizzled
+// K-major operand tile (8-row atoms of 1024 bytes).
+__device__ __forceinline__ uint32_t sw128(int r, int c) {
+  return (uint32_t)((r >> 3) * 1024 + (r & 7) * 128 + ((c ^ (r & 7)) << 4));
+}
 // K-major operand in a 128-byte-swizzled tile: rows of 128 bytes, 8-row atoms
 // 1024 bytes apart (stride byte offset), version 1 (sm_100), layout
 // SWIZZLE_128B.  The start address moves by 32 bytes per K=16 fp16 slice.

@@ -1073,6 +1073,7 @@ int attention_call(const char* name, const dqmk_kv_q40* kv, int layer, const flo
     return fail(DQMK_ERR_INVALID, api + ": workspace must be 16-byte aligned");
   a.group = n_heads / kv->n_kv_heads;
   const int64_t subs = (int64_t)kv->n_kv_heads * ((a.group + kGroup - 1) / kGroup);
+  if (width > INT_MAX - kThreads) return fail(DQMK_ERR_UNSUPPORTED, api + ": too many heads");
   if (subs * n_cols > INT_MAX) return fail(DQMK_ERR_UNSUPPORTED, api + ": too many columns");
   a.subs = (int)subs;
   const size_t need = workspace_need(n_cols, a.subs, kv->max_seq, kv->head_dim);

@@ -24,6 +24,7 @@ namespace dqmk {
 namespace {
 
 constexpr int kMaxHalf = 128;
+constexpr int kMaxRows = 1 << 30;  // rows of a token are counted in 32 bits
 constexpr int kThreads = 128;  // 84 us for 16384 tokens of 32 heads of 128, 88 with 256
 
 struct NormRopeArgs {
@@ -159,6 +160,7 @@ extern "C" int dqmk_qk_norm_rope(const float* q, int64_t ldq, const float* k, in
   const std::string api = "QkNormRope";
   if (n_tokens < 0 || n_heads < 0 || n_kv_heads < 0)
     return fail(DQMK_ERR_INVALID, api + ": counts must not be negative");
+  if ((int64_t)n_heads + n_kv_heads > kMaxRows) return fail(DQMK_ERR_UNSUPPORTED, api + ": too many heads");
   if (head_dim <= 0 || head_dim % 2 != 0)
     return fail(DQMK_ERR_INVALID, api + ": head_dim must be positive and even");
   if (head_dim / 2 > kMaxHalf) return fail(DQMK_ERR_UNSUPPORTED, api + ": head_dim larger than 256");

@@ -49,6 +49,20 @@ def test_spans_name_the_ctas_that_hold_a_group(grid, seed):
         assert [lo == 0 for _, lo, _ in mine] == [cta == x for cta, _, _ in mine]
 
 
+def test_rows_past_32_bits_are_refused(pkg):
+    """Rows whose heads or elements are counted past 31 bits."""
+    from importlib import import_module
+    L, p = pkg.lib(), C.c_void_p(64)
+    big = 1 << 30
+    with pytest.raises(RuntimeError, match="QkNormRope: too many heads"):
+        pkg.check(L.dqmk_qk_norm_rope(p, 2 * big, p, 2 * big, 1, big, big, 2, p, p, 1e-6, p, 1e6, 1, p,
+                                      2 * big, p, 2 * big, None))
+    kv = import_module(pkg.__name__ + "._lib").KvQ40(64, 128, 1, 1, 40, 1, 128)
+    with pytest.raises(RuntimeError, match="KvQ40Attention: too many heads"):
+        pkg.check(L.dqmk_kv_q40_attention(C.byref(kv), 0, p, 1 << 31, p, p, 1, 1 << 24, p, 1 << 31, p,
+                                          1 << 40, None))
+
+
 def test_withheld_copies_refusals(pkg):
     from importlib import import_module
     kv = import_module(pkg.__name__ + "._lib").KvQ40(64, 128, 2, 3, 40, 2, 64)

@@ -46,11 +46,13 @@
 // next one's first (with the list, 396 -> 260 us for 33 ragged prompts of 28 / 4
 // heads of 128; the queries under the last tiles 240 -> 233).
 //
-// Bound: the tensor cores, and an item's ends where it has few keys.  28 / 4 heads
-// of 128 on one B200: 8192 tokens 1072 us, 1346 TFLOP/s of fp16 products (80% of
-// the measured 1686; 1249 us at 1477 MHz in a run of seconds, at the power limit),
-// 33 ragged prompts 230 us; 602 tokens of 14 / 2 heads of 64 20 us.  A score product
-// of 64 keys takes 44.8 cycles, 32 by its operations; one of 128 its full 64.
+// Bound: a tile's products, 1840 cycles at 128 and 1075 at 64, and its softmax, which
+// they overlap in part (2670 and 1950 cycles a tile); an item's ends where it has few
+// keys.  28 / 4 heads of 128 on one B200, graphs of calls: 8192 tokens 1069 us, 1350
+// TFLOP/s of fp16 products (80% of the measured 1686; 1249 us at 1477 MHz in a run of
+// seconds, at the power limit), 33 ragged prompts 233 us (280 by a call on new inputs);
+// 602 tokens of 14 / 2 heads of 64 19.5 us.  A score product of 64 keys takes 44.8
+// cycles, 32 by its operations; one of 128 its full 64.
 #include <climits>
 #include <type_traits>
 

@@ -249,8 +249,8 @@ __global__ void __launch_bounds__(kRowThreads) kv_q40_read_kernel(const RowsArgs
 // where d is above 1) and d a power of two where it is below 2^-6.  The terms
 // of w come from p = ph + pl and d in fp16 arithmetic: hi = ph d, lo = (ph d -
 // hi) + pl d, whose first part a fused multiply-add leaves exact.  Terms end at
-// 2^-24, so a w that is small beside the largest (at least 2^8) is off by 2^-32 of
-// that one rather than by 2^-22 of itself.  Blocks' scales far apart (2^10) would
+// 2^-24, so a w that is small beside the largest p times the largest d (at least 2^8)
+// is off by 2^-32 of that rather than by 2^-22 of itself.  Blocks' scales far apart (2^10) would
 // need a power of two for each block; that was built and took 16 columns of 65536
 // positions from 167 to 170 us, for values that f32 rows seldom hold.
 //
@@ -264,10 +264,10 @@ __global__ void __launch_bounds__(kRowThreads) kv_q40_read_kernel(const RowsArgs
 // Bound: 18 bytes for 32 values, each used by every head of the group; at the
 // memory rate a scheduler has 3.1 lane slots a value of the cache, 1.5 for half2
 // and integer instructions, which issue at half rate, and f32 arithmetic adds its
-// time to the products'.  So it is bound by its instructions: 168 us for 16 columns
+// time to the products'.  So it is bound by its instructions: 167 us for 16 columns
 // of 65536 positions, 28 / 4 heads of 128 (3.6 TB/s, 56% of the measured copy rate;
 // 180 us at 1860 MHz in a run of seconds, at the power limit); 64 ragged columns up
-// to 2048 22 us, 1 x 32768 14.5 us.  3 CTAs an SM with 168 registers: 4 with 128 took
+// to 2048 21 us (23 with the cache not in L2), 1 x 32768 14.7 us (16).  3 CTAs an SM with 168 registers: 4 with 128 took
 // 184 us for 168.
 //
 // Work: the positions of all columns and heads form one list of units, kExtra
@@ -959,8 +959,8 @@ cudaError_t launch_rows(bool write, const RowsArgs& a, cudaStream_t st) {
 template <int NB>
 cudaError_t launch_rows(bool write, bool vec, const RowsArgs& a, cudaStream_t st) {
   // Several tokens a CTA once they fill the SMs.  Write and read, 4 heads of 128,
-  // one / several, us: 148 tokens 4.3 / 7.0, 888 6.3 / 7.3, 1184 7.7 / 7.8, 1480
-  // 9.3 / 8.6, 8191 32.5 / 21.0
+  // one / several, us, rows in L2: 148 tokens 4.3 / 7.0, 888 6.3 / 7.3, 1184 7.7 / 7.8,
+  // 1480 9.3 / 8.6, 8191 32.5 / 21.0 (29 with rows from memory)
   if (a.n_tokens >= 8 * sm_count())
     return vec ? launch_rows<NB, 8, true>(write, a, st) : launch_rows<NB, 8, false>(write, a, st);
   return vec ? launch_rows<NB, 1, true>(write, a, st) : launch_rows<NB, 1, false>(write, a, st);

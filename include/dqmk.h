@@ -396,7 +396,8 @@ int dqmk_kv_q40_read(const dqmk_kv_q40* kv, int layer, const int* slots_dev,
  * same for the same arguments every time.  They are those of f32 sums over the
  * cache's values with operands of 22 bits: a query is off by at most 2^-22 of itself
  * or 2^-35 of its head's largest, and a weight times a block's scale by 2^-22 or
- * 2^-32 of the column's largest such product (scales between 2^-14 and 2^7).
+ * 2^-32 of the row's largest weight times the column's largest scale of V (where
+ * that is between 2^-14 and 2^7).
  * More than 8 query heads to a KV head read the cache once for every 8.
  * workspace_dev: dqmk_kv_q40_attention_workspace
  * bytes, 16-byte aligned, contents ignored; calls that may overlap on the GPU

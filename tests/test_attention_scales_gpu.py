@@ -167,8 +167,9 @@ def cache_of(pkg, torch, k, v):
 def test_cache_attention_value_blocks_of_many_sizes(pkg, cuda, gen, heads, bits, size):  # noqa: F811
     """Blocks of the values that differ by up to 2^22, also where the large ones
     come late or in few rows.  Beside the bound of any attention here, a
-    product of a weight and a scale is off by 2^-32 of the largest of them, and
-    a value is up to 8 times its scale (its block's largest at least 7 times)."""
+    product of a weight and a scale is off by 2^-32 of the largest weight times the
+    largest scale, and a value is up to 8 times its scale (its block's largest at
+    least 7 times)."""
     torch = cuda
     h, kv, d = heads
     n = 1100
@@ -186,7 +187,7 @@ def test_cache_attention_value_blocks_of_many_sizes(pkg, cuda, gen, heads, bits,
             seen = torch.ones(1, length, dtype=torch.bool, device="cuda")
             ref, bound = attend(torch, q[0][:, None], kk, vv, seen)
             p = torch.softmax(q[0].double()[:, None] @ kk.transpose(-1, -2) / d ** 0.5, -1)
-            largest = (p[:, 0] * vv.abs().amax(-1) / 7).amax(-1)[:, None, None]
+            largest = p.amax(-1, keepdim=True) * vv.abs().amax((1, 2))[:, None, None] / 7
             check_close(out[0][:, None], ref, bound + 8 * length * 2.0 ** -32 * largest,
                         f"{bits} {size} {late} {length}")
 

@@ -74,3 +74,99 @@ def test_cache_rows_written_back_stay(pkg, cuda, gen, dim):  # noqa: F811
     b.write(0, *held, p, torch.zeros_like(p))
     for x, y in zip(held, b.read(0, p, torch.zeros_like(p))):
         assert torch.equal(x, y)
+
+
+def spread(torch, gen, n, bits):  # noqa: F811
+    return torch.exp2(-torch.rand(n, generator=gen, device="cuda") * bits)
+
+
+def off_by(torch, x):
+    """How far a key or value may be off: 2^-22 of itself or 2^-23 r c / t, the
+    largest of its row, its channel and its tile of 64 tokens."""
+    a = x.abs().double()
+    out = torch.zeros_like(a)
+    for t in range(0, x.shape[0], 64):
+        b = a[t:t + 64]
+        r, c, top = b.amax(2), b.amax(0), b.amax((0, 2)).clamp(min=1e-300)
+        out[t:t + 64] = torch.maximum(b * 2.0 ** -22, 2.0 ** -23 * r[:, :, None] * c[None] / top[None, :, None])
+    return out
+
+
+@pytest.mark.parametrize("seed", range(12))
+def test_attention_prompt_stated_bounds(pkg, cuda, seed):
+    """Rows and channels of random sizes on both sides of what marks a tile:
+    outputs within what follows from the errors stated for queries (2^-22, or
+    2^-34 of the row's largest), keys, values and weights (2^-22, or 2^-39 of the
+    row's largest), with f32 sums (6 e a term and addition, as in the tests of
+    the attention block) and 2^-22 of a score for its scaling and exponent."""
+    torch = cuda
+    gen = torch.Generator(device="cuda").manual_seed(seed)  # noqa: F811
+    h, kv, d = [(14, 2, 64), (6, 2, 128), (9, 1, 36), (5, 5, 100)][seed % 4]
+    lengths = [[200, 1, 33], [64, 65, 3, 130], [500]][seed % 3]
+    starts = [0]
+    for x in lengths:
+        starts.append(starts[-1] + x)
+    n = starts[-1]
+    size, channels = 2.0 ** (0, -12, 7, -40)[seed % 4], spread(torch, gen, d, (0, 7, 12)[seed % 3])
+    q = randn(torch, gen, n, h, d) * channels * size
+    k = randn(torch, gen, n, kv, d) / channels / size * spread(torch, gen, n, (0, 6, 20)[seed % 3])[:, None, None]
+    v = randn(torch, gen, n, kv, d) * spread(torch, gen, n, (3, 12, 25, 0)[seed % 4])[:, None, None]
+    v = v * spread(torch, gen, d, (9, 0, 5, 20, 3)[seed % 5])
+    k[n // 2] = 0
+    out = pkg.attention_prompt(q, k, v, i32(torch, starts))
+    e = 2.0 ** -24
+    for a, b in zip(starts[:-1], starts[1:]):
+        qs = q[a:b].double().permute(1, 0, 2)
+        ks, vs, dk, dv = (x.double().permute(1, 0, 2).repeat_interleave(h // kv, 0)
+                          for x in (k[a:b], v[a:b], off_by(torch, k[a:b]), off_by(torch, v[a:b])))
+        dq = torch.maximum(qs.abs() * 2.0 ** -22, 2.0 ** -34 * qs.abs().amax(-1, keepdim=True))
+        seen = torch.ones(b - a, b - a, dtype=torch.bool, device="cuda").tril()
+        root = d ** 0.5
+        s = qs @ ks.transpose(-1, -2) / root
+        ds = (qs.abs() @ dk.transpose(-1, -2) + dq @ ks.abs().transpose(-1, -2)
+              + (6 * d + 8) * e * (qs.abs() @ ks.abs().transpose(-1, -2))) / root + 4 * e * s.abs()
+        p = torch.softmax(s.masked_fill(~seen, -float("inf")), -1)
+        ds = ds.masked_fill(~seen, 0).amax(-1, keepdim=True)
+        bound = ((p @ vs.abs()) * (2 * torch.expm1(ds) + (16 + 6 * (b - a)) * e) + (p * torch.exp(ds)) @ dv
+                 + 2.0 ** -38 * p.amax(-1, keepdim=True) * (seen.double() @ vs.abs()))
+        off = (out[a:b].double().permute(1, 0, 2) - p @ vs).abs()
+        assert bool((off <= bound + 1e-37).all()), float((off / (bound + 1e-37)).max())
+
+
+@pytest.mark.parametrize("heads", [(14, 2, 64), (28, 4, 128)], ids=lambda h: "h%d_kv%d_d%d" % h)
+def test_attention_prompt_replayed_with_other_sequences(pkg, cuda, gen, heads):  # noqa: F811
+    """A captured call replayed with other offsets, rows and sizes in the same
+    memory, two graphs in turn on two streams: the bits of plain calls."""
+    torch = cuda
+    h, kv, d = heads
+    n = 400
+    q, k, v = (randn(torch, gen, n, x, d) for x in (h, kv, kv))
+    starts = i32(torch, [0, 100, 100, 350])
+    graphs = []
+    for _ in range(2):
+        pkg.attention_prompt(q, k, v, starts)
+        out = torch.zeros_like(q)
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g):
+            pkg.attention_prompt(q, k, v, starts, out=out)
+        graphs.append((g, out))
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    for offsets, far in (([0, 100, 100, 350], 0), ([0, 1, 2, 3], 0), ([7, 7, 7, 7], 0), ([0, 0, 0, 400], 1),
+                         ([2, 66, 131, 400], 2)):
+        starts.copy_(i32(torch, offsets))
+        k.copy_(randn(torch, gen, n, kv, d))
+        v.copy_(randn(torch, gen, n, kv, d))
+        if far:
+            (k if far == 1 else v)[100] *= 1e-9
+        want = pkg.attention_prompt(q, k, v, starts)
+        for _, out in graphs:
+            out.zero_()
+        torch.cuda.synchronize()
+        for (g, _), s in zip(graphs, streams):
+            with torch.cuda.stream(s):
+                g.replay()
+        torch.cuda.synchronize()
+        for _, out in graphs:
+            assert torch.equal(out, want)
+        check_prompt(torch, want, q, k, v, offsets)
+    assert pkg.lib().dqmk_device_error(0) == 0

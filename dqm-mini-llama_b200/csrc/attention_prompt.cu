@@ -124,7 +124,6 @@ __device__ __forceinline__ int item_tiles(const PromptArgs& a, int n, int row) {
   return (int)(last / a.group) / kKeys + 1;
 }
 
-
 // ------------------------------------------------------------ first kernel
 constexpr int kSplitThreads = 256;
 // Exponents from a tile's largest value to its smallest row's largest, and to its
@@ -267,7 +266,8 @@ __global__ void __launch_bounds__(kSplitThreads) prompt_split_kernel(const Promp
   }
   low_channel = __reduce_min_sync(0xffffffffu, low_channel);
   const int top = top_bits;
-  const bool marked = top >= 0x7f800000 || (top > 0 && 2 * (top >> 23) - (low_row >> 23) - (low_channel >> 23) > kMostSpread);
+  const int spread = 2 * (top >> 23) - (low_row >> 23) - (low_channel >> 23);
+  const bool marked = top >= 0x7f800000 || (top > 0 && spread > kMostSpread);
   const int e = pow2_ex(__int_as_float(top));
   const float down = pow2f(-e);
 #pragma unroll
@@ -767,7 +767,8 @@ __global__ void __launch_bounds__(Cfg<DP, CTAS>::kThreads, CTAS)
 #pragma unroll 4
             for (int d = 0; d < a.head_dim; d += 4) {
               const float4 x = *reinterpret_cast<const float4*>(qr + d);
-              const float4 y = *reinterpret_cast<const float4*>(kr + d), z = *reinterpret_cast<const float4*>(kr + k_next + d);
+              const float4 y = *reinterpret_cast<const float4*>(kr + d);
+              const float4 z = *reinterpret_cast<const float4*>(kr + k_next + d);
               s0 = fmaf(x.w, y.w, fmaf(x.z, y.z, fmaf(x.y, y.y, fmaf(x.x, y.x, s0))));
               s1 = fmaf(x.w, z.w, fmaf(x.z, z.z, fmaf(x.y, z.y, fmaf(x.x, z.x, s1))));
             }

@@ -250,9 +250,9 @@ __global__ void __launch_bounds__(kRowThreads) kv_q40_read_kernel(const RowsArgs
 // of w come from p = ph + pl and d in fp16 arithmetic: hi = ph d, lo = (ph d -
 // hi) + pl d, whose first part a fused multiply-add leaves exact.  Terms end at
 // 2^-24, so a w that is small beside the largest p times the largest d (at least 2^8)
-// is off by 2^-32 of that rather than by 2^-22 of itself.  Blocks' scales far apart (2^10) would
-// need a power of two for each block; that was built and took 16 columns of 65536
-// positions from 167 to 170 us, for values that f32 rows seldom hold.
+// is off by 2^-32 of that rather than by 2^-22 of itself.  Blocks' scales far apart
+// (2^10) would need a power of two for each block; that was built and took 16 columns
+// of 65536 positions from 167 to 170 us, for values that f32 rows seldom hold.
 //
 // A code becomes a half by one AND/OR, (w & 0x000f) | 0x6400 = 1024 + n, and
 // one addition that centres it: n - 8 (16 (n - 8) from a high nibble; for a key
@@ -267,8 +267,8 @@ __global__ void __launch_bounds__(kRowThreads) kv_q40_read_kernel(const RowsArgs
 // time to the products'.  So it is bound by its instructions: 167 us for 16 columns
 // of 65536 positions, 28 / 4 heads of 128 (3.6 TB/s, 56% of the measured copy rate;
 // 180 us at 1860 MHz in a run of seconds, at the power limit); 64 ragged columns up
-// to 2048 21 us (23 with the cache not in L2), 1 x 32768 14.7 us (16).  3 CTAs an SM with 168 registers: 4 with 128 took
-// 184 us for 168.
+// to 2048 21 us (23 with the cache not in L2), 1 x 32768 14.7 us (16).  3 CTAs an SM
+// with 168 registers: 4 with 128 took 184 us for 168.
 //
 // Work: the positions of all columns and heads form one list of units, kExtra
 // for each (column, group), what its start and end cost, and one for each of
@@ -509,9 +509,10 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm)
   if (tid == kThreads - 1) {
     Piece x = p;
     for (int64_t at = group0, r = u;;) {
-      if (x.ch0 == 0)
+      const int chunks = chunks_of(x.len);
+      if (x.ch0 == 0)  // only the last one can go on in other runs
         a.spans[(int64_t)x.col * a.subs + x.sub] =
-            make_int2(blockIdx.x, cta_of(at + kExtra + chunks_of(x.len) - 1, total, n_ctas));
+            make_int2(blockIdx.x, x.take == chunks ? blockIdx.x : cta_of(at + kExtra + chunks - 1, total, n_ctas));
       if (r >= u1) break;
       if (++x.sub == a.subs) {
         x.sub = 0;
@@ -1053,11 +1054,11 @@ extern "C" size_t dqmk_kv_q40_attention_workspace(const dqmk_kv_q40* kv, int n_c
 
 namespace {
 
-int attention_call(const char* name, const dqmk_kv_q40* kv, int layer, const float* q, int64_t ldq,
-                   const int* slots, const int* lengths, int n_cols, int n_heads, float* out,
-                   int64_t ldo, void* workspace, size_t workspace_bytes, int withhold_col,
-                   int withhold_tile, void* stream) {
-  const std::string api = name;
+int attention_call(const dqmk_kv_q40* kv, int layer, const float* q, int64_t ldq, const int* slots,
+                   const int* lengths, int n_cols, int n_heads, float* out, int64_t ldo,
+                   void* workspace, size_t workspace_bytes, int withhold_col, int withhold_tile,
+                   void* stream) {
+  const std::string api = "KvQ40Attention";
   AttnQ40Args a = {};
   int rc = check_cache(api, kv, layer, &a.c);
   if (rc) return rc;
@@ -1112,8 +1113,8 @@ extern "C" int dqmk_kv_q40_attention(const dqmk_kv_q40* kv, int layer, const flo
                                      const int* slots, const int* lengths, int n_cols, int n_heads,
                                      float* out, int64_t ldo, void* workspace,
                                      size_t workspace_bytes, void* stream) {
-  return attention_call("KvQ40Attention", kv, layer, q, ldq, slots, lengths, n_cols, n_heads, out, ldo,
-                        workspace, workspace_bytes, -1, -1, stream);
+  return attention_call(kv, layer, q, ldq, slots, lengths, n_cols, n_heads, out, ldo, workspace,
+                        workspace_bytes, -1, -1, stream);
 }
 
 extern "C" int dqmk_kv_q40_attention_withhold_tile(const dqmk_kv_q40* kv, int layer, const float* q,
@@ -1121,6 +1122,6 @@ extern "C" int dqmk_kv_q40_attention_withhold_tile(const dqmk_kv_q40* kv, int la
                                                    int n_cols, int n_heads, float* out, int64_t ldo,
                                                    void* workspace, size_t workspace_bytes, int column,
                                                    int tile, void* stream) {
-  return attention_call("KvQ40Attention", kv, layer, q, ldq, slots, lengths, n_cols, n_heads, out, ldo,
-                        workspace, workspace_bytes, column, tile, stream);
+  return attention_call(kv, layer, q, ldq, slots, lengths, n_cols, n_heads, out, ldo, workspace,
+                        workspace_bytes, column, tile, stream);
 }
